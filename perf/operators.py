@@ -9,6 +9,8 @@ generic odd sizes.
 """
 
 import math
+import os
+import sys
 
 import torch
 
@@ -323,6 +325,9 @@ def _plain_embed(st):
 # -------------------------------------------------------------------------------- the framework's
 
 def _run_own(st):
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pararnn-torch_b200")
+    if root not in sys.path:  # the package is not installed, it lies below the repository's root
+        sys.path.insert(0, root)
     import pararnn_b200 as prb
 
     if st["op"] == "prefill":
