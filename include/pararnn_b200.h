@@ -404,6 +404,76 @@ int prb_bwd_nlru_static(const void* states, const void* wx, const void* u, const
                         const void* grad_states, void* g_wx, float* g_params, float* g_h0, int B,
                         int T, int d, int dtype, prb_stats* stats, prb_stream_t stream);
 
+/* ---- token-model operators ------------------------------------------------------------ */
+
+/* A (rows, time, heads, channels) device array with unit channel stride; strides in elements. */
+typedef struct prb_heads {
+    const void* data;
+    long long stride_b, stride_t, stride_h;
+} prb_heads;
+
+/* Linear attention with a decay for each head:  S_t = w S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t,
+ * w = exp(log_decay[h]), log_decay <= 0 (-inf: no memory).  No counterpart in the reference (its
+ * matrix-state cells are cells/para_m2rnn.py and cells/para_rwkv7.py).
+ *   q (rows,time,q_heads,dk); k (..,kv_heads,dk); v (..,kv_heads,dv) in `dtype`; dk, dv in 1..128;
+ *   q_heads a multiple of kv_heads, query head h reads state head h / (q_heads / kv_heads);
+ *   log_decay fp32 (kv_heads); state_in / state_out fp32 (n_seq,kv_heads,dk,dv) or NULL;
+ *   out (rows,time,q_heads,dv) contiguous in `dtype`.
+ * cu_seqlens NULL: n_seq = rows sequences of `time` tokens.  Otherwise a packed batch: rows = 1 and
+ * n_seq + 1 device int32 offsets; offsets outside [0, time] or out of order are clamped, and a
+ * sequence without tokens passes its state through.  max_len bounds the sequences' lengths.
+ * Tokens behind the last sequence are neither read nor written.  Values at later positions never
+ * reach earlier outputs, not even when they are inf or NaN. */
+size_t prb_linear_attention_workspace_bytes(int rows, int time, int n_seq, int max_len, int q_heads, int kv_heads,
+                                            int dk, int dv, int dtype, int packed, int backward);
+int prb_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads* v, const float* log_decay,
+                         const float* state_in, const int* cu_seqlens, void* out, float* state_out, int rows,
+                         int time, int n_seq, int max_len, int q_heads, int kv_heads, int dk, int dv, int dtype,
+                         float scale, void* workspace, size_t workspace_bytes, prb_stream_t stream);
+
+/* Gradients from grad_out (same layout rules as q) and grad_state_out (fp32, NULL = zeros): g_q, g_k,
+ * g_v contiguous in `dtype` (g_k, g_v summed over the query heads that share them), g_state fp32 or
+ * NULL.  log_decay is a constant of the head. */
+int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads* v, const prb_heads* grad_out,
+                             const float* log_decay, const float* state_in, const float* grad_state_out,
+                             const int* cu_seqlens, void* g_q, void* g_k, void* g_v, float* g_state, int rows,
+                             int time, int n_seq, int max_len, int q_heads, int kv_heads, int dk, int dv, int dtype,
+                             float scale, void* workspace, size_t workspace_bytes, prb_stream_t stream);
+
+/* One token per row on a pool of fp32 states (slots,kv_heads,dk,dv), updated in place.  q (rows,q_heads,dk),
+ * k (rows,kv_heads,dk), v (rows,kv_heads,dv), out (rows,q_heads,dv) contiguous.  block_table (int32 or
+ * int64, NULL = row r uses slot r): a slot outside [0, slots) marks a padding row, which touches no
+ * state and gives zeros; a slot named by several rows takes them in row order. */
+int prb_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, float* state,
+                              const void* block_table, int table_is_int64, void* out, int rows, int slots, int q_heads,
+                              int kv_heads, int dk, int dv, int dtype, float scale, prb_stream_t stream);
+
+/* Group norm with an activation over channel-last x (samples,positions,channels): the statistics of
+ * channels / groups neighbouring channels over all positions of a sample, biased variance,
+ * y = act(xhat weight + bias).  weight / bias (channels) in weight_dtype or NULL; stats fp32
+ * (samples,groups,2) = mean, 1/sqrt(var + eps), NULL to drop them; x, y, grad_y, g_x 16-byte aligned.
+ * g_weight / g_bias (in weight_dtype, NULL to drop them) are summed in a fixed order. */
+enum { PRB_ACT_NONE = 0, PRB_ACT_SILU = 1, PRB_ACT_GELU = 2 };
+size_t prb_group_norm_workspace_bytes(long long samples, int positions, int channels, int groups, int dtype,
+                                      int backward);
+int prb_group_norm(const void* x, const void* weight, const void* bias, void* y, float* stats, long long samples,
+                   int positions, int channels, int groups, float eps, int activation, int dtype, int weight_dtype,
+                   void* workspace, size_t workspace_bytes, prb_stream_t stream);
+int prb_bwd_group_norm(const void* x, const void* grad_y, const void* weight, const void* bias, const float* stats,
+                       void* g_x, void* g_weight, void* g_bias, long long samples, int positions, int channels,
+                       int groups, int activation, int dtype, int weight_dtype, void* workspace,
+                       size_t workspace_bytes, prb_stream_t stream);
+
+/* Embedding lookup out_t = scale table[id_t] and its dense gradient g_table[v] = scale sum_{id_t = v}
+ * grad_out_t, added in fp32 in the order of the positions.  ids int32 or int64 (tokens); an id outside
+ * [0, vocab) gives a row of zeros and takes part in no gradient.  Every row of g_table is written. */
+int prb_embedding(const void* ids, int ids_is_int64, const void* table, void* out, long long tokens, int vocab,
+                  int channels, int dtype, float scale, prb_stream_t stream);
+size_t prb_bwd_embedding_workspace_bytes(long long tokens, int vocab, int channels);
+int prb_bwd_embedding(const void* ids, int ids_is_int64, const void* grad_out, void* g_table, long long tokens,
+                      int vocab, int channels, int dtype, float scale, void* workspace, size_t workspace_bytes,
+                      prb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,652 @@
+// Group norm with an activation over channel-last tensors (samples, positions, channels), forward and
+// backward:  y = act(xhat w + b),  xhat = (x - mean) rstd,  statistics of a group of channels over all
+// positions of a sample.  With one position per sample this is the norm over each head's channels
+// behind a sequence mixer.
+//
+//   du = dy act'(xhat w + b);  dx = rstd (w du - mean(w du) - xhat mean(w du xhat));
+//   dw = sum du xhat;  db = sum du
+//
+// Everything is HBM-bound (2 resp. 3 passes over the data against some 30 flops per element), so the
+// kernels are about touching memory once:
+//   rows   one position, groups up to 32 lanes x 4 vectors: a group sits in the registers of 1 - 32
+//          lanes, mean and variance are two register passes, the data moves exactly once.
+//   slabs  everything else: a first launch leaves each slab's (mean, M2) or (sum du, sum du xhat) per
+//          group, a second one merges them and writes the result; it finds the data still in L2
+//          because the host walks the samples in pieces of at most kPieceBytes.
+// Variances are merged as (count, mean, M2), never as sums of squares, and all partial sums are
+// added in a fixed order, so results repeat bit for bit.
+#include "groupnorm.cuh"
+
+namespace prb {
+
+namespace {
+
+constexpr int kT = 256;
+constexpr int kMaxLocal = kT + 2;  // groups that one CTA's channels can touch
+
+template <typename T, int V>
+struct __align__(sizeof(T) * V) Pack {
+    T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ void load_v(float (&r)[V], const T* p) {
+    const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = static_cast<float>(u.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const float (&r)[V]) {
+    Pack<T, V> u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) st_f(&u.v[i], r[i]);
+    *reinterpret_cast<Pack<T, V>*>(p) = u;
+}
+__device__ __forceinline__ float affine(const void* p, int f32, int i, float none) {
+    if (!p) return none;
+    return f32 ? __ldg(reinterpret_cast<const float*>(p) + i)
+               : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p) + i));
+}
+
+template <int ACT>
+__device__ __forceinline__ float act(float u) {
+    if constexpr (ACT == kActSilu) return u * sigmoid_f(u);
+    if constexpr (ACT == kActGelu) return u * normcdff(u);
+    return u;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float u) {
+    if constexpr (ACT == kActSilu) {
+        const float s = sigmoid_f(u);
+        return s * fmaf(u, 1.f - s, 1.f);
+    }
+    if constexpr (ACT == kActGelu) return fmaf(u, 0.3989422804014327f * expf(-0.5f * u * u), normcdff(u));
+    return 1.f;
+}
+
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// ---------------------------------------------------------------------------------------- rows
+// Thread slots: LANES lanes per group, NV vectors of V channels per lane; a CTA holds kT / slots
+// rows at a time (or a 256-slot piece of a wide row, blockIdx.y).
+struct RowSlot {
+    int g, sub, lane, rows;
+    bool live;
+};
+template <int LANES>
+__device__ __forceinline__ RowSlot row_slot(int groups) {
+    RowSlot r;
+    const int slots = groups * LANES;
+    const int wide = slots > kT;
+    const int per = wide ? kT : slots;
+    r.rows = kT / per;
+    r.sub = threadIdx.x / per;
+    const int slot = threadIdx.x % per + blockIdx.y * kT;
+    r.g = slot / LANES;
+    r.lane = slot % LANES;
+    r.live = r.sub < r.rows && r.g < groups;
+    return r;
+}
+
+template <typename T, int V, int NV, int LANES, int ACT>
+__global__ void __launch_bounds__(kT) gn_rows_fwd(const __grid_constant__ GroupNormArgs p) {
+    const RowSlot rs = row_slot<LANES>(p.groups);
+    const int cg = p.channels / p.groups;
+    float w[NV][V], b[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (j * LANES + rs.lane) * V + i;
+            const bool in = rs.live && c < cg;
+            w[j][i] = in ? affine(p.w, p.w_f32, rs.g * cg + c, 1.f) : 0.f;
+            b[j][i] = in ? affine(p.b, p.w_f32, rs.g * cg + c, 0.f) : 0.f;
+        }
+    const float inv = 1.f / cg;
+    for (long long r0 = (long long)blockIdx.x * rs.rows; r0 < p.samples; r0 += (long long)gridDim.x * rs.rows) {
+        const long long row = r0 + rs.sub;
+        const bool live = rs.live && row < p.samples;
+        const size_t at = (size_t)row * p.channels + (size_t)rs.g * cg;
+        float x[NV][V];
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * LANES + rs.lane) * V;
+            if (live && c < cg) {
+                load_v<T, V>(x[j], reinterpret_cast<const T*>(p.x) + at + c);
+#pragma unroll
+                for (int i = 0; i < V; ++i) s += x[j][i];
+            }
+        }
+        const float mean = lane_sum<LANES>(s) * inv;
+        float m2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (live && (j * LANES + rs.lane) * V < cg) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = x[j][i] - mean;
+                    m2 = fmaf(d, d, m2);
+                }
+            }
+        const float rstd = rsqrtf(lane_sum<LANES>(m2) * inv + p.eps);
+        if (!live) continue;
+        if (rs.lane == 0 && p.stats) p.stats[(size_t)row * p.groups + rs.g] = make_float2(mean, rstd);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * LANES + rs.lane) * V;
+            if (c >= cg) continue;
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[i] = act<ACT>(fmaf((x[j][i] - mean) * rstd, w[j][i], b[j][i]));
+            store_v<T, V>(reinterpret_cast<T*>(p.y) + at + c, y);
+        }
+    }
+}
+
+template <typename T, int V, int NV, int LANES, int ACT>
+__global__ void __launch_bounds__(kT) gn_rows_bwd(const __grid_constant__ GroupNormArgs p) {
+    const RowSlot rs = row_slot<LANES>(p.groups);
+    const int cg = p.channels / p.groups;
+    float w[NV][V], b[NV][V], dw[NV][V] = {}, db[NV][V] = {};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (j * LANES + rs.lane) * V + i;
+            const bool in = rs.live && c < cg;
+            w[j][i] = in ? affine(p.w, p.w_f32, rs.g * cg + c, 1.f) : 0.f;
+            b[j][i] = in ? affine(p.b, p.w_f32, rs.g * cg + c, 0.f) : 0.f;
+        }
+    const float inv = 1.f / cg;
+    for (long long r0 = (long long)blockIdx.x * rs.rows; r0 < p.samples; r0 += (long long)gridDim.x * rs.rows) {
+        const long long row = r0 + rs.sub;
+        const bool live = rs.live && row < p.samples;
+        const size_t at = (size_t)row * p.channels + (size_t)rs.g * cg;
+        float2 st = make_float2(0.f, 0.f);
+        if (live) st = p.stats[(size_t)row * p.groups + rs.g];
+        float h[NV][V], d[NV][V];  // xhat, then w du
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * LANES + rs.lane) * V;
+            if (live && c < cg) {
+                load_v<T, V>(h[j], reinterpret_cast<const T*>(p.x) + at + c);
+                load_v<T, V>(d[j], reinterpret_cast<const T*>(p.dy) + at + c);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (live && (j * LANES + rs.lane) * V < cg) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    h[j][i] = (h[j][i] - st.x) * st.y;
+                    const float du = d[j][i] * act_slope<ACT>(fmaf(h[j][i], w[j][i], b[j][i]));
+                    dw[j][i] = fmaf(du, h[j][i], dw[j][i]);
+                    db[j][i] += du;
+                    d[j][i] = du * w[j][i];
+                    s1 += d[j][i];
+                    s2 = fmaf(d[j][i], h[j][i], s2);
+                }
+            }
+        }
+        s1 = lane_sum<LANES>(s1) * inv;
+        s2 = lane_sum<LANES>(s2) * inv;
+        if (!live) continue;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * LANES + rs.lane) * V;
+            if (c >= cg) continue;
+            float dx[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) dx[i] = st.y * (d[j][i] - s1 - h[j][i] * s2);
+            store_v<T, V>(reinterpret_cast<T*>(p.dx) + at + c, dx);
+        }
+    }
+    // one row of partial sums per CTA: its rows in order of `sub`
+    __shared__ float red[2][kT][V];
+    const int slots = min(kT, p.groups * LANES);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            red[0][threadIdx.x][i] = dw[j][i];
+            red[1][threadIdx.x][i] = db[j][i];
+        }
+        __syncthreads();
+        const int c = (j * LANES + rs.lane) * V;
+        if (rs.live && rs.sub == 0 && c < cg) {
+            float* dst = p.partial + (size_t)blockIdx.x * 2 * p.channels + rs.g * cg + c;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float a0 = 0.f, a1 = 0.f;
+                for (int k = 0; k < rs.rows; ++k) {
+                    a0 += red[0][threadIdx.x + k * slots][i];
+                    a1 += red[1][threadIdx.x + k * slots][i];
+                }
+                dst[i] = a0;
+                dst[p.channels + i] = a1;
+            }
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------- slabs
+// blockIdx = (slab of positions, sample, block of kT * V channels).  A thread keeps one vector of V
+// channels (all of one group) and walks the slab's positions.
+struct SlabSlot {
+    int c, g, sub, rows, p0, p1;
+    bool live;
+};
+template <int V>
+__device__ __forceinline__ SlabSlot slab_slot(const GroupNormArgs& p) {
+    SlabSlot s;
+    const int slots = p.channels / V;
+    const int per = min(slots, kT);
+    s.rows = kT / per;
+    s.sub = threadIdx.x / per;
+    const int slot = threadIdx.x % per + blockIdx.z * kT;
+    s.c = slot * V;
+    s.live = s.sub < s.rows && slot < slots;
+    s.g = s.live ? s.c / (p.channels / p.groups) : 0;
+    s.p0 = (int)((long long)blockIdx.x * p.positions / p.slabs);
+    s.p1 = (int)((long long)(blockIdx.x + 1) * p.positions / p.slabs);
+    return s;
+}
+__device__ __forceinline__ void chan(float& n, float& mean, float& m2, float n2, float mean2, float m22) {
+    const float t = n + n2;
+    if (t == 0.f) return;
+    const float d = mean2 - mean, f = n2 / t;
+    mean = fmaf(d, f, mean);
+    m2 += m22 + d * d * n * f;
+    n = t;
+}
+__device__ __forceinline__ void warp_chan(float& n, float& mean, float& m2) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float n2 = __shfl_xor_sync(0xffffffffu, n, o), a = __shfl_xor_sync(0xffffffffu, mean, o),
+                    b = __shfl_xor_sync(0xffffffffu, m2, o);
+        // both lanes of a pair compute the same merge: order the operands by lane
+        if (threadIdx.x & o) {
+            float nn = n2, aa = a, bb = b;
+            chan(nn, aa, bb, n, mean, m2);
+            n = nn, mean = aa, m2 = bb;
+        } else {
+            chan(n, mean, m2, n2, a, b);
+        }
+    }
+}
+// groups that this CTA's channels touch
+template <int V>
+__device__ __forceinline__ void local_groups(const GroupNormArgs& p, int& lo, int& n) {
+    const int cg = p.channels / p.groups;
+    lo = blockIdx.z * kT * V / cg;
+    n = (min(p.channels, (int)(blockIdx.z + 1) * kT * V) - 1) / cg - lo + 1;
+}
+// channel blocks that hold a piece of group g
+template <int V>
+__device__ __forceinline__ void group_blocks(const GroupNormArgs& p, int g, int& lo, int& n) {
+    const int cg = p.channels / p.groups;
+    lo = g * cg / (kT * V);
+    n = (g * cg + cg - 1) / (kT * V) - lo + 1;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kT) gn_slab_stats(const __grid_constant__ GroupNormArgs p) {
+    __shared__ float sn[kT], sm[kT], sv[kT];
+    const SlabSlot s = slab_slot<V>(p);
+    const size_t n = p.sample0 + blockIdx.y;
+    const T* x = reinterpret_cast<const T*>(p.x) + n * p.positions * p.channels + s.c;
+    // sums about the thread's first value, so that a large mean cancels nothing
+    float pivot = 0.f, s1 = 0.f, s2 = 0.f, cnt = 0.f;
+    if (s.live && s.p0 + s.sub < s.p1) {
+        float v[V];
+        load_v<T, V>(v, x + (size_t)(s.p0 + s.sub) * p.channels);
+        pivot = v[0];
+#pragma unroll 4
+        for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
+            load_v<T, V>(v, x + (size_t)q * p.channels);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = v[i] - pivot;
+                s1 += d;
+                s2 = fmaf(d, d, s2);
+            }
+            cnt += V;
+        }
+    }
+    const float m = cnt > 0.f ? s1 / cnt : 0.f;
+    sn[threadIdx.x] = cnt;
+    sm[threadIdx.x] = pivot + m;
+    sv[threadIdx.x] = cnt > 0.f ? fmaxf(s2 - s1 * m, 0.f) + 0.f * s2 : 0.f;
+    __syncthreads();
+    int g0, ng;
+    local_groups<V>(p, g0, ng);
+    const int cg = p.channels / p.groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per = min(p.channels / V, kT);
+    for (int k = warp; k < ng; k += kT / 32) {
+        const int g = g0 + k;
+        const int lo = max(0, g * cg / V - (int)blockIdx.z * kT), hi = min(per, (g + 1) * cg / V - (int)blockIdx.z * kT);
+        const int width = hi - lo, total = width * s.rows;
+        float cn = 0.f, cm = 0.f, cv = 0.f;
+        for (int t = lane; t < total; t += 32) {
+            const int id = (t / width) * per + lo + t % width;
+            chan(cn, cm, cv, sn[id], sm[id], sv[id]);
+        }
+        warp_chan(cn, cm, cv);
+        if (lane == 0)
+            reinterpret_cast<float4*>(p.group_part)[((n * p.slabs + blockIdx.x) * gridDim.z + blockIdx.z) * p.groups + g] =
+                make_float4(cn, cm, cv, 0.f);
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kT) gn_slab_fwd(const __grid_constant__ GroupNormArgs p) {
+    __shared__ float2 st[kMaxLocal];
+    const SlabSlot s = slab_slot<V>(p);
+    const size_t n = p.sample0 + blockIdx.y;
+    int g0, ng;
+    local_groups<V>(p, g0, ng);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int k = warp; k < ng; k += kT / 32) {
+        int b0, nb;
+        group_blocks<V>(p, g0 + k, b0, nb);
+        float cn = 0.f, cm = 0.f, cv = 0.f;
+        for (int t = lane; t < p.slabs * nb; t += 32) {
+            const float4 u = reinterpret_cast<const float4*>(
+                p.group_part)[((n * p.slabs + t / nb) * gridDim.z + b0 + t % nb) * p.groups + g0 + k];
+            chan(cn, cm, cv, u.x, u.y, u.z);
+        }
+        warp_chan(cn, cm, cv);
+        if (lane == 0) {
+            const float2 r = make_float2(cm, rsqrtf(cv / cn + p.eps));
+            st[k] = r;
+            if (blockIdx.x == 0 && p.stats && b0 == (int)blockIdx.z) p.stats[n * p.groups + g0 + k] = r;
+        }
+    }
+    __syncthreads();
+    if (!s.live) return;
+    const float2 ms = st[s.g - g0];
+    float w[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        w[i] = affine(p.w, p.w_f32, s.c + i, 1.f);
+        b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
+    }
+    const size_t base = n * p.positions * p.channels + s.c;
+#pragma unroll 4
+    for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
+        float v[V];
+        load_v<T, V>(v, reinterpret_cast<const T*>(p.x) + base + (size_t)q * p.channels);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = act<ACT>(fmaf((v[i] - ms.x) * ms.y, w[i], b[i]));
+        store_v<T, V>(reinterpret_cast<T*>(p.y) + base + (size_t)q * p.channels, v);
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kT) gn_slab_sums(const __grid_constant__ GroupNormArgs p) {
+    __shared__ float red[2][kT][V];
+    __shared__ float gs[2][kT];
+    const SlabSlot s = slab_slot<V>(p);
+    const size_t n = p.sample0 + blockIdx.y;
+    float w[V], b[V], dw[V] = {}, db[V] = {};
+    const size_t base = n * p.positions * p.channels + s.c;
+    if (s.live) {
+        const float2 ms = p.stats[n * p.groups + s.g];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            w[i] = affine(p.w, p.w_f32, s.c + i, 1.f);
+            b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
+        }
+#pragma unroll 2
+        for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
+            float h[V], d[V];
+            load_v<T, V>(h, reinterpret_cast<const T*>(p.x) + base + (size_t)q * p.channels);
+            load_v<T, V>(d, reinterpret_cast<const T*>(p.dy) + base + (size_t)q * p.channels);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                h[i] = (h[i] - ms.x) * ms.y;
+                const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
+                dw[i] = fmaf(du, h[i], dw[i]);
+                db[i] += du;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        red[0][threadIdx.x][i] = dw[i];
+        red[1][threadIdx.x][i] = db[i];
+    }
+    __syncthreads();
+    const int per = min(p.channels / V, kT);
+    float t1 = 0.f, t2 = 0.f;  // sum of w du, of w du xhat over this thread's channels
+    if (s.live && s.sub == 0) {
+        float* dst = p.partial + ((n * p.slabs + blockIdx.x) * 2) * p.channels + s.c;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float a0 = 0.f, a1 = 0.f;
+            for (int k = 0; k < s.rows; ++k) {
+                a0 += red[0][threadIdx.x + k * per][i];
+                a1 += red[1][threadIdx.x + k * per][i];
+            }
+            dst[i] = a0;
+            dst[p.channels + i] = a1;
+            t1 = fmaf(w[i], a1, t1);
+            t2 = fmaf(w[i], a0, t2);
+        }
+    }
+    gs[0][threadIdx.x] = t1;
+    gs[1][threadIdx.x] = t2;
+    __syncthreads();
+    int g0, ng;
+    local_groups<V>(p, g0, ng);
+    const int cg = p.channels / p.groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int k = warp; k < ng; k += kT / 32) {
+        const int g = g0 + k;
+        const int lo = max(0, g * cg / V - (int)blockIdx.z * kT), hi = min(per, (g + 1) * cg / V - (int)blockIdx.z * kT);
+        float a = 0.f, c = 0.f;
+        for (int t = lo + lane; t < hi; t += 32) {
+            a += gs[0][t];
+            c += gs[1][t];
+        }
+        a = lane_sum<32>(a);
+        c = lane_sum<32>(c);
+        if (lane == 0)
+            reinterpret_cast<float4*>(p.group_part)[((n * p.slabs + blockIdx.x) * gridDim.z + blockIdx.z) * p.groups + g] =
+                make_float4(a, c, 0.f, 0.f);
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kT) gn_slab_bwd(const __grid_constant__ GroupNormArgs p) {
+    __shared__ float2 st[kMaxLocal];
+    const SlabSlot s = slab_slot<V>(p);
+    const size_t n = p.sample0 + blockIdx.y;
+    int g0, ng;
+    local_groups<V>(p, g0, ng);
+    const int cg = p.channels / p.groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float inv = 1.f / ((float)cg * (float)p.positions);
+    for (int k = warp; k < ng; k += kT / 32) {
+        int b0, nb;
+        group_blocks<V>(p, g0 + k, b0, nb);
+        float a = 0.f, c = 0.f;
+        for (int t = lane; t < p.slabs * nb; t += 32) {
+            const float4 u = reinterpret_cast<const float4*>(
+                p.group_part)[((n * p.slabs + t / nb) * gridDim.z + b0 + t % nb) * p.groups + g0 + k];
+            a += u.x;
+            c += u.y;
+        }
+        a = lane_sum<32>(a);
+        c = lane_sum<32>(c);
+        if (lane == 0) st[k] = make_float2(a * inv, c * inv);
+    }
+    __syncthreads();
+    if (!s.live) return;
+    const float2 ms = p.stats[n * p.groups + s.g], sums = st[s.g - g0];
+    float w[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        w[i] = affine(p.w, p.w_f32, s.c + i, 1.f);
+        b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
+    }
+    const size_t base = n * p.positions * p.channels + s.c;
+#pragma unroll 2
+    for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
+        float h[V], d[V];
+        load_v<T, V>(h, reinterpret_cast<const T*>(p.x) + base + (size_t)q * p.channels);
+        load_v<T, V>(d, reinterpret_cast<const T*>(p.dy) + base + (size_t)q * p.channels);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            h[i] = (h[i] - ms.x) * ms.y;
+            const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
+            d[i] = ms.y * (fmaf(du, w[i], -sums.x) - h[i] * sums.y);
+        }
+        store_v<T, V>(reinterpret_cast<T*>(p.dx) + base + (size_t)q * p.channels, d);
+    }
+}
+
+// dw, db: sums of the partial rows, 32 channels x 32 strides of rows per CTA, added in a fixed order
+__global__ void __launch_bounds__(1024) gn_reduce(const float* part, long long rows, int channels, void* dw, void* db,
+                                                  int w_f32) {
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, k = threadIdx.x >> 5;
+    const float* src = part + (size_t)blockIdx.y * channels;
+    float s = 0.f;
+    if (c < channels) {
+#pragma unroll 8
+        for (long long r = k; r < rows; r += 32) s += src[(size_t)r * 2 * channels + c];
+    }
+    red[k][lane] = s;
+    __syncthreads();
+    void* dst = blockIdx.y == 0 ? dw : db;
+    if (k != 0 || c >= channels || !dst) return;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += red[i][lane];
+    if (w_f32) reinterpret_cast<float*>(dst)[c] = t;
+    else st_f(reinterpret_cast<__nv_bfloat16*>(dst) + c, t);
+}
+
+// ---------------------------------------------------------------------------------------- host
+constexpr long long kPieceBytes = 48ll << 20;  // half of L2: what a second pass still finds there
+
+template <typename T, int V, int NV, int LANES, int ACT>
+cudaError_t rows_t(const GroupNormArgs& a, bool backward, cudaStream_t s) {
+    const dim3 grid(a.slabs, (a.groups * LANES + kT - 1) / kT);
+    if (backward) gn_rows_bwd<T, V, NV, LANES, ACT><<<grid, kT, 0, s>>>(a);
+    else gn_rows_fwd<T, V, NV, LANES, ACT><<<grid, kT, 0, s>>>(a);
+    return cudaGetLastError();
+}
+template <typename T, int V, int ACT>
+cudaError_t rows_v(const GroupNormArgs& a, const GroupNormPlan& pl, bool backward, cudaStream_t s) {
+    if constexpr (V > 1) {
+        if (pl.nv == 4) return rows_t<T, V, 4, 32, ACT>(a, backward, s);
+        if (pl.nv == 2) return rows_t<T, V, 2, 32, ACT>(a, backward, s);
+    }
+    switch (pl.lanes) {
+        case 1: return rows_t<T, V, 1, 1, ACT>(a, backward, s);
+        case 2: return rows_t<T, V, 1, 2, ACT>(a, backward, s);
+        case 4: return rows_t<T, V, 1, 4, ACT>(a, backward, s);
+        case 8: return rows_t<T, V, 1, 8, ACT>(a, backward, s);
+        case 16: return rows_t<T, V, 1, 16, ACT>(a, backward, s);
+        default: return rows_t<T, V, 1, 32, ACT>(a, backward, s);
+    }
+}
+template <typename T, int V, int ACT>
+cudaError_t slabs_v(GroupNormArgs a, const GroupNormPlan& pl, bool backward, cudaStream_t s) {
+    const long long per = (long long)a.positions * a.channels * sizeof(T) * (backward ? 2 : 1);
+    long long step = kPieceBytes / per;
+    step = step < 1 ? 1 : step > 65535 ? 65535 : step;
+    for (long long n0 = 0; n0 < a.samples; n0 += step) {
+        const long long n = a.samples - n0 < step ? a.samples - n0 : step;
+        const dim3 grid(a.slabs, (unsigned)n, pl.blocks);
+        a.sample0 = n0;
+        if (backward) {
+            gn_slab_sums<T, V, ACT><<<grid, kT, 0, s>>>(a);
+            gn_slab_bwd<T, V, ACT><<<grid, kT, 0, s>>>(a);
+        } else {
+            gn_slab_stats<T, V><<<grid, kT, 0, s>>>(a);
+            gn_slab_fwd<T, V, ACT><<<grid, kT, 0, s>>>(a);
+        }
+    }
+    return cudaGetLastError();
+}
+template <typename T, int V>
+cudaError_t run_v(const GroupNormArgs& a, const GroupNormPlan& pl, bool backward, cudaStream_t s) {
+    if (pl.rows) {
+        if (a.act == kActSilu) return rows_v<T, V, kActSilu>(a, pl, backward, s);
+        if (a.act == kActGelu) return rows_v<T, V, kActGelu>(a, pl, backward, s);
+        return rows_v<T, V, kActNone>(a, pl, backward, s);
+    }
+    if (a.act == kActSilu) return slabs_v<T, V, kActSilu>(a, pl, backward, s);
+    if (a.act == kActGelu) return slabs_v<T, V, kActGelu>(a, pl, backward, s);
+    return slabs_v<T, V, kActNone>(a, pl, backward, s);
+}
+
+}  // namespace
+
+// A pure function of the shape, so that the size query and the launch agree.
+GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int channels, int groups) {
+    GroupNormPlan pl{};
+    const int cg = channels / groups, most = dtype == kF32 ? 4 : 8;
+    // vectors of 16 bytes where a group holds whole ones, else of 2, else single channels
+    pl.vec = cg % most == 0 ? most : cg % 2 == 0 ? 2 : 1;
+    const int sm = sm_count();
+    if (positions == 1 && cg <= pl.vec * 32 * (pl.vec > 1 ? 4 : 1)) {
+        pl.rows = 1;
+        const int need = (cg + pl.vec - 1) / pl.vec;
+        pl.lanes = 1;
+        while (pl.lanes < need && pl.lanes < 32) pl.lanes *= 2;
+        pl.nv = need <= 32 ? 1 : need <= 64 ? 2 : 4;
+        const long long slots = (long long)groups * pl.lanes;
+        const long long at_once = slots >= kT ? 1 : kT / slots;
+        const long long wide = (slots + kT - 1) / kT;
+        // persistent CTAs: 8 per SM keep enough loads in flight, and one partial row each
+        long long ctas = (long long)sm * 8 / wide;
+        const long long full = (samples + at_once - 1) / at_once;
+        ctas = ctas < 1 ? 1 : ctas > full ? full : ctas;
+        pl.slabs = (int)ctas;
+        pl.blocks = (int)wide;
+        pl.part_rows = ctas;
+        return pl;
+    }
+    const int slots = channels / pl.vec, per = slots < kT ? slots : kT;
+    pl.blocks = (slots + kT - 1) / kT;
+    const int at_once = kT / per;
+    // about 4 CTAs per SM over the piece of samples that one launch covers, 8 positions a thread at least
+    const long long bytes = (long long)positions * channels * (dtype == kF32 ? 4 : 2);
+    long long n = kPieceBytes / bytes;
+    n = n < 1 ? 1 : n > samples ? samples : n;
+    long long want = ((long long)sm * 4 + n * pl.blocks - 1) / (n * pl.blocks);
+    const long long room = (positions + 8ll * at_once - 1) / (8ll * at_once);
+    want = want < 1 ? 1 : want > room ? room : want;
+    pl.slabs = (int)want;
+    pl.part_rows = samples * want;
+    pl.group_floats = (size_t)samples * want * pl.blocks * groups * 4;
+    return pl;
+}
+
+cudaError_t launch_groupnorm(const GroupNormArgs& args, int dtype, bool backward, cudaStream_t s) {
+    GroupNormPlan pl = groupnorm_plan(dtype, args.samples, args.positions, args.channels, args.groups);
+    GroupNormArgs a = args;
+    a.slabs = pl.slabs;
+    cudaError_t e;
+    if (dtype == kF32)
+        e = pl.vec == 4 ? run_v<float, 4>(a, pl, backward, s)
+                        : pl.vec == 2 ? run_v<float, 2>(a, pl, backward, s) : run_v<float, 1>(a, pl, backward, s);
+    else
+        e = pl.vec == 8 ? run_v<__nv_bfloat16, 8>(a, pl, backward, s)
+                        : pl.vec == 2 ? run_v<__nv_bfloat16, 2>(a, pl, backward, s)
+                                      : run_v<__nv_bfloat16, 1>(a, pl, backward, s);
+    if (e != cudaSuccess || !backward || (!a.dw && !a.db)) return e;
+    gn_reduce<<<dim3((a.channels + 31) / 32, 2), 1024, 0, s>>>(a.partial, pl.part_rows, a.channels, a.dw, a.db, a.w_f32);
+    return cudaGetLastError();
+}
+
+}  // namespace prb

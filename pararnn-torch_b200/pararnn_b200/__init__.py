@@ -16,8 +16,10 @@ from .config import (
 )
 from .decode import can_decode_step, decode_step, decode_wx
 from .layers import ParaRNN
+from .attn_ops import linear_attention, linear_attention_step
 from .newton import newton_apply
 from .sequential import sequential_apply
+from .token_ops import embedding, group_norm
 from .verify import AgreementError, AgreementReport, default_agreement_atol, verify_agreement
 from . import custom_ops  # noqa: E402,F401  registers torch.ops.pararnn_b200.*
 
@@ -26,6 +28,6 @@ __all__ = [
     "AgreementError", "AgreementReport", "NewtonConfig", "NewtonDivergenceError", "NewtonStats",
     "ParaCfC", "ParaGRU", "ParaLSTM", "ParaNLRU", "ParaRNN", "ParaSLSTM", "ParaTitans", "can_decode_step", "compile_safe_config", "decode_step",
     "decode_wx",
-    "default_agreement_atol", "newton_apply", "sequential_apply", "slstm_auto_picard",
+    "default_agreement_atol", "embedding", "group_norm", "linear_attention", "linear_attention_step", "newton_apply", "sequential_apply", "slstm_auto_picard",
     "slstm_picard_next", "verify_agreement",
 ]

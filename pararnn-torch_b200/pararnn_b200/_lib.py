@@ -25,6 +25,14 @@ _VOIDP = ctypes.c_void_p
 _INT = ctypes.c_int
 _SIZE = ctypes.c_size_t
 _FLOAT = ctypes.c_float
+_LONG = ctypes.c_longlong
+
+
+class Heads(ctypes.Structure):
+    """``prb_heads``: a (rows, time, heads, channels) array with unit channel stride."""
+
+    _fields_ = [("data", _VOIDP), ("stride_b", _LONG), ("stride_t", _LONG), ("stride_h", _LONG)]
+
 
 _SIGNATURES = {
     "prb_version": (ctypes.c_char_p, []),
@@ -68,6 +76,16 @@ _SIGNATURES = {
     "prb_decode_step": (_INT, [_INT, _VOIDP, _VOIDP, _VOIDP, _FLOAT, _VOIDP, _VOIDP, _INT, _INT, _INT, _FLOAT, _VOIDP]),
     "prb_static_scratch_bytes": (_SIZE, []),
     "prb_bwd_nlru_static": (_INT, [_VOIDP] * 8 + [_INT] * 4 + [_VOIDP, _VOIDP]),
+    "prb_linear_attention_workspace_bytes": (_SIZE, [_INT] * 11),
+    "prb_linear_attention": (_INT, [_VOIDP] * 8 + [_INT] * 9 + [_FLOAT, _VOIDP, _SIZE, _VOIDP]),
+    "prb_bwd_linear_attention": (_INT, [_VOIDP] * 12 + [_INT] * 9 + [_FLOAT, _VOIDP, _SIZE, _VOIDP]),
+    "prb_linear_attention_step": (_INT, [_VOIDP] * 6 + [_INT, _VOIDP] + [_INT] * 7 + [_FLOAT, _VOIDP]),
+    "prb_group_norm_workspace_bytes": (_SIZE, [_LONG] + [_INT] * 5),
+    "prb_group_norm": (_INT, [_VOIDP] * 5 + [_LONG] + [_INT] * 3 + [_FLOAT] + [_INT] * 3 + [_VOIDP, _SIZE, _VOIDP]),
+    "prb_bwd_group_norm": (_INT, [_VOIDP] * 8 + [_LONG] + [_INT] * 6 + [_VOIDP, _SIZE, _VOIDP]),
+    "prb_embedding": (_INT, [_VOIDP, _INT, _VOIDP, _VOIDP, _LONG] + [_INT] * 3 + [_FLOAT, _VOIDP]),
+    "prb_bwd_embedding_workspace_bytes": (_SIZE, [_LONG, _INT, _INT]),
+    "prb_bwd_embedding": (_INT, [_VOIDP, _INT, _VOIDP, _VOIDP, _LONG] + [_INT] * 3 + [_FLOAT, _VOIDP, _SIZE, _VOIDP]),
     "prb_residual_pass": (_INT, [_INT] + [_VOIDP] * 4 + [_INT] * 5 + [_FLOAT, _VOIDP, _VOIDP]),
 }
 

@@ -1,0 +1,273 @@
+"""Linear attention with a decay for each head: a matrix-state sequence mixer next to the cells.
+
+``S_t = w S_{t-1} + k_t v_t^T``, ``o_t = scale q_t S_t`` with ``w = exp(log_decay[h])``.  Unlike the
+cells its recurrence is linear in the state, so there is nothing to iterate: one call evaluates the
+whole sequence in chunks, and ``linear_attention_step`` is the single-token form on a pool of states
+(the counterpart of ``decode_step``).  The reference's matrix-state cells are ``cells/para_m2rnn.py``
+and ``cells/para_rwkv7.py``; this mixer has no counterpart there.
+
+``linear_attention`` is differentiable; ``linear_attention_fused`` and
+``linear_attention_reverse_vjp`` are the two operators behind it.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch import Tensor
+
+from . import _lib as L
+from .ops import _check_cuda, _dtype_code, _ptr, _raise, _stream, _workspace, gather_h0, validate_cu_seqlens
+
+MAX_HEAD_DIM = 128
+
+
+def _heads_view(t: Tensor) -> Tensor:
+    """``t`` itself where the kernels can address it (unit channel stride, no broadcast axes, 16-byte
+    aligned rows for bf16), else a contiguous copy."""
+    t = t.detach()
+    if t.stride(-1) != 1 and t.shape[-1] > 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        return t.contiguous()
+    if t.dtype == torch.bfloat16 and t.shape[-1] % 8 == 0:
+        bad = any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+        if bad or t.data_ptr() % 16:
+            return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _heads_arg(t: Tensor):
+    # an axis of length 1 may carry any stride; the kernels multiply it by 0
+    st = [s if n > 1 else t.shape[-1] for s, n in zip(t.stride(), t.shape)]
+    return ctypes.byref(L.Heads(ctypes.c_void_p(t.data_ptr()), st[0], st[1], st[2]))
+
+
+def _shapes(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor):
+    """(B, T, Hq, Hkv, dk, dv) after the argument checks."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be (B, T, heads, channels), got {tuple(t.shape)}")
+        if t.dtype != q.dtype:
+            raise TypeError(f"q, k, v must have one dtype, got {q.dtype} and {t.dtype} ({name})")
+    B, T, Hq, dk = q.shape
+    Hkv, dv = k.shape[2], v.shape[3]
+    if tuple(k.shape) != (B, T, Hkv, dk) or tuple(v.shape) != (B, T, Hkv, dv):
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    _check_heads(Hq, Hkv, dk, dv, log_decay)
+    if T < 1 or B < 1:
+        raise ValueError("batch and time must be >= 1")
+    return B, T, Hq, Hkv, dk, dv
+
+
+def _check_heads(Hq: int, Hkv: int, dk: int, dv: int, log_decay: Tensor) -> None:
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"query heads ({Hq}) must be a multiple of key / value heads ({Hkv})")
+    if not (1 <= dk <= MAX_HEAD_DIM and 1 <= dv <= MAX_HEAD_DIM):
+        raise TypeError(f"the CUDA backend covers head sizes 1..{MAX_HEAD_DIM}, got dk={dk}, dv={dv}")
+    if tuple(log_decay.shape) != (Hkv,):
+        raise ValueError(f"log_decay must be ({Hkv},), one for each key / value head, got {tuple(log_decay.shape)}")
+
+
+def _check_state(state: Tensor | None, shape: tuple[int, ...], name: str) -> Tensor | None:
+    if state is None:
+        return None
+    if state.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32 (states are kept in 32 bits), got {state.dtype}")
+    if tuple(state.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(state.shape)}")
+    return state.detach().contiguous()
+
+
+def _offsets(cu_seqlens: Tensor | None, batch: int, time: int, dev):
+    """(device int32 offsets, sequences, longest sequence).  Offsets are checked on the host, which
+    reads a CUDA tensor back; while a CUDA graph is being captured that is not possible, so they
+    have to be int32 on the device and the kernels clamp what a replay finds there."""
+    if cu_seqlens is None:
+        return None, batch, time
+    if batch != 1:
+        raise ValueError(f"cu_seqlens packs x with batch=1, got batch={batch}")
+    if dev is not None and torch.cuda.is_current_stream_capturing():
+        if not cu_seqlens.is_cuda or cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous():
+            raise RuntimeError("a CUDA graph needs cu_seqlens as a contiguous int32 CUDA tensor")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+            raise ValueError(f"cu_seqlens must be (S+1,), got {tuple(cu_seqlens.shape)}")
+        return cu_seqlens, cu_seqlens.numel() - 1, time
+    cs = validate_cu_seqlens(cu_seqlens, time)
+    longest = max(b - a for a, b in zip(cs[:-1], cs[1:]))
+    return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous(), len(cs) - 1, longest
+
+
+def linear_attention_fused(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor | None = None,
+                           cu_seqlens: Tensor | None = None, *, scale: float | None = None,
+                           want_state: bool = True):
+    """``(o, final state or None)``: ``o (B,T,Hq,dv)`` in ``q.dtype``, states fp32 ``(n_seq,Hkv,dk,dv)``."""
+    B, T, Hq, Hkv, dk, dv = _shapes(q, k, v, log_decay)
+    code = _dtype_code(q)
+    dev = _check_cuda(q, k, v, log_decay, state)
+    cu, n_seq, longest = _offsets(cu_seqlens, B, T, dev)
+    s_in = _check_state(state, (n_seq, Hkv, dk, dv), "state")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    qv, kv, vv = _heads_view(q), _heads_view(k), _heads_view(v)
+    g = log_decay.detach().to(torch.float32).contiguous()
+    # tokens that no sequence holds keep zeros (a captured call cannot check that there are none)
+    make = torch.zeros if cu is not None else torch.empty
+    out = make(B, T, Hq, dv, dtype=q.dtype, device=dev)
+    s_out = torch.empty(n_seq, Hkv, dk, dv, dtype=torch.float32, device=dev) if want_state else None
+    lib = L.lib()
+    with torch.cuda.device(dev):
+        n = lib.prb_linear_attention_workspace_bytes(B, T, n_seq, longest, Hq, Hkv, dk, dv, code, cu is not None, 0)
+        ws = _workspace(n, dev)
+        rc = lib.prb_linear_attention(_heads_arg(qv), _heads_arg(kv), _heads_arg(vv), _ptr(g), _ptr(s_in), _ptr(cu),
+                                      _ptr(out), _ptr(s_out), B, T, n_seq, longest, Hq, Hkv, dk, dv, code, scale,
+                                      _ptr(ws), ws.numel(), _stream(dev))
+    _raise(rc, "linear_attention_fused")
+    return out, s_out
+
+
+def linear_attention_reverse_vjp(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, grad_out: Tensor,
+                                 state: Tensor | None = None, grad_state: Tensor | None = None,
+                                 cu_seqlens: Tensor | None = None, *, scale: float | None = None,
+                                 want_state: bool = False):
+    """``(g_q, g_k, g_v, g_state or None)`` from the cotangents of the output and of the final state.
+    Gradients of shared key / value heads are summed over their query heads in fp32."""
+    B, T, Hq, Hkv, dk, dv = _shapes(q, k, v, log_decay)
+    code = _dtype_code(q)
+    if tuple(grad_out.shape) != (B, T, Hq, dv):
+        raise ValueError(f"grad_out must be {(B, T, Hq, dv)}, got {tuple(grad_out.shape)}")
+    dev = _check_cuda(q, k, v, log_decay, grad_out, state, grad_state)
+    cu, n_seq, longest = _offsets(cu_seqlens, B, T, dev)
+    s_in = _check_state(state, (n_seq, Hkv, dk, dv), "state")
+    gs = _check_state(grad_state, (n_seq, Hkv, dk, dv), "grad_state")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    qv, kv, vv, gv = _heads_view(q), _heads_view(k), _heads_view(v), _heads_view(grad_out.to(q.dtype))
+    g = log_decay.detach().to(torch.float32).contiguous()
+    make = torch.zeros if cu is not None else torch.empty
+    g_q = make(B, T, Hq, dk, dtype=q.dtype, device=dev)
+    g_k = make(B, T, Hkv, dk, dtype=q.dtype, device=dev)
+    g_v = make(B, T, Hkv, dv, dtype=q.dtype, device=dev)
+    g_s = torch.empty(n_seq, Hkv, dk, dv, dtype=torch.float32, device=dev) if want_state else None
+    lib = L.lib()
+    with torch.cuda.device(dev):
+        n = lib.prb_linear_attention_workspace_bytes(B, T, n_seq, longest, Hq, Hkv, dk, dv, code, cu is not None, 1)
+        ws = _workspace(n, dev)
+        rc = lib.prb_bwd_linear_attention(_heads_arg(qv), _heads_arg(kv), _heads_arg(vv), _heads_arg(gv), _ptr(g),
+                                          _ptr(s_in), _ptr(gs), _ptr(cu), _ptr(g_q), _ptr(g_k), _ptr(g_v), _ptr(g_s),
+                                          B, T, n_seq, longest, Hq, Hkv, dk, dv, code, scale, _ptr(ws), ws.numel(),
+                                          _stream(dev))
+    _raise(rc, "linear_attention_reverse_vjp")
+    return g_q, g_k, g_v, g_s
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, cu_seqlens, scale, want_state):
+        out, s_out = linear_attention_fused(q, k, v, log_decay, state, cu_seqlens, scale=scale,
+                                            want_state=want_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, cu_seqlens)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, s_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out, grad_state):
+        q, k, v, log_decay, state, cu = ctx.saved_tensors
+        if grad_out is None and grad_state is None:
+            return (None,) * 8
+        if grad_out is None:
+            grad_out = q.new_zeros(*q.shape[:3], v.shape[3])
+        g_q, g_k, g_v, g_s = linear_attention_reverse_vjp(
+            q, k, v, log_decay, grad_out, state, grad_state, cu, scale=ctx.scale,
+            want_state=ctx.needs_input_grad[4])
+        need = ctx.needs_input_grad
+        return (g_q if need[0] else None, g_k if need[1] else None, g_v if need[2] else None, None, g_s, None, None,
+                None)
+
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor | None = None,
+                     cu_seqlens: Tensor | None = None, block_table: Tensor | None = None, *,
+                     scale: float | None = None, return_state: bool = False):
+    """Linear attention with a decay for each head over whole sequences, differentiable in ``q``, ``k``,
+    ``v`` and ``state``.
+
+    ``q (B,T,Hq,dk)``, ``k (B,T,Hkv,dk)``, ``v (B,T,Hkv,dv)`` in float32 or bfloat16 (views with a unit
+    channel stride are read in place), ``Hq`` a multiple of ``Hkv`` (query head ``h`` reads state head
+    ``h // (Hq // Hkv)``), ``dk, dv <= 128``; ``log_decay (Hkv,) <= 0`` is a fixed schedule, not a
+    parameter; ``state (B,Hkv,dk,dv)`` float32 is the initial state.  With ``cu_seqlens`` the batch is
+    packed ``(1,N,...)`` and ``state`` has one row for each sequence; with ``block_table`` ``state`` is a
+    pool and row ``i`` starts from slot ``block_table[i]``.  ``scale`` defaults to ``dk ** -0.5``.
+    Returns ``o (B,T,Hq,dv)``, or ``(o, final states)`` with ``return_state=True``."""
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise TypeError("log_decay is a fixed schedule of the heads and has no gradient: detach it")
+    if block_table is not None:
+        if state is None or state.dim() != 4:
+            raise ValueError("block_table needs state as a pool (C, Hkv, dk, dv)")
+        rows = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
+        state = gather_h0(state, block_table, rows, (k.shape[2], k.shape[3], v.shape[3]))
+    out, s_out = _LinearAttention.apply(q, k, v, log_decay, state, cu_seqlens, scale, return_state)
+    return (out, s_out) if return_state else out
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, *,
+                          scale: float | None = None, block_table: Tensor | None = None,
+                          out: Tensor | None = None) -> Tensor:
+    """One token for each row: updates ``state`` in place and returns ``o (B,Hq,dv)``.
+
+    ``q (B,Hq,dk)``, ``k (B,Hkv,dk)``, ``v (B,Hkv,dv)`` (or with a time axis of length 1, which the
+    result then has too); ``state`` is a contiguous float32 ``(B,Hkv,dk,dv)``, or with ``block_table``
+    ``(B,)`` a pool ``(C,Hkv,dk,dv)`` whose named slots are updated.  Slots outside the pool mark padding
+    rows: they touch no state and their outputs are zero.  A slot that several rows name takes
+    them in row order.  One launch, no allocation with ``out=``: CUDA graphs can capture it."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise RuntimeError("linear_attention_step has no backward: call it under torch.no_grad()")
+    timed = q.dim() == 4
+    if timed:
+        if any(t.dim() != 4 or t.shape[1] != 1 for t in (q, k, v)):
+            raise ValueError("linear_attention_step takes one token: time axes must have length 1")
+        q, k, v = q[:, 0], k[:, 0], v[:, 0]
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be (B, heads, channels), got {tuple(t.shape)}")
+        if t.dtype != q.dtype:
+            raise TypeError(f"q, k, v must have one dtype, got {q.dtype} and {t.dtype} ({name})")
+    B, Hq, dk = q.shape
+    Hkv, dv = k.shape[1], v.shape[2]
+    if tuple(k.shape) != (B, Hkv, dk) or tuple(v.shape) != (B, Hkv, dv):
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    _check_heads(Hq, Hkv, dk, dv, log_decay)
+    if B < 1:
+        raise ValueError("batch must be >= 1")
+    if state.dtype != torch.float32:
+        raise TypeError(f"state must be float32 (states are kept in 32 bits), got {state.dtype}")
+    if state.dim() != 4 or tuple(state.shape[1:]) != (Hkv, dk, dv) or state.shape[0] < 1:
+        raise ValueError(f"state must be (slots, {Hkv}, {dk}, {dv}), got {tuple(state.shape)}")
+    if not state.is_contiguous():
+        raise ValueError("linear_attention_step updates state in place: it must be contiguous")
+    if block_table is None and state.shape[0] != B:
+        raise ValueError(f"state has {state.shape[0]} rows for a batch of {B}: pass block_table for a pool")
+    if block_table is not None:
+        if block_table.dim() != 1 or block_table.numel() != B:
+            raise ValueError(f"block_table must be ({B},), got {tuple(block_table.shape)}")
+        if block_table.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"block_table must be int32 or int64, got {block_table.dtype}")
+    code = _dtype_code(q)
+    dev = _check_cuda(q, k, v, log_decay, state)
+    shape = (B, 1, Hq, dv) if timed else (B, Hq, dv)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {shape} {q.dtype} on {dev}")
+    bt = None
+    if block_table is not None:
+        if not block_table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a CUDA graph needs block_table on the device")
+        bt = block_table.to(dev).contiguous()
+    q, k, v = q.detach().contiguous(), k.detach().contiguous(), v.detach().contiguous()
+    g = log_decay.detach().to(torch.float32).contiguous()
+    scale = dk ** -0.5 if scale is None else float(scale)
+    with torch.cuda.device(dev):
+        rc = L.lib().prb_linear_attention_step(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state), _ptr(bt),
+                                               int(bt is not None and bt.dtype == torch.int64), _ptr(out), B,
+                                               state.shape[0], Hq, Hkv, dk, dv, code, scale, _stream(dev))
+    _raise(rc, "linear_attention_step")
+    return out
