@@ -440,6 +440,11 @@ int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_h
                              int time, int n_seq, int max_len, int q_heads, int kv_heads, int dk, int dv, int dtype,
                              float scale, void* workspace, size_t workspace_bytes, prb_stream_t stream);
 
+/* 0, or PRB_STATUS_CHAIN_TIMEOUT when a bounded device wait of an earlier prb_linear_attention or
+ * prb_bwd_linear_attention call has run out on the current device (that call's results are not
+ * valid).  Waits for the device; clear != 0 resets it. */
+int prb_linear_attention_status(int clear);
+
 /* One token per row on a pool of fp32 states (slots,kv_heads,dk,dv), updated in place.  q (rows,q_heads,dk),
  * k (rows,kv_heads,dk), v (rows,kv_heads,dv), out (rows,q_heads,dv) contiguous.  block_table (int32 or
  * int64, NULL = row r uses slot r): a slot outside [0, slots) marks a padding row, which touches no

@@ -30,10 +30,11 @@ SegMap plan_segments(const AttnShape& s, const int* cu, bool backward) {
     const long long tokens = cu ? s.time : (long long)s.rows * s.time;
     long long len = s.max_len;
     if ((long long)s.n_seq * jobs < sm) {
-        const long long even = (tokens * jobs + sm - 1) / sm;
-        len = (even + chunk - 1) / chunk * chunk;
+        // rectangular: as many equal segments as one wave holds; packed: an even share of all tokens
+        const long long cuts = sm / (s.n_seq * jobs);
+        len = cu ? (tokens * jobs + sm - 1) / sm : (s.time + cuts - 1) / cuts;
+        len = (len + chunk - 1) / chunk * chunk;
         if (len < 8 * chunk) len = 8 * chunk;
-        if (len >= s.max_len) len = s.max_len;
     }
     if (len >= s.max_len) {
         m.seg_len = s.max_len;
@@ -64,8 +65,10 @@ int check_attn(const AttnShape& s) {
     return PRB_OK;
 }
 
-cudaError_t launch_mix(const MixParams& p, int dtype, bool state_only, cudaStream_t s) {
-    return launch_mix_simt(p, dtype, state_only, s);
+// bf16 goes to the tensor cores wherever TMA can address its tensors; fp32 and the rest to the CUDA cores
+cudaError_t launch_mix(const MixParams& p, const AttnShape& a, bool state_only, cudaStream_t s) {
+    if (options().kernel_family != 0 && mix_tc_usable(p, a.dtype)) return launch_mix_tc(p, a.rows, state_only, s);
+    return launch_mix_simt(p, a.dtype, state_only, s);
 }
 
 // the state sweep of (b, c) and its fold; leaves the states entering the segments in `dst`
@@ -86,7 +89,7 @@ cudaError_t segment_states(MixParams p, const HeadView& b, const HeadView& c, in
     j.reverse = reverse;
     j.upd_scale = upd;
     p.n_jobs = 1;
-    cudaError_t e = launch_mix(p, a.dtype, true, s);
+    cudaError_t e = launch_mix(p, a, true, s);
     if (e != cudaSuccess) return e;
     return launch_fold_states(p, dst, s_in, s_out, reverse != 0, s);
 }
@@ -148,7 +151,7 @@ int prb_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads
     j.p_scale = j.row_scale = scale;
     j.upd_scale = 1.f;
     p.n_jobs = 1;
-    return done(launch_mix(p, dtype, false, s));
+    return done(launch_mix(p, a, false, s));
 }
 
 int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads* v, const prb_heads* grad_out,
@@ -222,8 +225,10 @@ int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_h
     jv.s_row = dv;
     jv.s_col = 1;
     p.n_jobs = 3;
-    return done(launch_mix(p, dtype, false, s));
+    return done(launch_mix(p, a, false, s));
 }
+
+int prb_linear_attention_status(int clear) { return linattn_status(clear); }
 
 int prb_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, float* state,
                               const void* block_table, int table_is_int64, void* out, int rows, int slots, int q_heads,

@@ -124,7 +124,10 @@ __device__ inline bool locate(const SegMap& m, int x, Seg& s) {
 __device__ __forceinline__ float decay_pow(double g, int n) { return n == 0 ? 1.0f : (float)exp(g * n); }
 
 cudaError_t launch_mix_simt(const MixParams& p, int dtype, bool state_only, cudaStream_t s);
-cudaError_t launch_mix_tc(const MixParams& p, bool state_only, cudaStream_t s);
+bool mix_tc_usable(const MixParams& p, int dtype);
+cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStream_t s);
+// 0, or kErrChainTimeout when a bounded wait of a tensor-core sweep has run out on this device
+int linattn_status(int clear);
 // states [item][head] from per-segment contributions (in place); s_out = state behind the last segment
 cudaError_t launch_fold_states(const MixParams& p, float* seg_states, const float* s_in, float* s_out,
                                bool reverse, cudaStream_t s);

@@ -113,4 +113,7 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
 bool make_tile_map(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint32_t mid,
                    uint64_t inner, uint32_t box_rows);
 
+// cuTensorMapEncodeTiled for callers with other layouts; null when the driver lacks it
+void* tensor_map_encoder();
+
 }  // namespace prb

@@ -25,6 +25,8 @@ static EncodeTiledFn encode_fn() {
     return fn;
 }
 
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
+
 bool make_tile_map(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint32_t mid,
                    uint64_t inner, uint32_t box_rows) {
     EncodeTiledFn fn = encode_fn();

@@ -18,7 +18,8 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from .ops import _check_cuda, _dtype_code, _ptr, _raise, _stream, _workspace, gather_h0, validate_cu_seqlens
+from .ops import (_attention_devices, _check_cuda, _dtype_code, _ptr, _raise, _stream, _workspace, gather_h0,
+                  validate_cu_seqlens)
 
 MAX_HEAD_DIM = 128
 
@@ -121,6 +122,7 @@ def linear_attention_fused(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s
                                       _ptr(out), _ptr(s_out), B, T, n_seq, longest, Hq, Hkv, dk, dv, code, scale,
                                       _ptr(ws), ws.numel(), _stream(dev))
     _raise(rc, "linear_attention_fused")
+    _attention_devices.add(dev)
     return out, s_out
 
 
@@ -155,6 +157,7 @@ def linear_attention_reverse_vjp(q: Tensor, k: Tensor, v: Tensor, log_decay: Ten
                                           B, T, n_seq, longest, Hq, Hkv, dk, dv, code, scale, _ptr(ws), ws.numel(),
                                           _stream(dev))
     _raise(rc, "linear_attention_reverse_vjp")
+    _attention_devices.add(dev)
     return g_q, g_k, g_v, g_s
 
 

@@ -125,9 +125,25 @@ def _track_backward(sb: DeviceStats) -> None:
         del _pending_backward[0]
 
 
+# Devices on which linear attention ran since its status word was last read.
+_attention_devices: set = set()
+
+
+def _check_attention() -> None:
+    for dev in list(_attention_devices):
+        _attention_devices.discard(dev)
+        with torch.cuda.device(dev):
+            status = L.lib().prb_linear_attention_status(1)
+        if status != 0:
+            raise RuntimeError("pararnn_b200: a bounded device-side wait ran out in an earlier linear attention "
+                               f"call on {dev} (status {status}); the results of that call are not valid")
+
+
 def check_pending_backward() -> None:
-    """Raise if a reverse scan issued since the last check ran into a bounded device-side wait
-    that gave up (its gradients are not valid).  One small device-to-host copy per device."""
+    """Raise if a reverse scan (or a linear attention sweep) issued since the last check ran into a
+    bounded device-side wait that gave up (its results are not valid).  One small device-to-host
+    copy per device."""
+    _check_attention()
     if not _pending_backward:
         return
     pending, _pending_backward[:] = list(_pending_backward), []

@@ -385,3 +385,20 @@ def test_step_in_a_graph():
         want = prb.linear_attention_step(q, k, v, g, ref, block_table=bt.clone())
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(pool, ref)
+
+
+def test_first_call_of_a_fresh_thread():
+    """The tensor-core path encodes tensor maps through the driver, which needs the device's context
+    in the calling thread; a new thread has none until something binds it."""
+    import threading
+
+    q, k, v = (torch.randn(1, 200, 2, 64, device="cuda").bfloat16() for _ in range(3))
+    g = torch.tensor([-0.1, -0.2], device="cuda")
+    want = la.linear_attention_fused(q, k, v, g)
+    torch.cuda.synchronize()
+    got = []
+    th = threading.Thread(target=lambda: got.append(la.linear_attention_fused(q, k, v, g)))
+    th.start()
+    th.join()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0][0], want[0]) and torch.equal(got[0][1], want[1])
