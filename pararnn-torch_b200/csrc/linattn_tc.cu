@@ -9,7 +9,13 @@
 //
 // Roles: warp 8 keeps a ring of (a, b, c) chunk tiles full with TMA; one thread of warp 9 issues the
 // tcgen05.mma; warps 0-3 own a query row per thread (mask and decay of the scores, epilogue); warps
-// 4-7 own a state row per thread (b^T decayed and moved to TMEM, S update).
+// 4-7 own a state row per thread (b^T decayed and moved to TMEM, S update); warp 10 stores the output
+// tile with TMA out of the stage whose a and b it has replaced.
+//
+// b^T reaches TMEM through transposing ldmatrix loads: a fragment of 8 x 8 holds token pairs of one
+// channel, which is what a 16x128b TMEM store wants, so a warp moves its 32 x 128 piece in some 750
+// instructions (reading single bf16 values down the columns took 16,000 cycles per chunk).  The
+// decay of a score off the diagonal 32 x 32 blocks is a product of a row and a column factor.
 //
 // Roundings: the scores and the state are rounded to bf16 once as operands, 2^-9 each, which is
 // what the bf16 output loses anyway.  The decayed b^T is split into two bf16 halves (2^-17): the state
@@ -34,7 +40,7 @@ namespace prb {
 namespace {
 
 constexpr int kC = 128;        // tokens per chunk
-constexpr int kThreads = 320;  // 4 output warps, 4 state warps, TMA warp, MMA warp
+constexpr int kThreads = 352;  // 4 output warps, 4 state warps, TMA, MMA and store warp
 constexpr uint32_t kPanel = kC * 128;  // bytes of a 128-token x 64-channel bf16 panel
 constexpr uint32_t kWaitLimit = 1u << 22;
 
@@ -85,6 +91,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_16x128b_x2(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0), "r"(r1),
+                 "r"(r2), "r"(r3)
+                 : "memory");
+}
+// four 8 x 8 bf16 matrices, transposed; lane l gives the address of row l % 8 of matrix l / 8
+__device__ __forceinline__ void ldmatrix_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
 // Shared-memory operand in 128-byte-swizzled panels of 64 bf16 channels.  Read along the channels
 // (K-major) only the stride between groups of 8 rows matters; read along the rows (MN-major) `lead`
 // is the stride between panels.
@@ -105,6 +124,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -116,9 +141,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 struct TcParams {
     MixParams p;
-    CUtensorMap map[3][3];  // [job][a, b, c]
+    CUtensorMap map[3][4];  // [job][a, b, c, out]
     int units;              // heads of all jobs per state head
 };
+
+constexpr uint32_t kCtlBytes = 1536;
 
 template <int DA, int DC, bool STATE_ONLY>
 struct Layout {
@@ -130,17 +157,18 @@ struct Layout {
     static constexpr int kStages = (int)((224 * 1024 - kS) / kStage) < 4 ? (int)((224 * 1024 - kS) / kStage) : 4;
     static constexpr uint32_t kOffS = kStages * kStage;
     static constexpr uint32_t kOffCtl = kOffS + kS;
-    static constexpr uint32_t kBytes = kOffCtl + 1024 + 1024;  // control block, alignment slack
+    static constexpr uint32_t kBytes = kOffCtl + kCtlBytes + 1024;  // alignment slack
 };
 
 struct Control {
     uint64_t full[4], empty[4];
-    uint64_t p_full, p_ready, b_ready, u_full, u_free, s_ready, o_full, x_free, drain;
+    uint64_t p_full, p_ready, b_ready, u_full, u_free, s_ready, o_full, x_free, staged, drain;
     uint32_t tmem;
     int dead;
-    float pw[kC + 1];
+    float pw[kC + 1];  // w^0 .. w^128
+    alignas(8) float wb[kC];  // w^pos' of a full chunk, read in pairs
 };
-static_assert(sizeof(Control) <= 1024, "control block");
+static_assert(sizeof(Control) <= kCtlBytes, "control block");
 
 // false: the limit ran out, or another warp's did
 __device__ __forceinline__ bool wait(Control& ct, uint64_t* bar, uint32_t parity) {
@@ -158,9 +186,11 @@ __device__ __forceinline__ bool wait_warp(Control& ct, uint64_t* bar, uint32_t p
     return __all_sync(0xffffffffu, wait(ct, bar, parity));
 }
 
-// 8 channels of a row of a swizzled panel set
-__device__ __forceinline__ void row8(const unsigned char* tile, int row, int ch, float (&v)[8]) {
-    const unsigned char* at = tile + (ch >> 6) * kPanel + row * 128 + (((ch & 63) * 2) ^ ((row & 7) << 4));
+// The rows that hold something not finite read their operands again from global memory.
+__device__ __forceinline__ const __nv_bfloat16* token(const HeadView& v, int row, long long t, int h) {
+    return reinterpret_cast<const __nv_bfloat16*>(v.p) + row * v.sb + t * v.st + h * v.sh;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* at, float (&v)[8]) {
     const uint4 u = *reinterpret_cast<const uint4*>(at);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -169,27 +199,32 @@ __device__ __forceinline__ void row8(const unsigned char* tile, int row, int ch,
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
-// the scores of one row over the positions [j0, j1) that it may see, rounded as the operand is
-__device__ __noinline__ void row_scores(const unsigned char* a, const unsigned char* b, int da_pad, int i, int j0,
-                                        int j1, const float* pw, float scale, float* p) {
+// the scores of row i over the positions [j0, j1) that it may see, rounded as the operand is
+__device__ __noinline__ void row_scores(const MixJob& jb, int row, long long t0, int head, int hb, int i, int j0,
+                                        int j1, const float* pw, float* p) {
+    const __nv_bfloat16* a = token(jb.a, row, t0 + i, head);
     for (int j = j0; j < j1; ++j) {
+        const __nv_bfloat16* b = token(jb.b, row, t0 + j, hb);
         float s = 0.f, x[8], y[8];
-        for (int d = 0; d < da_pad; d += 8) {
-            row8(a, i, d, x);
-            row8(b, j, d, y);
+        for (int d = 0; d < jb.da; d += 8) {
+            load8(a + d, x);
+            load8(b + d, y);
 #pragma unroll
             for (int k = 0; k < 8; ++k) s = fmaf(x[k], y[k], s);
         }
-        p[j] = __bfloat162float(__float2bfloat16_rn(s * (scale * pw[j < i ? i - j : j - i])));
+        p[j] = __bfloat162float(__float2bfloat16_rn(s * (jb.p_scale * pw[j < i ? i - j : j - i])));
     }
 }
-__device__ __noinline__ void row_mix(const unsigned char* c, const float* p, int j0, int j1, int c0, float* out) {
+__device__ __noinline__ void row_mix(const MixJob& jb, int row, long long t0, int hb, const float* p, int j0, int j1,
+                                     int c0, float* out) {
     float acc[32] = {};
     for (int j = j0; j < j1; ++j) {
+        const __nv_bfloat16* c = token(jb.c, row, t0 + j, hb) + c0;
 #pragma unroll
         for (int k = 0; k < 32; k += 8) {
+            if (c0 + k >= jb.dc) break;
             float v[8];
-            row8(c, j, c0 + k, v);
+            load8(c + k, v);
 #pragma unroll
             for (int q = 0; q < 8; ++q) acc[k + q] = fmaf(p[j], v[q], acc[k + q]);
         }
@@ -225,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     if (tid == 0) {
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(&ct.full[i], 1);
-            mbar_init(&ct.empty[i], STATE_ONLY ? 5 : 9);
+            mbar_init(&ct.empty[i], STATE_ONLY ? 5 : 6);
         }
         mbar_init(&ct.p_full, 1);
         mbar_init(&ct.p_ready, 4);
@@ -235,11 +270,20 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         mbar_init(&ct.s_ready, 4);
         mbar_init(&ct.o_full, 1);
         mbar_init(&ct.x_free, 4);
+        mbar_init(&ct.staged, 4);
         mbar_init(&ct.drain, 1);
         ct.dead = 0;
         mbar_fence_init();
     }
-    if (tid < kC + 1) ct.pw[tid] = decay_pow(p.log_decay[hs], tid);
+    if (tid < kC + 1) {
+        const float w = decay_pow(p.log_decay[hs], tid);
+        ct.pw[tid] = w;
+        if (jb.reverse) {
+            if (tid > 0) ct.wb[tid - 1] = w;
+        } else if (tid < kC) {
+            ct.wb[kC - 1 - tid] = w;
+        }
+    }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ct.tmem))
                      : "memory");
@@ -342,6 +386,24 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             tc_commit(&ct.drain);
             mbar_wait_bounded(&ct.drain, 0, kWaitLimit);
         }
+    } else if (warp == 10) {
+        // ---- store: whole chunks leave through TMA, ragged ones the output warps have written themselves
+        if (!STATE_ONLY && lane == 0) {
+            for (int it = 0; it < n_it; ++it) {
+                const int st = it % L::kStages, off = chunk_off(it);
+                if (!wait(ct, &ct.staged, it & 1)) break;
+                if (seg.len - off >= kC && (!GROUPED || it % share == share - 1)) {
+                    for (int q = 0; q < DC / 64; ++q)
+                        if (q * 64 < jb.dc)
+                            tma_store_4d(&tp.map[ji][3], base + st * L::kStage + q * kPanel, q * 64, head,
+                                         seg.t0 + off, seg.row);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                }
+                mbar_arrive(&ct.empty[st]);
+            }
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
     } else if (warp >= 4) {
         // ---- state: thread r owns row r of S
         const int r = tid - 128;
@@ -388,28 +450,40 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 fence_proxy_async();
             }
             if (mine) {
-                const unsigned char* col = tile + (r >> 6) * kPanel;
-                const int cb = (r & 63) * 2;
+                const int d0 = (warp & 3) * 32, t2 = 2 * (lane & 3);
+                const uint32_t from = smem_u32(tile) + (d0 >> 6) * kPanel + (lane & 7) * 128 +
+                                      ((((d0 & 63) + 8 * (lane >> 3)) * 2) ^ ((lane & 7) << 4));
 #pragma unroll 1
-                for (int j0 = 0; j0 < kC; j0 += 32) {
-                    uint32_t hi[16], lo[16];
+                for (int tg = 0; tg < kC / 8; tg += 2) {
+                    uint32_t hi[2][4], lo[2][4];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float f[2];
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t f[4];
+                        ldmatrix_t(from + (tg + e) * 1024, f);
+                        const int t = (tg + e) * 8 + t2;
+                        float2 w = *reinterpret_cast<const float2*>(&ct.wb[t]);
+                        if (n < kC) {
+                            w.x = t < n ? ct.pw[reverse ? t + 1 : n - 1 - t] : 0.f;
+                            w.y = t + 1 < n ? ct.pw[reverse ? t + 2 : n - 2 - t] : 0.f;
+                            const uint32_t keep = (t < n ? 0xffffu : 0u) | (t + 1 < n ? 0xffff0000u : 0u);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int t = j0 + j + e;
-                            const unsigned short b =
-                                *reinterpret_cast<const unsigned short*>(col + t * 128 + (cb ^ ((t & 7) << 4)));
-                            const int pos = reverse ? t + 1 : n - 1 - t;
-                            f[e] = t < n ? __uint_as_float((uint32_t)b << 16) * ct.pw[max(pos, 0)] : 0.f;
+                            for (int q = 0; q < 4; ++q) f[q] &= keep;
                         }
-                        const uint32_t h = pack_bf16(f[0], f[1]);
-                        hi[j >> 1] = h;
-                        lo[j >> 1] = pack_bf16(f[0] - __uint_as_float(h << 16), f[1] - __uint_as_float(h & 0xffff0000u));
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float2 v = __fmul2_rn(
+                                make_float2(__uint_as_float(f[q] << 16), __uint_as_float(f[q] & 0xffff0000u)), w);
+                            const uint32_t h = pack_bf16(v.x, v.y);
+                            hi[e][q] = h;
+                            lo[e][q] = pack_bf16(v.x - __uint_as_float(h << 16),
+                                                 v.y - __uint_as_float(h & 0xffff0000u));
+                        }
                     }
-                    tmem_st16(lanes + kColB + (j0 >> 1), hi);
-                    tmem_st16(lanes + kColB + 64 + (j0 >> 1), lo);
+                    const uint32_t col = lanes + kColB + tg * 4, low16 = 16u << 16;
+                    tmem_st_16x128b_x2(col, hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
+                    tmem_st_16x128b_x2(col + low16, hi[0][2], hi[0][3], hi[1][2], hi[1][3]);
+                    tmem_st_16x128b_x2(col + 64, lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
+                    tmem_st_16x128b_x2(col + 64 + low16, lo[0][2], lo[0][3], lo[1][2], lo[1][3]);
                 }
                 tc_wait_st();
             }
@@ -449,36 +523,64 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         const uint32_t lanes = tmem + ((uint32_t)warp << 21);
         float acc[GROUPED ? DC : 1];
         __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(jb.out);
+        // column factors of the blocks off the diagonal: forwards w^(31 - k), backwards w^k
+        float2 colw[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            colw[k].x = jb.p_scale * ct.pw[reverse ? 2 * k : 31 - 2 * k];
+            colw[k].y = jb.p_scale * ct.pw[reverse ? 2 * k + 1 : 30 - 2 * k];
+        }
         for (int it = 0; it < n_it; ++it) {
             const int st = it % L::kStages, g = GROUPED ? it % share : 0;
             const int off = chunk_off(it), n = min(kC, seg.len - off);
             const uint32_t par = it & 1;
             if (!wait_warp(ct, &ct.p_full, par)) break;
             tc_fence_after();
-            const float ps = jb.p_scale;
 #pragma unroll 1
-            for (int jb4 = 0; jb4 < 4; ++jb4) {
+            for (int jc = 0; jc < 4; ++jc) {
                 uint32_t v[32], h[16];
-                if (reverse ? jb4 < warp : jb4 > warp) {
+                if (reverse ? jc < warp : jc > warp) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) h[k] = 0u;
                 } else {
-                    tmem_ld32(lanes + kColP + jb4 * 32, v);
+                    tmem_ld32(lanes + kColP + jc * 32, v);
+                    const float row = ct.pw[jc == warp ? 0 : reverse ? jc * 32 - i : i - jc * 32 - 31];
                     tc_wait_ld();
-                    const int gap0 = reverse ? jb4 * 32 - i : i - jb4 * 32;  // distance of column 0
+                    if (jc != warp) {
+                        const float2 row2 = make_float2(row, row);
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        float f[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int gap = reverse ? gap0 + k + e : gap0 - k - e;
-                            const bool in = gap >= 0 && jb4 * 32 + k + e < n;
-                            f[e] = in ? __uint_as_float(v[k + e]) * (ps * ct.pw[max(gap, 0)]) : 0.f;
+                        for (int k = 0; k < 16; ++k) {
+                            const float2 f = __fmul2_rn(
+                                make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])),
+                                __fmul2_rn(colw[k], row2));
+                            h[k] = pack_bf16(f.x, f.y);
                         }
-                        h[k >> 1] = pack_bf16(f[0], f[1]);
+                    } else {
+                        // a masked score is replaced, not multiplied by 0: it may be inf or NaN
+                        const float* pw = reverse ? ct.pw - lane : ct.pw + lane;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            float f[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const bool in = reverse ? k + e >= lane : k + e <= lane;
+                                f[e] = 0.f;
+                                if (in)
+                                    f[e] = __uint_as_float(v[k + e]) *
+                                           (jb.p_scale * (reverse ? pw[k + e] : pw[-(k + e)]));
+                            }
+                            h[k >> 1] = pack_bf16(f[0], f[1]);
+                        }
+                    }
+                    if (reverse && n < kC) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const int j = jc * 32 + 2 * k;
+                            h[k] &= (j < n ? 0xffffu : 0u) | (j + 1 < n ? 0xffff0000u : 0u);
+                        }
                     }
                 }
-                tmem_st16(lanes + kColP + jb4 * 32, h);
+                tmem_st16(lanes + kColP + jc * 32, h);
             }
             tc_wait_st();
             tc_fence_before();
@@ -487,7 +589,10 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             if (!wait_warp(ct, &ct.o_full, par)) break;
             tc_fence_after();
             const float rw = i < n ? jb.row_scale * ct.pw[reverse ? n - 1 - i : i + 1] : 0.f;
+            const float2 rw2 = make_float2(rw, rw);
+            const bool whole = n == kC, final = g == share - 1;
             __nv_bfloat16* dst = out + (((size_t)seg.row * p.map.time + seg.t0 + off + i) * jb.heads + head) * jb.dc;
+            unsigned char* tile = smem + st * L::kStage + i * 128;
             float again[kC];
             bool have = false;
 #pragma unroll
@@ -496,45 +601,55 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 tmem_ld32(lanes + kColX + c0, x);
                 if (g == 0) tmem_ld32(lanes + kColI + c0, in);
                 tc_wait_ld();
-                float o[32], bad = 0.f;
+                float2 o[16], bad = make_float2(0.f, 0.f);
+                const float2 zero = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    o[k] = __uint_as_float(x[k]);
-                    bad = fmaf(o[k], 0.f, bad);
+                for (int k = 0; k < 16; ++k) {
+                    o[k] = make_float2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]));
+                    bad = __ffma2_rn(o[k], zero, bad);
                 }
-                if (bad != 0.f && i < n) {  // NaN: some o[k] is not finite
-                    const unsigned char* ta = smem + st * L::kStage;
+                if (!(bad.x + bad.y == 0.f) && i < n) {  // NaN: some o[k] is not finite
                     const int j0 = reverse ? i : 0, j1 = reverse ? n : i + 1;
-                    if (!have) row_scores(ta, ta + L::kA, DA, i, j0, j1, ct.pw, ps, again);
+                    const int hb = share > 1 ? head * share + g : hs;
+                    if (!have) row_scores(jb, seg.row, seg.t0 + off, head, hb, i, j0, j1, ct.pw, again);
                     have = true;
                     float t[32];
-                    row_mix(ta + L::kA + L::kB, again, j0, j1, c0, t);
+                    row_mix(jb, seg.row, seg.t0 + off, hb, again, j0, j1, c0, t);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = t[k];
+                    for (int k = 0; k < 16; ++k) o[k] = make_float2(t[2 * k], t[2 * k + 1]);
                 }
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    if (g == 0) o[k] = fmaf(rw, __uint_as_float(in[k]), o[k]);
-                    if (GROUPED) o[k] = acc[c0 + k] = g == 0 ? o[k] : acc[c0 + k] + o[k];
+                for (int k = 0; k < 16; ++k) {
+                    if (g == 0)
+                        o[k] = __ffma2_rn(rw2, make_float2(__uint_as_float(in[2 * k]), __uint_as_float(in[2 * k + 1])),
+                                          o[k]);
+                    if (GROUPED) {
+                        if (g > 0) o[k] = __fadd2_rn(o[k], make_float2(acc[c0 + 2 * k], acc[c0 + 2 * k + 1]));
+                        acc[c0 + 2 * k] = o[k].x;
+                        acc[c0 + 2 * k + 1] = o[k].y;
+                    }
                 }
-                if (i < n && g == share - 1) {
+                if (!final) continue;
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8)
-                        if (c0 + k < jb.dc) {
-                            uint4 w;
-                            w.x = pack_bf16(o[k], o[k + 1]);
-                            w.y = pack_bf16(o[k + 2], o[k + 3]);
-                            w.z = pack_bf16(o[k + 4], o[k + 5]);
-                            w.w = pack_bf16(o[k + 6], o[k + 7]);
-                            *reinterpret_cast<uint4*>(dst + c0 + k) = w;
-                        }
+                for (int k = 0; k < 16; k += 4) {
+                    uint4 w;
+                    w.x = pack_bf16(o[k].x, o[k].y);
+                    w.y = pack_bf16(o[k + 1].x, o[k + 1].y);
+                    w.z = pack_bf16(o[k + 2].x, o[k + 2].y);
+                    w.w = pack_bf16(o[k + 3].x, o[k + 3].y);
+                    const int c = c0 + 2 * k;
+                    if (whole)
+                        *reinterpret_cast<uint4*>(tile + (c >> 6) * kPanel + (((c & 63) * 2) ^ ((i & 7) << 4))) = w;
+                    else if (i < n && c < jb.dc)
+                        *reinterpret_cast<uint4*>(dst + c) = w;
                 }
             }
             tc_fence_before();
+            fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&ct.x_free);
-                mbar_arrive(&ct.empty[st]);
+                mbar_arrive(&ct.staged);
             }
         }
     }
@@ -594,7 +709,7 @@ bool mix_tc_usable(const MixParams& p, int dtype) {
     if (dtype != kBF16 || !tensor_map_encoder()) return false;
     for (int j = 0; j < p.n_jobs; ++j) {
         const MixJob& jb = p.job[j];
-        if (jb.da % 8 || jb.dc % 8) return false;
+        if (jb.da % 8 || jb.dc % 8 || (reinterpret_cast<uintptr_t>(jb.out) & 15)) return false;
         for (const HeadView* v : {&jb.a, &jb.b, &jb.c}) {
             if (reinterpret_cast<uintptr_t>(v->p) & 15) return false;
             for (long long st : {v->sb, v->st, v->sh})
@@ -631,6 +746,9 @@ cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStr
             if (!head_map(&tp.map[k][0], jb.a, jb.da, jb.heads, p.map.time, rows) ||
                 !head_map(&tp.map[k][1], jb.b, jb.da, hb, p.map.time, rows) ||
                 !head_map(&tp.map[k][2], jb.c, jb.dc, hb, p.map.time, rows))
+                return cudaErrorInvalidValue;
+            const HeadView o{jb.out, (long long)p.map.time * jb.heads * jb.dc, (long long)jb.heads * jb.dc, jb.dc};
+            if (!state_only && !head_map(&tp.map[k][3], o, jb.dc, jb.heads, p.map.time, rows))
                 return cudaErrorInvalidValue;
         }
         const cudaError_t e = launch_set(tp, state_only, s);
