@@ -209,9 +209,12 @@ __global__ void fold_states_kernel(const __grid_constant__ MixParams p, float* s
         n = max(1, (hi - lo + m.seg_len - 1) / m.seg_len);
         n = max(0, min(n, m.n_items - base));
     }
+    __shared__ float w[2];  // decay over a full segment and over the last one
+    if (threadIdx.x < 2)
+        w[threadIdx.x] = decay_pow(p.log_decay[hs], threadIdx.x ? max(0, hi - lo - (n - 1) * m.seg_len) : m.seg_len);
+    __syncthreads();
     if (e >= p.state_elems) return;
-    const double g = p.log_decay[hs];
-    const float w_full = decay_pow(g, m.seg_len), w_last = decay_pow(g, max(0, hi - lo - (n - 1) * m.seg_len));
+    const float w_full = w[0], w_last = w[1];
     const size_t own = ((size_t)seq * p.state_heads + hs) * p.state_elems + e;
     float run = s_in ? s_in[own] : 0.f;
     for (int i = 0; i < n; ++i) {

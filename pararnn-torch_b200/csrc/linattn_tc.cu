@@ -1,32 +1,43 @@
 // Linear attention with a decay for each head on the tensor cores (bf16 inputs, head sizes that are
 // multiples of 8 up to 128).  One CTA walks a segment of one head in chunks of 128 tokens:
 //
-//   P  = a b^T            (128 x 128 x da)   a, b from shared memory             -> TMEM, fp32
-//   X  = (w^|i-j| P) c    (128 x dc x 128)   scores as a bf16 TMEM operand       -> TMEM
-//   I  = a S              (128 x dc x da)    S as a bf16 shared-memory operand   -> TMEM
-//   U  = (w^pos' b)^T c   (da x dc x 128)    decayed b^T as a TMEM operand       -> TMEM
-//   out = X + w^pos I,   S = w^n S + U       S itself stays in fp32 registers
+//   P = a b^T                 (128 x 128 x da)   a, b from shared memory             -> TMEM, fp32
+//   X = a S                   (128 x dc x da)    S as a bf16 shared-memory operand   -> TMEM
+//   X = w^pos X + (w^|i-j| P) c                  scores as a bf16 TMEM operand       -> TMEM
+//   U = (w^pos' b)^T c        (da x dc x 128)    decayed b^T as a TMEM operand       -> TMEM
+//   out = X,   S = w^n S + U                     S itself stays in fp32 registers
 //
-// Roles: warp 8 keeps a ring of (a, b, c) chunk tiles full with TMA; one thread of warp 9 issues the
-// tcgen05.mma; warps 0-3 own a query row per thread (mask and decay of the scores, epilogue); warps
-// 4-7 own a state row per thread (b^T decayed and moved to TMEM, S update); warp 10 stores the output
-// tile with TMA out of the stage whose a and b it has replaced.
+// With share_b > 1 (gradients of shared heads) a chunk is visited once per query head; X and U add up
+// in TMEM and the epilogue and the state update run at the last visit.
 //
-// b^T reaches TMEM through transposing ldmatrix loads: a fragment of 8 x 8 holds token pairs of one
-// channel, which is what a 16x128b TMEM store wants, so a warp moves its 32 x 128 piece in some 750
-// instructions (reading single bf16 values down the columns took 16,000 cycles per chunk).  The
-// decay of a score off the diagonal 32 x 32 blocks is a product of a row and a column factor.
+// Roles: warps 0-3 own a state row per thread (b^T decayed and moved to TMEM, S update); warps 4-11 own
+// half a query row per thread (mask and decay of the scores, row factor of X, epilogue); warp 12 keeps
+// a ring of (a, b, c) tiles full with TMA; one thread of warp 13 issues the tcgen05.mma; warp 14
+// stores the output tile with TMA out of the stage whose a and b it has replaced; warp 15 looks for
+// inf and NaN in c.  The state rows take up to 128 registers a thread, so the warpgroups trade
+// registers (setmaxnreg).
 //
 // Roundings: the scores and the state are rounded to bf16 once as operands, 2^-9 each, which is
 // what the bf16 output loses anyway.  The decayed b^T is split into two bf16 halves (2^-17): the state
-// it builds is returned in fp32 and may be read by thousands of later tokens.  The two halves cost
-// a second pass of U's matrix product, and keep the tile of b itself untouched in shared memory.
+// it builds is returned in fp32 and may be read by thousands of later tokens.  With da = 128 the
+// halves follow one another along K; with da = 64 they fill the two halves of the 128 TMEM lanes, so
+// that the second half costs no further matrix instructions: threads 64-127 then carry the
+// state of the low halves, and S is the sum of the two.
 //
-// TMEM columns: scores 0-127 (fp32, then bf16 in place), I 128-255, U and then X 256-383, decayed b^T
-// 384-511 (two halves).  U is read into registers before X overwrites it.
+// b^T reaches TMEM through transposing ldmatrix loads: a fragment of 8 x 8 holds token pairs of one
+// channel, which is what a 16x128b TMEM store wants.  It is made in two halves of 64 tokens, so that
+// one half is written while the matrix unit reads the other.  The decay of a score off the diagonal
+// 32 x 32 blocks is a product of a row and a column factor.
 //
-// A masked score is 0, and 0 x inf = NaN: a row whose X is not finite is summed again over the
-// positions that it may see (row_scores / row_mix), so that nothing behind the mask can reach it.
+// With da = dc = 64 there is room for the scores and X twice (kTwice): the scores of visit i + 1 are made
+// and converted while the matrix unit works on X of visit i.  With 128 channels the four
+// regions fill all 512 columns.  The state warps publish S, read U and write b^T in program order, so
+// one barrier (b_ready) tells the MMA thread all three; every further barrier would cost it some 200
+// cycles a visit.
+//
+// A masked score is 0, and 0 x inf = NaN: a chunk whose c holds an inf or a NaN skips the product with c
+// on the tensor cores; its rows are summed over the positions that they may see (row_mix),
+// so that nothing behind the mask can reach them.
 //
 // Every wait has a limit; a CTA whose wait runs out raises g_status, lets its copies and matrix
 // products in flight end, frees its TMEM and leaves.
@@ -40,11 +51,9 @@ namespace prb {
 namespace {
 
 constexpr int kC = 128;        // tokens per chunk
-constexpr int kThreads = 352;  // 4 output warps, 4 state warps, TMA, MMA and store warp
+constexpr int kThreads = 512;  // 4 state warps, 8 output warps, TMA, MMA, store and scan warp
 constexpr uint32_t kPanel = kC * 128;  // bytes of a 128-token x 64-channel bf16 panel
 constexpr uint32_t kWaitLimit = 1u << 22;
-
-constexpr uint32_t kColP = 0, kColI = 128, kColX = 256, kColB = 384;
 
 __device__ int g_status;
 
@@ -91,9 +100,31 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_16x128b_x2(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
-    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0), "r"(r1),
-                 "r"(r2), "r"(r3)
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// 16 lanes x 16 columns: pairs (r[2j], r[2j+1]) are the rows l / 4 and l / 4 + 8 of columns 4j ...
+__device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
 // four 8 x 8 bf16 matrices, transposed; lane l gives the address of row l % 8 of matrix l / 8
@@ -124,6 +155,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
+template <int N>
+__device__ __forceinline__ void regs_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
                      reinterpret_cast<uint64_t>(map)),
@@ -139,13 +178,16 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
+
 struct TcParams {
     MixParams p;
     CUtensorMap map[3][4];  // [job][a, b, c, out]
     int units;              // heads of all jobs per state head
 };
 
-constexpr uint32_t kCtlBytes = 1536;
+constexpr uint32_t kCtlBytes = 2048;
 
 template <int DA, int DC, bool STATE_ONLY>
 struct Layout {
@@ -153,25 +195,37 @@ struct Layout {
     static constexpr uint32_t kB = DA / 64 * kPanel;
     static constexpr uint32_t kCc = DC / 64 * kPanel;
     static constexpr uint32_t kStage = kA + kB + kCc;
-    static constexpr uint32_t kS = STATE_ONLY ? 0 : DA * DC * 2;
+    static constexpr uint32_t kS = 128 * DC * 2;  // 128 state rows (da = 64: high and low halves)
     static constexpr int kStages = (int)((224 * 1024 - kS) / kStage) < 4 ? (int)((224 * 1024 - kS) / kStage) : 4;
     static constexpr uint32_t kOffS = kStages * kStage;
     static constexpr uint32_t kOffCtl = kOffS + kS;
     static constexpr uint32_t kBytes = kOffCtl + kCtlBytes + 1024;  // alignment slack
+    // TMEM columns: scores (fp32, then bf16 in place), X, U, decayed b^T
+    static constexpr bool kTwice = DA == 64 && DC == 64;
+    static constexpr int kHalves = DA == 64 ? 1 : 2;  // pieces in which b^T is made
+    static constexpr uint32_t kColP = 0, kColX = kTwice ? 256 : 128, kColU = kTwice ? 384 : 256,
+                              kColB = kTwice ? 448 : 384;
 };
 
 struct Control {
-    uint64_t full[4], empty[4];
-    uint64_t p_full, p_ready, b_ready, u_full, u_free, s_ready, o_full, x_free, staged, drain;
+    // one per stage: their producers may be several visits ahead of (or behind) the others
+    uint64_t full[4], empty[4], scanned[4], staged[4];
+    // one visit or chunk at a time
+    uint64_t p_full[2], p_ready, b_ready[2], b_free[2], i_full, o_full, x_free, drain;
     uint32_t tmem;
     int dead;
-    float pw[kC + 1];  // w^0 .. w^128
-    alignas(8) float wb[kC];  // w^pos' of a full chunk, read in pairs
+    int dirty[4];
+    float pw[kC + 1];              // w^0 .. w^128
+    float ps[kC];                  // p_scale w^0 .. w^127
+    alignas(8) uint2 wb[kC / 2];   // upd_scale w^pos' of a token pair: bf16 pairs, high and low parts
+    alignas(16) float wc[32];      // p_scale times the column factors of the score blocks off the diagonal
 };
 static_assert(sizeof(Control) <= kCtlBytes, "control block");
 
 // false: the limit ran out, or another warp's did
 __device__ __forceinline__ bool wait(Control& ct, uint64_t* bar, uint32_t parity) {
+    // one compact loop: the roles' code shares the instruction cache, and every visit passes a dozen waits
+#pragma unroll 1
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255) == 255 && *reinterpret_cast<volatile int*>(&ct.dead)) return false;
@@ -199,49 +253,41 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* at, float (&v)[8]) {
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
-// the scores of row i over the positions [j0, j1) that it may see, rounded as the operand is
-__device__ __noinline__ void row_scores(const MixJob& jb, int row, long long t0, int head, int hb, int i, int j0,
-                                        int j1, const float* pw, float* p) {
+// acc (8 channels from c0 of row i): the row's scores, rounded as the operand is, times c
+__device__ __forceinline__ void row_mix(const MixJob& jb, int row, long long t0, int head, int hb, int i, int j0,
+                                        int j1, int c0, const float* ps, float (&acc)[8]) {
     const __nv_bfloat16* a = token(jb.a, row, t0 + i, head);
+#pragma unroll 1
     for (int j = j0; j < j1; ++j) {
         const __nv_bfloat16* b = token(jb.b, row, t0 + j, hb);
-        float s = 0.f, x[8], y[8];
+        float s = 0.f, y[8], z[8];
+#pragma unroll 1
         for (int d = 0; d < jb.da; d += 8) {
-            load8(a + d, x);
-            load8(b + d, y);
+            load8(a + d, y);
+            load8(b + d, z);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s = fmaf(x[k], y[k], s);
+            for (int q = 0; q < 8; ++q) s = fmaf(y[q], z[q], s);
         }
-        p[j] = __bfloat162float(__float2bfloat16_rn(s * (jb.p_scale * pw[j < i ? i - j : j - i])));
+        s = __bfloat162float(__float2bfloat16_rn(s * ps[j < i ? i - j : j - i]));
+        load8(token(jb.c, row, t0 + j, hb) + c0, y);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] = fmaf(s, y[q], acc[q]);
     }
-}
-__device__ __noinline__ void row_mix(const MixJob& jb, int row, long long t0, int hb, const float* p, int j0, int j1,
-                                     int c0, float* out) {
-    float acc[32] = {};
-    for (int j = j0; j < j1; ++j) {
-        const __nv_bfloat16* c = token(jb.c, row, t0 + j, hb) + c0;
-#pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-            if (c0 + k >= jb.dc) break;
-            float v[8];
-            load8(c + k, v);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) acc[k + q] = fmaf(p[j], v[q], acc[k + q]);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 32; ++k) out[k] = acc[k];
 }
 
-template <int DA, int DC, bool STATE_ONLY, bool GROUPED>
+template <int DA, int DC, bool STATE_ONLY>
 __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_constant__ TcParams tp) {
     using L = Layout<DA, DC, STATE_ONLY>;
+    constexpr bool kSplit = DA == 64;  // low halves of b^T in lanes 64-127
     extern __shared__ unsigned char raw[];
     const uint32_t raw_at = smem_u32(raw), base = (raw_at + 1023) & ~1023u;
     unsigned char* smem = raw + (base - raw_at);
     Control& ct = *reinterpret_cast<Control*>(smem + L::kOffCtl);
     const MixParams& p = tp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // shares of the 512 x 128 registers of the launch: 128 S + 256 O + 128 M <= 65536
+    constexpr int kRegS = 208, kRegO = 112, kRegM = 64;
+    static_assert(128 * kRegS + 256 * kRegO + 128 * kRegM <= kThreads * 128, "register shares");
 
     // unit fastest: the jobs and heads that read the same tokens run side by side and share them in L2
     const int unit = blockIdx.x % tp.units, rest = blockIdx.x / tp.units;
@@ -260,17 +306,19 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     if (tid == 0) {
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(&ct.full[i], 1);
-            mbar_init(&ct.empty[i], STATE_ONLY ? 5 : 6);
+            mbar_init(&ct.empty[i], STATE_ONLY ? 1 : 2);
+            mbar_init(&ct.scanned[i], 1);
+            mbar_init(&ct.staged[i], 8);
         }
-        mbar_init(&ct.p_full, 1);
-        mbar_init(&ct.p_ready, 4);
-        mbar_init(&ct.b_ready, 4);
-        mbar_init(&ct.u_full, 1);
-        mbar_init(&ct.u_free, 4);
-        mbar_init(&ct.s_ready, 4);
+        mbar_init(&ct.p_ready, 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ct.p_full[i], 1);
+            mbar_init(&ct.b_ready[i], 4);
+            mbar_init(&ct.b_free[i], 1);
+        }
+        mbar_init(&ct.i_full, 1);
         mbar_init(&ct.o_full, 1);
-        mbar_init(&ct.x_free, 4);
-        mbar_init(&ct.staged, 4);
+        mbar_init(&ct.x_free, 8);
         mbar_init(&ct.drain, 1);
         ct.dead = 0;
         mbar_fence_init();
@@ -278,13 +326,11 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     if (tid < kC + 1) {
         const float w = decay_pow(p.log_decay[hs], tid);
         ct.pw[tid] = w;
-        if (jb.reverse) {
-            if (tid > 0) ct.wb[tid - 1] = w;
-        } else if (tid < kC) {
-            ct.wb[kC - 1 - tid] = w;
-        }
+        if (tid < kC) ct.ps[tid] = jb.p_scale * w;
+        // forwards w^(31 - k), backwards w^k
+        if (tid < 32) ct.wc[jb.reverse ? tid : 31 - tid] = jb.p_scale * w;
     }
-    if (warp == 9) {
+    if (warp == 13) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ct.tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -294,282 +340,384 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     tc_fence_after();
     const uint32_t tmem = ct.tmem;
 
-    const int n_chunk = (seg.len + kC - 1) / kC, share = GROUPED ? jb.share_b : 1, n_it = n_chunk * share;
+    const int n_chunk = (seg.len + kC - 1) / kC, share = jb.share_b, n_it = n_chunk * share;
     const int reverse = jb.reverse;
-    auto chunk_off = [&](int it) {
-        const int m = GROUPED ? it / share : it;
-        return (reverse ? n_chunk - 1 - m : m) * kC;
-    };
     const size_t sbase = ((size_t)item * p.state_heads + hs) * p.state_elems;
+    // visit `it` = (chunk m of the walk, query head g of the group); advanced without divisions
+    struct Visit {
+        int m = 0, g = 0, st = 0;
+        uint32_t lap = 0;  // parity of the ring
+    };
+    auto next = [&](Visit& v) {
+        if (++v.st == L::kStages) v.st = 0, v.lap ^= 1;
+        if (++v.g == share) v.g = 0, ++v.m;
+    };
+    // the scores of visit `it`: their TMEM region, their barrier and its parity
+    constexpr bool kTwice = L::kTwice;
+    auto p_buf = [&](int it) { return kTwice ? it & 1 : 0; };
+    auto p_par = [&](int it) { return kTwice ? (it >> 1) & 1 : it & 1; };
+    auto x_col = [&](const Visit& v) { return tmem + L::kColX + (kTwice ? (v.m & 1) * 64 : 0); };
+    auto offset = [&](const Visit& v) { return (reverse ? n_chunk - 1 - v.m : v.m) * kC; };
 
-    if (warp == 8) {
+    if (warp >= 12) regs_down<kRegM>();
+    if (warp == 12) {
         // ---- TMA
         if (lane == 0) {
             const CUtensorMap* ma = &tp.map[ji][0];
             const CUtensorMap* mb = &tp.map[ji][1];
             const CUtensorMap* mc = &tp.map[ji][2];
             int it = 0;
-            for (; it < n_it; ++it) {
-                const int st = it % L::kStages;
-                if (it >= L::kStages && !wait(ct, &ct.empty[st], (it / L::kStages - 1) & 1)) break;
-                const uint32_t at = base + st * L::kStage;
-                const int t = seg.t0 + chunk_off(it), hb = share > 1 ? head * share + it % share : hs;
-                mbar_expect_tx(&ct.full[st], L::kStage);
+            for (Visit v; it < n_it; ++it, next(v)) {
+                if (it >= L::kStages && !wait(ct, &ct.empty[v.st], v.lap ^ 1)) break;
+                const uint32_t at = base + v.st * L::kStage;
+                const int t = seg.t0 + offset(v), hb = share > 1 ? head * share + v.g : hs;
+                uint64_t* full = &ct.full[v.st];
+                mbar_expect_tx(full, L::kStage);
                 // b first: the state warps start on it
                 for (int q = 0; q < DA / 64; ++q)
-                    tma_load_4d(at + L::kA + q * kPanel, mb, &ct.full[st], q * 64, hb, t, seg.row);
+                    tma_load_4d(at + L::kA + q * kPanel, mb, full, q * 64, hb, t, seg.row);
                 if (!STATE_ONLY)
-                    for (int q = 0; q < DA / 64; ++q)
-                        tma_load_4d(at + q * kPanel, ma, &ct.full[st], q * 64, head, t, seg.row);
+                    for (int q = 0; q < DA / 64; ++q) tma_load_4d(at + q * kPanel, ma, full, q * 64, head, t, seg.row);
                 for (int q = 0; q < DC / 64; ++q)
-                    tma_load_4d(at + L::kA + L::kB + q * kPanel, mc, &ct.full[st], q * 64, hb, t, seg.row);
+                    tma_load_4d(at + L::kA + L::kB + q * kPanel, mc, full, q * 64, hb, t, seg.row);
             }
             if (it < n_it) drain_ring(ct.full, L::kStages, it, kDrainLimit);
         }
-    } else if (warp == 9) {
+    } else if (warp == 13) {
         // ---- MMA
         if (lane == 0) {
             constexpr uint32_t kScores = instr_desc(kC, false), kOut = instr_desc(DC, true);
-            bool ok = true;
-            for (int it = 0; it < n_it; ++it) {
-                const int st = it % L::kStages, g = GROUPED ? it % share : 0;
-                const uint32_t at = base + st * L::kStage, par = it & 1;
-                const uint32_t sa = at, sb = at + L::kA, sc = at + L::kA + L::kB;
-                if (!(ok = wait(ct, &ct.full[st], (it / L::kStages) & 1))) break;
-                if (!STATE_ONLY) {
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < DA / 16; ++k) {
-                        const uint32_t off = (k >> 2) * kPanel + (k & 3) * 32;
-                        mma_ss(tmem + kColP, smem_desc(sa + off, 16), smem_desc(sb + off, 16), kScores, k > 0);
-                    }
-                    tc_commit(&ct.p_full);
-                    if (g == 0) {
-                        const int m = GROUPED ? it / share : it;
-                        if (!(ok = wait(ct, &ct.s_ready, m & 1))) break;
-                        if (it > 0 && !(ok = wait(ct, &ct.x_free, (it - 1) & 1))) break;
-                        tc_fence_after();
-                        const uint32_t ss = base + L::kOffS;
-#pragma unroll
-                        for (int k = 0; k < DA / 16; ++k) {
-                            const uint32_t off = (k >> 2) * kPanel + (k & 3) * 32;
-                            mma_ss(tmem + kColI, smem_desc(sa + off, 16), smem_desc(ss + k * 2048, DA * 128), kOut,
-                                   k > 0);
-                        }
-                    } else if (!(ok = wait(ct, &ct.x_free, (it - 1) & 1))) {
-                        break;
-                    }
-                } else if (it > 0 && !(ok = wait(ct, &ct.u_free, (it - 1) & 1))) {
-                    break;
-                }
-                if (!(ok = wait(ct, &ct.b_ready, par))) break;
+            // scores of visit it (stage v.st); false: a wait ran out
+            auto scores = [&](int it, const Visit& v) {
+                if (!wait(ct, &ct.full[v.st], v.lap)) return false;
                 tc_fence_after();
+                const uint32_t sa = base + v.st * L::kStage;
+                const uint64_t da = smem_desc(sa, 16), db = smem_desc(sa + L::kA, 16);
+                const uint32_t to = tmem + L::kColP + p_buf(it) * 128;
 #pragma unroll
-                for (int k = 0; k < 2 * kC / 16; ++k)
-                    mma_ts(tmem + kColX, tmem + kColB + k * 8, smem_desc(sc + (k & 7) * 2048, kPanel), kOut, k > 0);
-                tc_commit(&ct.u_full);
-                if (!STATE_ONLY) {
-                    if (!(ok = wait(ct, &ct.p_ready, par)) || !(ok = wait(ct, &ct.u_free, par))) break;
+                for (int k = 0; k < DA / 16; ++k) {
+                    const uint64_t off = ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
+                    mma_ss(to, da + off, db + off, kScores, k > 0);
+                }
+                tc_commit(&ct.p_full[p_buf(it)]);
+                return true;
+            };
+            Visit v, ahead;
+            for (int it = kTwice && !STATE_ONLY ? -1 : 0; it < n_it; ++it) {
+                const uint32_t par = it & 1, mpar = v.m & 1;
+                if (STATE_ONLY) {
+                    if (!wait(ct, &ct.full[v.st], v.lap)) break;
+                } else if (kTwice) {
+                    // one visit ahead; the region is free when the product of visit it - 1 has ended
+                    if (it + 1 < n_it) {
+                        if (it > 0 && !wait(ct, &ct.o_full, par ^ 1)) break;
+                        if (!scores(it + 1, ahead)) break;
+                        next(ahead);
+                    }
+                    if (it < 0) continue;
+                } else {
+                    if (it > 0 && !wait(ct, &ct.o_full, par ^ 1)) break;
+                    if (!scores(it, v)) break;
+                }
+                const uint32_t sa = base + v.st * L::kStage;
+                const uint64_t dcd = smem_desc(sa + L::kA + L::kB, kPanel);
+                bool ok = true;
+#pragma unroll
+                for (int hf = 0; hf < L::kHalves; ++hf) {
+                    if (!(ok = wait(ct, &ct.b_ready[hf], par))) break;
+                    if (!STATE_ONLY && hf == 0 && v.g == 0) {
+                        // twice: p_ready of the last chunk told that the epilogue before it has read this X
+                        if (!kTwice && v.m > 0 && !(ok = wait(ct, &ct.x_free, mpar ^ 1))) break;
+                        tc_fence_after();
+                        const uint64_t da = smem_desc(sa, 16), ds = smem_desc(base + L::kOffS, 128 * 128);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint64_t off =
+                                kSplit ? (k & 3) * 32 >> 4 : ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
+                            mma_ss(x_col(v), da + off, ds + (k * 2048 >> 4), kOut, k > 0);
+                        }
+                        tc_commit(&ct.i_full);
+                    }
                     tc_fence_after();
 #pragma unroll
-                    for (int k = 0; k < kC / 16; ++k)
-                        mma_ts(tmem + kColX, tmem + kColP + (k >> 1) * 32 + (k & 1) * 8,
-                               smem_desc(sc + k * 2048, kPanel), kOut, k > 0);
-                    tc_commit(&ct.o_full);
-                    // the next scores overwrite the operand that these products read
-                    tc_commit(&ct.empty[st]);
-                    if (!(ok = wait(ct, &ct.o_full, par))) break;
-                } else {
-                    tc_commit(&ct.empty[st]);
+                    for (int k = 0; k < 8 / L::kHalves; ++k) {
+                        const uint64_t c = dcd + ((hf * 4 + k) * 2048 >> 4);
+                        const uint32_t bt = tmem + L::kColB + hf * 32 + k * 8;
+                        mma_ts(tmem + L::kColU, bt, c, kOut, v.g > 0 || hf > 0 || k > 0);
+                        if (!kSplit) mma_ts(tmem + L::kColU, bt + 64, c, kOut, true);
+                    }
+                    tc_commit(&ct.b_free[hf]);
                 }
+                if (!ok) break;
+                if (!STATE_ONLY) {
+                    if (!wait(ct, &ct.p_ready, par)) break;
+                    tc_fence_after();
+                    if (!*reinterpret_cast<volatile int*>(&ct.dirty[v.st])) {
+                        const uint32_t from = tmem + L::kColP + p_buf(it) * 128;
+#pragma unroll
+                        for (int k = 0; k < kC / 16; ++k)
+                            mma_ts(x_col(v), from + (k >> 1) * 32 + (k & 1) * 8, dcd + (k * 2048 >> 4), kOut, true);
+                    }
+                    tc_commit(&ct.o_full);
+                }
+                tc_commit(&ct.empty[v.st]);
+                next(v);
             }
             tc_commit(&ct.drain);
             mbar_wait_bounded(&ct.drain, 0, kWaitLimit);
         }
-    } else if (warp == 10) {
+    } else if (warp == 14) {
         // ---- store: whole chunks leave through TMA, ragged ones the output warps have written themselves
         if (!STATE_ONLY && lane == 0) {
-            for (int it = 0; it < n_it; ++it) {
-                const int st = it % L::kStages, off = chunk_off(it);
-                if (!wait(ct, &ct.staged, it & 1)) break;
-                if (seg.len - off >= kC && (!GROUPED || it % share == share - 1)) {
+            Visit v;
+            for (int it = 0; it < n_it; ++it, next(v)) {
+                if (!wait(ct, &ct.staged[v.st], v.lap)) break;
+                const int off = offset(v);
+                if (v.g == share - 1 && seg.len - off >= kC) {
                     for (int q = 0; q < DC / 64; ++q)
                         if (q * 64 < jb.dc)
-                            tma_store_4d(&tp.map[ji][3], base + st * L::kStage + q * kPanel, q * 64, head,
+                            tma_store_4d(&tp.map[ji][3], base + v.st * L::kStage + q * kPanel, q * 64, head,
                                          seg.t0 + off, seg.row);
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 }
-                mbar_arrive(&ct.empty[st]);
+                mbar_arrive(&ct.empty[v.st]);
             }
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
-    } else if (warp >= 4) {
-        // ---- state: thread r owns row r of S
-        const int r = tid - 128;
-        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // lane 32 * (warp % 4) in bits 31-16
-        const bool mine = (warp & 3) * 32 < DA;
-        float S[DC];
-#pragma unroll
-        for (int c = 0; c < DC; ++c)
-            S[c] = (!STATE_ONLY && jb.s_in && r < jb.da && c < jb.dc)
-                       ? jb.s_in[sbase + (size_t)r * jb.s_row + (size_t)c * jb.s_col]
-                       : 0.f;
-        unsigned char* ss = smem + L::kOffS;
-        auto publish = [&]() {
-            if (mine) {
-#pragma unroll
-                for (int c = 0; c < DC; c += 8) {
-                    uint4 v;
-                    v.x = pack_bf16(S[c], S[c + 1]);
-                    v.y = pack_bf16(S[c + 2], S[c + 3]);
-                    v.z = pack_bf16(S[c + 4], S[c + 5]);
-                    v.w = pack_bf16(S[c + 6], S[c + 7]);
-                    *reinterpret_cast<uint4*>(ss + (c >> 6) * (DA * 128) + r * 128 +
-                                              (((c & 63) * 2) ^ ((r & 7) << 4))) = v;
+    } else if (warp == 15) {
+        // ---- scan of c
+        if (!STATE_ONLY) {
+            Visit v;
+            for (int it = 0; it < n_it; ++it, next(v)) {
+                if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
+                const int rows = min(kC, seg.len - offset(v));
+                const unsigned char* tc = smem + v.st * L::kStage + L::kA + L::kB;
+                // 0 x inf and 0 x NaN are NaN
+                __nv_bfloat162 zero = __float2bfloat162_rn(0.f), sum[4] = {zero, zero, zero, zero};
+#pragma unroll 1
+                for (int q = 0; q < DC / 64; ++q)
+#pragma unroll 4
+                    for (int i = lane; i < rows * 8; i += 32) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(tc + q * kPanel + i * 16);
+                        sum[0] = __hfma2(as_bf162(x.x), zero, sum[0]);
+                        sum[1] = __hfma2(as_bf162(x.y), zero, sum[1]);
+                        sum[2] = __hfma2(as_bf162(x.z), zero, sum[2]);
+                        sum[3] = __hfma2(as_bf162(x.w), zero, sum[3]);
+                    }
+                const float2 f = __bfloat1622float2(__hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3])));
+                bool bad = !(f.x + f.y == 0.f);
+                bad = __any_sync(0xffffffffu, bad);
+                if (lane == 0) {
+                    ct.dirty[v.st] = bad;
+                    mbar_arrive(&ct.scanned[v.st]);
                 }
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ct.s_ready);
-        };
-        if (!STATE_ONLY && n_it > 0) publish();
-        for (int it = 0; it < n_it; ++it) {
-            const int st = it % L::kStages, g = GROUPED ? it % share : 0;
-            const int n = min(kC, seg.len - chunk_off(it));
-            if (!wait_warp(ct, &ct.full[st], (it / L::kStages) & 1)) break;
-            unsigned char* tile = smem + st * L::kStage + L::kA;
+        }
+    } else if (warp < 4) {
+        // ---- state: thread r owns row r of S (da = 64: row r - 64 of the low halves from thread 64 on)
+        regs_up<kRegS>();
+        const int r = tid;
+        const uint32_t lanes = tmem + ((uint32_t)warp << 21);  // lane 32 * warp in bits 31-16
+        float S[DC];
+        {
+            const bool given = !STATE_ONLY && jb.s_in && r < jb.da;
+            const float* from = given ? jb.s_in + sbase + (size_t)r * jb.s_row : nullptr;
+            const int limit = given ? jb.dc : 0;
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                S[c] = 0.f;
+                if (c < limit) S[c] = __ldg(from);
+                from += jb.s_col;
+            }
+        }
+        unsigned char* ss = smem + L::kOffS;
+        // channels of this warp's fragments, and whether it makes the low halves
+        const int d0 = (kSplit ? warp & 1 : warp) * 32;
+        const bool low = kSplit && warp >= 2;
+        const uint32_t from = base + L::kA + (d0 >> 6) * kPanel + (lane & 7) * 128 +
+                              ((((d0 & 63) + 8 * (lane >> 3)) * 2) ^ ((lane & 7) << 4));
+        bool ok = true;
+        int table_n = -1;
+        Visit v;
+        for (int it = 0; it < n_it; ++it, next(v)) {
+            const int n = min(kC, seg.len - offset(v));
+            const uint32_t par = it & 1;
+            if (!STATE_ONLY && v.g == 0) {
+                // S enters the chunk; the product with the last chunk's operand ended before that chunk's U
+#pragma unroll
+                for (int c = 0; c < DC; c += 8) {
+                    uint4 w;
+                    w.x = pack_bf16(S[c], S[c + 1]);
+                    w.y = pack_bf16(S[c + 2], S[c + 3]);
+                    w.z = pack_bf16(S[c + 4], S[c + 5]);
+                    w.w = pack_bf16(S[c + 6], S[c + 7]);
+                    *reinterpret_cast<uint4*>(ss + (c >> 6) * (128 * 128) + r * 128 +
+                                              (((c & 63) * 2) ^ ((r & 7) << 4))) = w;
+                }
+                fence_proxy_async();
+            }
+            if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
             if (n < kC) {
                 // tokens of the next sequence behind the last one of this: no value of theirs may reach a
                 // product, not even as 0 x inf
-                unsigned char* tc = tile + L::kB;
+                unsigned char* tb = smem + v.st * L::kStage + L::kA;
                 for (int i = n * 8 + r; i < kC * 8; i += 128)
 #pragma unroll
-                    for (int q = 0; q < DC / 64; ++q)
-                        *reinterpret_cast<uint4*>(tc + q * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
+                    for (int q = 0; q < (DA + DC) / 64; ++q)
+                        *reinterpret_cast<uint4*>(tb + q * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
             }
-            if (mine) {
-                const int d0 = (warp & 3) * 32, t2 = 2 * (lane & 3);
-                const uint32_t from = smem_u32(tile) + (d0 >> 6) * kPanel + (lane & 7) * 128 +
-                                      ((((d0 & 63) + 8 * (lane >> 3)) * 2) ^ ((lane & 7) << 4));
-#pragma unroll 1
-                for (int tg = 0; tg < kC / 8; tg += 2) {
-                    uint32_t hi[2][4], lo[2][4];
+            if (n != table_n) {
+                // the decays of this chunk length (all chunks but the ragged one have the same)
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (r < kC / 2) {
+                    float w[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        uint32_t f[4];
-                        ldmatrix_t(from + (tg + e) * 1024, f);
-                        const int t = (tg + e) * 8 + t2;
-                        float2 w = *reinterpret_cast<const float2*>(&ct.wb[t]);
-                        if (n < kC) {
-                            w.x = t < n ? ct.pw[reverse ? t + 1 : n - 1 - t] : 0.f;
-                            w.y = t + 1 < n ? ct.pw[reverse ? t + 2 : n - 2 - t] : 0.f;
-                            const uint32_t keep = (t < n ? 0xffffu : 0u) | (t + 1 < n ? 0xffff0000u : 0u);
+                        const int t = 2 * r + e;
+                        w[e] = t < n ? jb.upd_scale * ct.pw[reverse ? t + 1 : n - 1 - t] : 0.f;
+                    }
+                    const uint32_t h = pack_bf16(w[0], w[1]);
+                    ct.wb[r] = make_uint2(
+                        h, pack_bf16(w[0] - __uint_as_float(h << 16), w[1] - __uint_as_float(h & 0xffff0000u)));
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                table_n = n;
+            }
+            const uint32_t tile = from + v.st * L::kStage;
+#pragma unroll 1
+            for (int hf = 0; hf < L::kHalves; ++hf) {
+                if (it > 0 && !(ok = wait_warp(ct, &ct.b_free[hf], par ^ 1))) break;
+                tc_fence_after();
+                constexpr int kGroups = kC / 8 / L::kHalves;
+#pragma unroll 1
+                for (int tg = hf * kGroups; tg < hf * kGroups + kGroups; tg += 4) {
+                    // b w in two bf16 parts: high = rn(b wh), low = rn((b wh - high) + b wl), the bracket exact;
+                    // registers of lanes 0-15 and 16-31 of the warp's 32 channels, token groups tg .. tg+3
+                    uint32_t f[4][4], hi[2][8], lo[2][8];
+                    uint2 w[4];
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) f[q] &= keep;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        ldmatrix_t(tile + (tg + e) * 1024, f[e]);
+                        w[e] = ct.wb[(tg + e) * 4 + (lane & 3)];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const float2 v = __fmul2_rn(
-                                make_float2(__uint_as_float(f[q] << 16), __uint_as_float(f[q] & 0xffff0000u)), w);
-                            const uint32_t h = pack_bf16(v.x, v.y);
-                            hi[e][q] = h;
-                            lo[e][q] = pack_bf16(v.x - __uint_as_float(h << 16),
-                                                 v.y - __uint_as_float(h & 0xffff0000u));
+                            const __nv_bfloat162 b = as_bf162(f[e][q]), wh = as_bf162(w[e].x);
+                            const __nv_bfloat162 h = __hmul2_rn(b, wh);
+                            hi[q >> 1][2 * e + (q & 1)] = as_u32(h);
+                            if (!kSplit || low) {
+                                const uint32_t l = as_u32(__hfma2(b, as_bf162(w[e].y), __hfma2(b, wh, __hneg2(h))));
+                                (kSplit ? hi : lo)[q >> 1][2 * e + (q & 1)] = l;
+                            }
                         }
+                    const uint32_t col = lanes + L::kColB + tg * 4, low16 = 16u << 16;
+                    tmem_st_16x128b_x4(col, hi[0]);
+                    tmem_st_16x128b_x4(col + low16, hi[1]);
+                    if (!kSplit) {
+                        tmem_st_16x128b_x4(col + 64, lo[0]);
+                        tmem_st_16x128b_x4(col + 64 + low16, lo[1]);
                     }
-                    const uint32_t col = lanes + kColB + tg * 4, low16 = 16u << 16;
-                    tmem_st_16x128b_x2(col, hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
-                    tmem_st_16x128b_x2(col + low16, hi[0][2], hi[0][3], hi[1][2], hi[1][3]);
-                    tmem_st_16x128b_x2(col + 64, lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
-                    tmem_st_16x128b_x2(col + 64 + low16, lo[0][2], lo[0][3], lo[1][2], lo[1][3]);
                 }
                 tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ct.b_ready[hf]);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&ct.b_ready);
-                mbar_arrive(&ct.empty[st]);
-            }
-            if (!wait_warp(ct, &ct.u_full, it & 1)) break;
+            if (!ok) break;
+            if (v.g < share - 1) continue;
+            if (!wait_warp(ct, &ct.b_free[L::kHalves - 1], par)) break;  // U of the chunk is complete
             tc_fence_after();
-            const float wn = g == 0 ? ct.pw[n] : 1.f, us = jb.upd_scale;
-            if (mine) {
+            const float2 wn = make_float2(ct.pw[n], ct.pw[n]);
 #pragma unroll
-                for (int c0 = 0; c0 < DC; c0 += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(lanes + kColX + c0, v);
-                    tc_wait_ld();
+            for (int c0 = 0; c0 < DC; c0 += 32) {
+                uint32_t x[32];
+                tmem_ld32(lanes + L::kColU + c0, x);
+                tc_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) S[c0 + k] = fmaf(wn, S[c0 + k], us * __uint_as_float(v[k]));
+                for (int k = 0; k < 32; k += 2) {
+                    const float2 s2 = __ffma2_rn(wn, make_float2(S[c0 + k], S[c0 + k + 1]),
+                                                 make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])));
+                    S[c0 + k] = s2.x;
+                    S[c0 + k + 1] = s2.y;
                 }
             }
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ct.u_free);
-            // I = a S of this chunk has ended (committed before U): the operand may be replaced
-            if (!STATE_ONLY && g == share - 1 && it + 1 < n_it) publish();
         }
-        if (jb.s_out && head % jb.share_a == 0 && r < jb.da) {
+        if (jb.s_out && head % jb.share_a == 0) {
+            if (kSplit) {
+                // S = high + low: the low rows pass through the operand's place, which no product reads any more
+                float* ex = reinterpret_cast<float*>(ss);
+                if (r >= 64) {
 #pragma unroll
-            for (int c = 0; c < DC; ++c)
-                if (c < jb.dc) jb.s_out[sbase + (size_t)r * jb.s_row + (size_t)c * jb.s_col] = S[c];
+                    for (int c = 0; c < DC; ++c) ex[c * 64 + r - 64] = S[c];
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (r < 64) {
+#pragma unroll
+                    for (int c = 0; c < DC; ++c) S[c] += ex[c * 64 + r];
+                }
+            }
+            if (r < jb.da) {
+                float* to = jb.s_out + sbase + (size_t)r * jb.s_row;
+#pragma unroll
+                for (int c = 0; c < DC; ++c) {
+                    if (c < jb.dc) *to = S[c];
+                    to += jb.s_col;
+                }
+            }
         }
-    } else if (!STATE_ONLY) {
-        // ---- output: thread i owns row i of the chunk
-        const int i = tid;
-        const uint32_t lanes = tmem + ((uint32_t)warp << 21);
-        float acc[GROUPED ? DC : 1];
+    } else {
+        // ---- output: threads i and i + 128 own row i of the chunk
+        regs_down<kRegO>();
+        const int i = (tid - 128) & 127, half = warp >= 8, w4 = warp & 3;
+        const uint32_t lanes = tmem + ((uint32_t)w4 << 21);
+        constexpr int kCols = DC / 2;  // output channels of a thread
         __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(jb.out);
-        // column factors of the blocks off the diagonal: forwards w^(31 - k), backwards w^k
-        float2 colw[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            colw[k].x = jb.p_scale * ct.pw[reverse ? 2 * k : 31 - 2 * k];
-            colw[k].y = jb.p_scale * ct.pw[reverse ? 2 * k + 1 : 30 - 2 * k];
-        }
-        for (int it = 0; it < n_it; ++it) {
-            const int st = it % L::kStages, g = GROUPED ? it % share : 0;
-            const int off = chunk_off(it), n = min(kC, seg.len - off);
-            const uint32_t par = it & 1;
-            if (!wait_warp(ct, &ct.p_full, par)) break;
+        // scores of visit it: masked, decayed, to bf16 in place
+        auto convert = [&](int it, const Visit& v) {
+            const int n = min(kC, seg.len - offset(v));
+            if (!wait_warp(ct, &ct.p_full[p_buf(it)], p_par(it))) return false;
             tc_fence_after();
 #pragma unroll 1
-            for (int jc = 0; jc < 4; ++jc) {
-                uint32_t v[32], h[16];
-                if (reverse ? jc < warp : jc > warp) {
+            for (int jc = half; jc < 4; jc += 2) {  // blocks alternate, so that both halves have work
+                uint32_t x[32], h[16];
+                if (reverse ? jc < w4 : jc > w4) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) h[k] = 0u;
                 } else {
-                    tmem_ld32(lanes + kColP + jc * 32, v);
-                    const float row = ct.pw[jc == warp ? 0 : reverse ? jc * 32 - i : i - jc * 32 - 31];
+                    tmem_ld32(lanes + L::kColP + p_buf(it) * 128 + jc * 32, x);
+                    const float row = ct.pw[jc == w4 ? 0 : reverse ? jc * 32 - i : i - jc * 32 - 31];
                     tc_wait_ld();
-                    if (jc != warp) {
+                    if (jc != w4) {
                         const float2 row2 = make_float2(row, row);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float2 f = __fmul2_rn(
-                                make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])),
-                                __fmul2_rn(colw[k], row2));
-                            h[k] = pack_bf16(f.x, f.y);
+                        for (int k = 0; k < 16; k += 2) {
+                            const float4 w = *reinterpret_cast<const float4*>(&ct.wc[2 * k]);
+                            const float2 f0 = __fmul2_rn(
+                                make_float2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])),
+                                __fmul2_rn(make_float2(w.x, w.y), row2));
+                            const float2 f1 = __fmul2_rn(
+                                make_float2(__uint_as_float(x[2 * k + 2]), __uint_as_float(x[2 * k + 3])),
+                                __fmul2_rn(make_float2(w.z, w.w), row2));
+                            h[k] = pack_bf16(f0.x, f0.y);
+                            h[k + 1] = pack_bf16(f1.x, f1.y);
                         }
                     } else {
                         // a masked score is replaced, not multiplied by 0: it may be inf or NaN
-                        const float* pw = reverse ? ct.pw - lane : ct.pw + lane;
+                        const float* pw = reverse ? ct.ps - lane : ct.ps + lane;
+                        const int step = reverse ? 1 : -1;
+                        const uint32_t keep = reverse ? ~0u << lane : ~0u >> (31 - lane);
 #pragma unroll
                         for (int k = 0; k < 32; k += 2) {
-                            float f[2];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const bool in = reverse ? k + e >= lane : k + e <= lane;
-                                f[e] = 0.f;
-                                if (in)
-                                    f[e] = __uint_as_float(v[k + e]) *
-                                           (jb.p_scale * (reverse ? pw[k + e] : pw[-(k + e)]));
-                            }
-                            h[k >> 1] = pack_bf16(f[0], f[1]);
+                            // decays of masked places are never read: the address stays on the diagonal there
+                            const bool in0 = keep >> k & 1, in1 = keep >> (k + 1) & 1;
+                            const float f0 = __uint_as_float(x[k]) * pw[(in0 ? k : lane) * step];
+                            const float f1 = __uint_as_float(x[k + 1]) * pw[(in1 ? k + 1 : lane) * step];
+                            h[k >> 1] = pack_bf16(in0 ? f0 : 0.f, in1 ? f1 : 0.f);
                         }
                     }
                     if (reverse && n < kC) {
@@ -580,64 +728,88 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                         }
                     }
                 }
-                tmem_st16(lanes + kColP + jc * 32, h);
+                tmem_st16(lanes + L::kColP + p_buf(it) * 128 + jc * 32, h);
+            }
+            return true;
+        };
+        // X = w^pos X, and whatever keeps the matrix unit from adding the scores' product
+        auto scale = [&](int it, const Visit& v) {
+            const int off = offset(v), n = min(kC, seg.len - off);
+            const uint32_t mpar = v.m & 1;
+            if (!wait_warp(ct, &ct.scanned[v.st], v.lap)) return false;
+            const bool dirty = *reinterpret_cast<volatile int*>(&ct.dirty[v.st]) != 0;
+            if (v.g == 0) {
+                if (!wait_warp(ct, &ct.i_full, mpar)) return false;
+                tc_fence_after();
+                const float rw = i < n ? jb.row_scale * ct.pw[reverse ? n - 1 - i : i + 1] : 0.f;
+                const float2 rw2 = make_float2(rw, rw);
+#pragma unroll
+                for (int q = 0; q < kCols; q += 32) {
+                    const uint32_t at = lanes + (x_col(v) - tmem) + half * kCols + q;
+                    uint32_t x[32];
+                    tmem_ld32(at, x);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const float2 f =
+                            __fmul2_rn(make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), rw2);
+                        x[k] = __float_as_uint(f.x);
+                        x[k + 1] = __float_as_uint(f.y);
+                    }
+                    tmem_st32(at, x);
+                }
+            }
+            if (dirty) {
+                // the products so far are in X, and the matrix unit leaves this one out
+                tc_wait_st();
+                tc_fence_after();
+#pragma unroll 1
+                for (int c0 = half * kCols; c0 < half * kCols + kCols; c0 += 8) {
+                    uint32_t x[8];
+                    tmem_ld8(lanes + (x_col(v) - tmem) + c0, x);
+                    tc_wait_ld();
+                    float acc[8] = {};
+                    if (i < n && c0 < jb.dc)
+                        row_mix(jb, seg.row, seg.t0 + off, head, share > 1 ? head * share + v.g : hs, i, reverse ? i : 0,
+                                reverse ? n : i + 1, c0, ct.ps, acc);
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) + acc[k]);
+                    tmem_st8(lanes + (x_col(v) - tmem) + c0, x);
+                }
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ct.p_ready);
-            if (!wait_warp(ct, &ct.o_full, par)) break;
+            if (lane == 0) {
+                mbar_arrive(&ct.p_ready);
+                if (v.g < share - 1) mbar_arrive(&ct.staged[v.st]);
+            }
+            return true;
+        };
+        auto finish = [&](int it, const Visit& v) {
+            // every visit waits: p_ready of the next one tells the MMA thread that this product has ended
+            if (!wait_warp(ct, &ct.o_full, it & 1)) return false;
+            if (v.g < share - 1) return true;
+            const int off = offset(v), n = min(kC, seg.len - off);
             tc_fence_after();
-            const float rw = i < n ? jb.row_scale * ct.pw[reverse ? n - 1 - i : i + 1] : 0.f;
-            const float2 rw2 = make_float2(rw, rw);
-            const bool whole = n == kC, final = g == share - 1;
+            const bool whole = n == kC;
             __nv_bfloat16* dst = out + (((size_t)seg.row * p.map.time + seg.t0 + off + i) * jb.heads + head) * jb.dc;
-            unsigned char* tile = smem + st * L::kStage + i * 128;
-            float again[kC];
-            bool have = false;
+            unsigned char* tile = smem + v.st * L::kStage + i * 128;
 #pragma unroll
-            for (int c0 = 0; c0 < DC; c0 += 32) {
-                uint32_t x[32], in[32];
-                tmem_ld32(lanes + kColX + c0, x);
-                if (g == 0) tmem_ld32(lanes + kColI + c0, in);
+            for (int q = 0; q < kCols; q += 32) {
+                const int c0 = half * kCols + q;
+                uint32_t x[32];
+                tmem_ld32(lanes + (x_col(v) - tmem) + c0, x);
                 tc_wait_ld();
-                float2 o[16], bad = make_float2(0.f, 0.f);
-                const float2 zero = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    o[k] = make_float2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]));
-                    bad = __ffma2_rn(o[k], zero, bad);
-                }
-                if (!(bad.x + bad.y == 0.f) && i < n) {  // NaN: some o[k] is not finite
-                    const int j0 = reverse ? i : 0, j1 = reverse ? n : i + 1;
-                    const int hb = share > 1 ? head * share + g : hs;
-                    if (!have) row_scores(jb, seg.row, seg.t0 + off, head, hb, i, j0, j1, ct.pw, again);
-                    have = true;
-                    float t[32];
-                    row_mix(jb, seg.row, seg.t0 + off, hb, again, j0, j1, c0, t);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = make_float2(t[2 * k], t[2 * k + 1]);
-                }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    if (g == 0)
-                        o[k] = __ffma2_rn(rw2, make_float2(__uint_as_float(in[2 * k]), __uint_as_float(in[2 * k + 1])),
-                                          o[k]);
-                    if (GROUPED) {
-                        if (g > 0) o[k] = __fadd2_rn(o[k], make_float2(acc[c0 + 2 * k], acc[c0 + 2 * k + 1]));
-                        acc[c0 + 2 * k] = o[k].x;
-                        acc[c0 + 2 * k + 1] = o[k].y;
-                    }
-                }
-                if (!final) continue;
-#pragma unroll
-                for (int k = 0; k < 16; k += 4) {
+                for (int k = 0; k < 32; k += 8) {
                     uint4 w;
-                    w.x = pack_bf16(o[k].x, o[k].y);
-                    w.y = pack_bf16(o[k + 1].x, o[k + 1].y);
-                    w.z = pack_bf16(o[k + 2].x, o[k + 2].y);
-                    w.w = pack_bf16(o[k + 3].x, o[k + 3].y);
-                    const int c = c0 + 2 * k;
+                    w.x = pack_bf16(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                    w.y = pack_bf16(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+                    w.z = pack_bf16(__uint_as_float(x[k + 4]), __uint_as_float(x[k + 5]));
+                    w.w = pack_bf16(__uint_as_float(x[k + 6]), __uint_as_float(x[k + 7]));
+                    const int c = c0 + k;
                     if (whole)
                         *reinterpret_cast<uint4*>(tile + (c >> 6) * kPanel + (((c & 63) * 2) ^ ((i & 7) << 4))) = w;
                     else if (i < n && c < jb.dc)
@@ -649,14 +821,33 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&ct.x_free);
-                mbar_arrive(&ct.staged);
+                mbar_arrive(&ct.staged[v.st]);
+            }
+            return true;
+        };
+        Visit v, ahead;
+        if (!STATE_ONLY) {
+            if (kTwice) {
+                for (int it = -1; it < n_it; ++it) {
+                    if (it >= 0 && !scale(it, v)) break;
+                    if (it + 1 < n_it) {
+                        if (!convert(it + 1, ahead)) break;
+                        next(ahead);
+                    }
+                    if (it < 0) continue;
+                    if (!finish(it, v)) break;
+                    next(v);
+                }
+            } else {
+                for (int it = 0; it < n_it; ++it, next(v))
+                    if (!convert(it, v) || !scale(it, v) || !finish(it, v)) break;
             }
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 13) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
@@ -677,10 +868,10 @@ bool head_map(CUtensorMap* out, const HeadView& v, int d, int heads, int time, i
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DA, int DC, bool STATE_ONLY, bool GROUPED>
+template <int DA, int DC, bool STATE_ONLY>
 cudaError_t launch_g(const TcParams& tp, cudaStream_t s) {
     using L = Layout<DA, DC, STATE_ONLY>;
-    auto* fn = mix_tc_kernel<DA, DC, STATE_ONLY, GROUPED>;
+    auto* fn = mix_tc_kernel<DA, DC, STATE_ONLY>;
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
     if (e != cudaSuccess) return e;
     const long long grid = (long long)tp.units * tp.p.map.n_items * tp.p.state_heads;
@@ -689,17 +880,13 @@ cudaError_t launch_g(const TcParams& tp, cudaStream_t s) {
     return cudaGetLastError();
 }
 template <int DA, int DC>
-cudaError_t launch_d(const TcParams& tp, bool state_only, bool grouped, cudaStream_t s) {
-    if (state_only)
-        return grouped ? launch_g<DA, DC, true, true>(tp, s) : launch_g<DA, DC, true, false>(tp, s);
-    return grouped ? launch_g<DA, DC, false, true>(tp, s) : launch_g<DA, DC, false, false>(tp, s);
+cudaError_t launch_d(const TcParams& tp, bool state_only, cudaStream_t s) {
+    return state_only ? launch_g<DA, DC, true>(tp, s) : launch_g<DA, DC, false>(tp, s);
 }
 cudaError_t launch_set(const TcParams& tp, bool state_only, cudaStream_t s) {
-    bool grouped = false;
-    for (int j = 0; j < tp.p.n_jobs; ++j) grouped |= tp.p.job[j].share_b > 1;
     const bool a = tp.p.job[0].da > 64, c = tp.p.job[0].dc > 64;
-    if (a) return c ? launch_d<128, 128>(tp, state_only, grouped, s) : launch_d<128, 64>(tp, state_only, grouped, s);
-    return c ? launch_d<64, 128>(tp, state_only, grouped, s) : launch_d<64, 64>(tp, state_only, grouped, s);
+    if (a) return c ? launch_d<128, 128>(tp, state_only, s) : launch_d<128, 64>(tp, state_only, s);
+    return c ? launch_d<64, 128>(tp, state_only, s) : launch_d<64, 64>(tp, state_only, s);
 }
 
 }  // namespace
