@@ -872,8 +872,16 @@ template <int DA, int DC, bool STATE_ONLY>
 cudaError_t launch_g(const TcParams& tp, cudaStream_t s) {
     using L = Layout<DA, DC, STATE_ONLY>;
     auto* fn = mix_tc_kernel<DA, DC, STATE_ONLY>;
-    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
+    // the attribute is a property of the function on the device: set once for each
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
     const long long grid = (long long)tp.units * tp.p.map.n_items * tp.p.state_heads;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     fn<<<(unsigned)grid, kThreads, L::kBytes, s>>>(tp);

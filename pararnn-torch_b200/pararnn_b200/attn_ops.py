@@ -18,29 +18,33 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from .ops import (_attention_devices, _check_cuda, _dtype_code, _ptr, _raise, _stream, _workspace, gather_h0,
+from .ops import (_attention_devices, _check_cuda, _device_guard, _dtype_code, _once, _raise, _raw_stream, gather_h0,
                   validate_cu_seqlens)
+from .token_ops import _p, _scratch
 
 MAX_HEAD_DIM = 128
 
 
-def _heads_view(t: Tensor) -> Tensor:
-    """``t`` itself where the kernels can address it (unit channel stride, no broadcast axes, 16-byte
-    aligned rows for bf16), else a contiguous copy."""
-    t = t.detach()
-    if t.stride(-1) != 1 and t.shape[-1] > 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-        return t.contiguous()
-    if t.dtype == torch.bfloat16 and t.shape[-1] % 8 == 0:
-        bad = any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
-        if bad or t.data_ptr() % 16:
-            return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _heads_arg(t: Tensor):
-    # an axis of length 1 may carry any stride; the kernels multiply it by 0
-    st = [s if n > 1 else t.shape[-1] for s, n in zip(t.stride(), t.shape)]
-    return ctypes.byref(L.Heads(ctypes.c_void_p(t.data_ptr()), st[0], st[1], st[2]))
+def _heads(t: Tensor):
+    """``(tensor to keep alive, prb_heads)``: ``t`` itself where the kernels can address it (unit channel
+    stride, no broadcast axes, for bf16 16-byte aligned rows), else a contiguous copy."""
+    if not t.is_contiguous():
+        shape, st = t.shape, t.stride()
+        copy = st[3] != 1 and shape[3] > 1
+        for s, n in zip(st[:3], shape[:3]):
+            # an axis of length 1 may carry any stride
+            copy |= n > 1 and (s == 0 or (t.dtype == torch.bfloat16 and s % 8 != 0))
+        if copy:
+            t = t.contiguous()
+    ptr = t.data_ptr()
+    if ptr % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ptr = t.data_ptr()
+    _, n1, n2, n3 = t.shape
+    if t.is_contiguous():
+        return t, L.Heads(ptr, n1 * n2 * n3, n2 * n3, n3)
+    st = [s if n > 1 else n3 for s, n in zip(t.stride(), t.shape)]
+    return t, L.Heads(ptr, st[0], st[1], st[2])
 
 
 def _shapes(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor):
@@ -76,7 +80,7 @@ def _check_state(state: Tensor | None, shape: tuple[int, ...], name: str) -> Ten
         raise TypeError(f"{name} must be float32 (states are kept in 32 bits), got {state.dtype}")
     if tuple(state.shape) != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(state.shape)}")
-    return state.detach().contiguous()
+    return state.contiguous()
 
 
 def _offsets(cu_seqlens: Tensor | None, batch: int, time: int, dev):
@@ -98,6 +102,19 @@ def _offsets(cu_seqlens: Tensor | None, batch: int, time: int, dev):
     return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous(), len(cs) - 1, longest
 
 
+_ref = ctypes.byref
+
+
+def _decay(log_decay: Tensor) -> Tensor:
+    return log_decay.to(torch.float32).contiguous()
+
+
+def _maker(cu: Tensor | None):
+    """Checked offsets cover every token; those that a graph replays with may not, and tokens that no
+    sequence holds are left as they were: zeros."""
+    return torch.zeros if cu is not None and torch.cuda.is_current_stream_capturing() else torch.empty
+
+
 def linear_attention_fused(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor | None = None,
                            cu_seqlens: Tensor | None = None, *, scale: float | None = None,
                            want_state: bool = True):
@@ -108,20 +125,19 @@ def linear_attention_fused(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s
     cu, n_seq, longest = _offsets(cu_seqlens, B, T, dev)
     s_in = _check_state(state, (n_seq, Hkv, dk, dv), "state")
     scale = dk ** -0.5 if scale is None else float(scale)
-    qv, kv, vv = _heads_view(q), _heads_view(k), _heads_view(v)
-    g = log_decay.detach().to(torch.float32).contiguous()
-    # tokens that no sequence holds keep zeros (a captured call cannot check that there are none)
-    make = torch.zeros if cu is not None else torch.empty
-    out = make(B, T, Hq, dv, dtype=q.dtype, device=dev)
-    s_out = torch.empty(n_seq, Hkv, dk, dv, dtype=torch.float32, device=dev) if want_state else None
+    (qv, qh), (kv, kh), (vv, vh) = _heads(q), _heads(k), _heads(v)
+    g = _decay(log_decay)
+    make = _maker(cu)
+    out = make((B, T, Hq, dv), dtype=q.dtype, device=dev)
+    s_out = torch.empty((n_seq, Hkv, dk, dv), dtype=torch.float32, device=dev) if want_state else None
     lib = L.lib()
-    with torch.cuda.device(dev):
+    with _device_guard(dev):
         n = lib.prb_linear_attention_workspace_bytes(B, T, n_seq, longest, Hq, Hkv, dk, dv, code, cu is not None, 0)
-        ws = _workspace(n, dev)
-        rc = lib.prb_linear_attention(_heads_arg(qv), _heads_arg(kv), _heads_arg(vv), _ptr(g), _ptr(s_in), _ptr(cu),
-                                      _ptr(out), _ptr(s_out), B, T, n_seq, longest, Hq, Hkv, dk, dv, code, scale,
-                                      _ptr(ws), ws.numel(), _stream(dev))
-    _raise(rc, "linear_attention_fused")
+        ws = _scratch(n, dev)
+        rc = lib.prb_linear_attention(_ref(qh), _ref(kh), _ref(vh), _p(g), _p(s_in), _p(cu), _p(out), _p(s_out), B, T,
+                                      n_seq, longest, Hq, Hkv, dk, dv, code, scale, _p(ws), n, _raw_stream(dev))
+    if rc:
+        _raise(rc, "linear_attention_fused")
     _attention_devices.add(dev)
     return out, s_out
 
@@ -141,22 +157,22 @@ def linear_attention_reverse_vjp(q: Tensor, k: Tensor, v: Tensor, log_decay: Ten
     s_in = _check_state(state, (n_seq, Hkv, dk, dv), "state")
     gs = _check_state(grad_state, (n_seq, Hkv, dk, dv), "grad_state")
     scale = dk ** -0.5 if scale is None else float(scale)
-    qv, kv, vv, gv = _heads_view(q), _heads_view(k), _heads_view(v), _heads_view(grad_out.to(q.dtype))
-    g = log_decay.detach().to(torch.float32).contiguous()
-    make = torch.zeros if cu is not None else torch.empty
-    g_q = make(B, T, Hq, dk, dtype=q.dtype, device=dev)
-    g_k = make(B, T, Hkv, dk, dtype=q.dtype, device=dev)
-    g_v = make(B, T, Hkv, dv, dtype=q.dtype, device=dev)
-    g_s = torch.empty(n_seq, Hkv, dk, dv, dtype=torch.float32, device=dev) if want_state else None
+    (qv, qh), (kv, kh), (vv, vh), (gv, gh) = _heads(q), _heads(k), _heads(v), _heads(grad_out.to(q.dtype))
+    g = _decay(log_decay)
+    make = _maker(cu)
+    g_q = make((B, T, Hq, dk), dtype=q.dtype, device=dev)
+    g_k = make((B, T, Hkv, dk), dtype=q.dtype, device=dev)
+    g_v = make((B, T, Hkv, dv), dtype=q.dtype, device=dev)
+    g_s = torch.empty((n_seq, Hkv, dk, dv), dtype=torch.float32, device=dev) if want_state else None
     lib = L.lib()
-    with torch.cuda.device(dev):
+    with _device_guard(dev):
         n = lib.prb_linear_attention_workspace_bytes(B, T, n_seq, longest, Hq, Hkv, dk, dv, code, cu is not None, 1)
-        ws = _workspace(n, dev)
-        rc = lib.prb_bwd_linear_attention(_heads_arg(qv), _heads_arg(kv), _heads_arg(vv), _heads_arg(gv), _ptr(g),
-                                          _ptr(s_in), _ptr(gs), _ptr(cu), _ptr(g_q), _ptr(g_k), _ptr(g_v), _ptr(g_s),
-                                          B, T, n_seq, longest, Hq, Hkv, dk, dv, code, scale, _ptr(ws), ws.numel(),
-                                          _stream(dev))
-    _raise(rc, "linear_attention_reverse_vjp")
+        ws = _scratch(n, dev)
+        rc = lib.prb_bwd_linear_attention(_ref(qh), _ref(kh), _ref(vh), _ref(gh), _p(g), _p(s_in), _p(gs), _p(cu),
+                                          _p(g_q), _p(g_k), _p(g_v), _p(g_s), B, T, n_seq, longest, Hq, Hkv, dk, dv,
+                                          code, scale, _p(ws), n, _raw_stream(dev))
+    if rc:
+        _raise(rc, "linear_attention_reverse_vjp")
     _attention_devices.add(dev)
     return g_q, g_k, g_v, g_s
 
@@ -172,8 +188,8 @@ class _LinearAttention(torch.autograd.Function):
         return out, s_out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out, grad_state):
+        _once("linear_attention")
         q, k, v, log_decay, state, cu = ctx.saved_tensors
         if grad_out is None and grad_state is None:
             return (None,) * 8
@@ -265,12 +281,12 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         if not block_table.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a CUDA graph needs block_table on the device")
         bt = block_table.to(dev).contiguous()
-    q, k, v = q.detach().contiguous(), k.detach().contiguous(), v.detach().contiguous()
-    g = log_decay.detach().to(torch.float32).contiguous()
+    q, k, v, g = q.contiguous(), k.contiguous(), v.contiguous(), _decay(log_decay)
     scale = dk ** -0.5 if scale is None else float(scale)
-    with torch.cuda.device(dev):
-        rc = L.lib().prb_linear_attention_step(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state), _ptr(bt),
-                                               int(bt is not None and bt.dtype == torch.int64), _ptr(out), B,
-                                               state.shape[0], Hq, Hkv, dk, dv, code, scale, _stream(dev))
-    _raise(rc, "linear_attention_step")
+    with _device_guard(dev):
+        rc = L.lib().prb_linear_attention_step(_p(q), _p(k), _p(v), _p(g), _p(state), _p(bt),
+                                               bt is not None and bt.dtype == torch.int64, _p(out), B,
+                                               state.shape[0], Hq, Hkv, dk, dv, code, scale, _raw_stream(dev))
+    if rc:
+        _raise(rc, "linear_attention_step")
     return out

@@ -9,14 +9,22 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from .ops import _check_cuda, _dtype_code, _ptr, _raise, _stream, _workspace
+from .ops import _check_cuda, _device_guard, _dtype_code, _once, _raise, _raw_stream
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
 
 
 def _aligned(t: Tensor) -> Tensor:
-    t = t.detach().contiguous()
+    t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
+
+
+def _p(t: Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _scratch(nbytes: int, dev) -> Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
 # ------------------------------------------------------------------------------------ group norm
@@ -47,7 +55,7 @@ def _norm_shape(x: Tensor, num_groups: int, weight: Tensor | None, bias: Tensor 
 
 
 def _plain(p: Tensor | None) -> Tensor | None:
-    return None if p is None else p.detach().contiguous()
+    return None if p is None else p.contiguous()
 
 
 def group_norm_fused(x: Tensor, num_groups: int, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -57,14 +65,16 @@ def group_norm_fused(x: Tensor, num_groups: int, weight: Tensor | None = None, b
     code = _dtype_code(x)
     dev = _check_cuda(x, weight, bias)
     xc, w, b = _aligned(x), _plain(weight), _plain(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty(N, num_groups, 2, dtype=torch.float32, device=dev) if want_stats else None
+    y = torch.empty_like(xc)
+    stats = torch.empty((N, num_groups, 2), dtype=torch.float32, device=dev) if want_stats else None
     lib = L.lib()
-    with torch.cuda.device(dev):
-        ws = _workspace(lib.prb_group_norm_workspace_bytes(N, P, C, num_groups, code, 0), dev)
-        rc = lib.prb_group_norm(_ptr(xc), _ptr(w), _ptr(b), _ptr(y), _ptr(stats), N, P, C, num_groups, float(eps),
-                                ACTIVATIONS[activation], code, w_code, _ptr(ws), ws.numel(), _stream(dev))
-    _raise(rc, "group_norm_fused")
+    with _device_guard(dev):
+        need = lib.prb_group_norm_workspace_bytes(N, P, C, num_groups, code, 0)
+        ws = _scratch(need, dev)
+        rc = lib.prb_group_norm(_p(xc), _p(w), _p(b), _p(y), _p(stats), N, P, C, num_groups, eps,
+                                ACTIVATIONS[activation], code, w_code, _p(ws), need, _raw_stream(dev))
+    if rc:
+        _raise(rc, "group_norm_fused")
     return y, stats
 
 
@@ -79,16 +89,18 @@ def group_norm_vjp(x: Tensor, grad_y: Tensor, stats: Tensor, num_groups: int, we
         raise ValueError(f"stats must be float32 {(N, num_groups, 2)}, got {stats.dtype} {tuple(stats.shape)}")
     dev = _check_cuda(x, grad_y, stats, weight, bias)
     xc, gy, w, b, st = _aligned(x), _aligned(grad_y.to(x.dtype)), _plain(weight), _plain(bias), _plain(stats)
-    g_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    g_x = torch.empty_like(xc)
     g_w = torch.empty_like(w) if weight is not None and want_params else None
     g_b = torch.empty_like(b) if bias is not None and want_params else None
     lib = L.lib()
-    with torch.cuda.device(dev):
-        ws = _workspace(lib.prb_group_norm_workspace_bytes(N, P, C, num_groups, code, 1), dev)
-        rc = lib.prb_bwd_group_norm(_ptr(xc), _ptr(gy), _ptr(w), _ptr(b), _ptr(st), _ptr(g_x), _ptr(g_w), _ptr(g_b),
-                                    N, P, C, num_groups, ACTIVATIONS[activation], code, w_code, _ptr(ws), ws.numel(),
-                                    _stream(dev))
-    _raise(rc, "group_norm_vjp")
+    with _device_guard(dev):
+        need = lib.prb_group_norm_workspace_bytes(N, P, C, num_groups, code, 1)
+        ws = _scratch(need, dev)
+        rc = lib.prb_bwd_group_norm(_p(xc), _p(gy), _p(w), _p(b), _p(st), _p(g_x), _p(g_w), _p(g_b), N, P, C,
+                                    num_groups, ACTIVATIONS[activation], code, w_code, _p(ws), need,
+                                    _raw_stream(dev))
+    if rc:
+        _raise(rc, "group_norm_vjp")
     return g_x, g_w, g_b
 
 
@@ -101,8 +113,8 @@ class _GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y):
+        _once("group_norm")
         x, weight, bias, stats = ctx.saved_tensors
         num_groups, activation = ctx.args
         need = ctx.needs_input_grad
@@ -137,15 +149,16 @@ def embedding_fused(ids: Tensor, weight: Tensor, scale: float = 1.0) -> Tensor:
         raise ValueError(f"weight must be (vocab, channels), got {tuple(weight.shape)}")
     code = _dtype_code(weight)
     dev = _check_cuda(ids, weight)
-    idc, w = ids.contiguous(), weight.detach().contiguous()
+    idc, w = ids.contiguous(), weight.contiguous()
     V, C = w.shape
-    out = torch.empty(*ids.shape, C, dtype=w.dtype, device=dev)
+    out = torch.empty((*ids.shape, C), dtype=w.dtype, device=dev)
     if ids.numel() == 0:
         return out
-    with torch.cuda.device(dev):
-        rc = L.lib().prb_embedding(_ptr(idc), int(ids.dtype == torch.int64), _ptr(w), _ptr(out), ids.numel(), V, C,
-                                   code, float(scale), _stream(dev))
-    _raise(rc, "embedding_fused")
+    with _device_guard(dev):
+        rc = L.lib().prb_embedding(_p(idc), ids.dtype == torch.int64, _p(w), _p(out), ids.numel(), V, C, code, scale,
+                                   _raw_stream(dev))
+    if rc:
+        _raise(rc, "embedding_fused")
     return out
 
 
@@ -159,17 +172,19 @@ def embedding_vjp(ids: Tensor, grad_out: Tensor, vocab: int, scale: float = 1.0)
         raise ValueError(f"vocab must be >= 1, got {vocab}")
     code = _dtype_code(grad_out)
     dev = _check_cuda(ids, grad_out)
-    idc, g = ids.contiguous(), grad_out.detach().contiguous()
+    idc, g = ids.contiguous(), grad_out.contiguous()
     C = grad_out.shape[-1]
     if ids.numel() == 0:
         return torch.zeros(vocab, C, dtype=g.dtype, device=dev)
-    out = torch.empty(vocab, C, dtype=g.dtype, device=dev)
+    out = torch.empty((vocab, C), dtype=g.dtype, device=dev)
     lib = L.lib()
-    with torch.cuda.device(dev):
-        ws = _workspace(lib.prb_bwd_embedding_workspace_bytes(ids.numel(), vocab, C), dev)
-        rc = lib.prb_bwd_embedding(_ptr(idc), int(ids.dtype == torch.int64), _ptr(g), _ptr(out), ids.numel(), vocab,
-                                   C, code, float(scale), _ptr(ws), ws.numel(), _stream(dev))
-    _raise(rc, "embedding_vjp")
+    with _device_guard(dev):
+        need = lib.prb_bwd_embedding_workspace_bytes(ids.numel(), vocab, C)
+        ws = _scratch(need, dev)
+        rc = lib.prb_bwd_embedding(_p(idc), ids.dtype == torch.int64, _p(g), _p(out), ids.numel(), vocab, C, code,
+                                   scale, _p(ws), need, _raw_stream(dev))
+    if rc:
+        _raise(rc, "embedding_vjp")
     return out
 
 
@@ -181,8 +196,8 @@ class _Embedding(torch.autograd.Function):
         return embedding_fused(ids, weight, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
+        _once("embedding")
         (ids,) = ctx.saved_tensors
         vocab, scale, dtype = ctx.args
         return None, embedding_vjp(ids, grad_out.to(dtype), vocab, scale), None
