@@ -18,15 +18,19 @@ struct AttnShape {
     int dtype, rows, time, n_seq, max_len, hq, hkv, dk, dv;
 };
 
-// Segments of the time axis.  One CTA walks a segment of one head, so few (sequence, head) pairs leave
-// SMs idle; cutting costs a second read of two inputs (the state sweep) and two more launches.
+// Segments of the time axis.  One CTA walks a segment of one head (and of one block of 64 value channels on
+// the CUDA cores), so few (sequence, head) pairs leave SMs idle; cutting costs a second read of two
+// inputs (the state sweep) and two more launches, some 12 us.  A segment has at least kMinSegment
+// tokens, which take about as long: 8 chunks of 128 on the tensor cores, 4 of 64 on the CUDA cores.
 SegMap plan_segments(const AttnShape& s, const int* cu, bool backward) {
     SegMap m{};
     m.cu = cu;
     m.n_seq = s.n_seq;
     m.time = s.time;
-    const int chunk = 128, sm = sm_count();
-    const long long jobs = backward ? (long long)s.hq + 2 * s.hkv : s.hq;
+    const int chunk = 128, sm = sm_count(), least = s.dtype == PRB_F32 ? 2 * chunk : 8 * chunk;
+    const int blocks_v = s.dtype == PRB_F32 ? (s.dv + 63) / 64 : 1, blocks_k = s.dtype == PRB_F32 ? (s.dk + 63) / 64 : 1;
+    const long long jobs =
+        backward ? (long long)s.hq * blocks_k + s.hkv * (blocks_k + blocks_v) : (long long)s.hq * blocks_v;
     const long long tokens = cu ? s.time : (long long)s.rows * s.time;
     long long len = s.max_len;
     if ((long long)s.n_seq * jobs < sm) {
@@ -34,7 +38,7 @@ SegMap plan_segments(const AttnShape& s, const int* cu, bool backward) {
         const long long cuts = sm / (s.n_seq * jobs);
         len = cu ? (tokens * jobs + sm - 1) / sm : (s.time + cuts - 1) / cuts;
         len = (len + chunk - 1) / chunk * chunk;
-        if (len < 8 * chunk) len = 8 * chunk;
+        if (len < least) len = least;
     }
     if (len >= s.max_len) {
         m.seg_len = s.max_len;
@@ -246,7 +250,7 @@ int prb_linear_attention_step(const void* q, const void* k, const void* v, const
 size_t prb_group_norm_workspace_bytes(long long samples, int positions, int channels, int groups, int dtype,
                                       int backward) {
     if (samples < 1 || positions < 1 || channels < 1 || groups < 1 || channels % groups || bad_type(dtype)) return 0;
-    const GroupNormPlan pl = groupnorm_plan(dtype, samples, positions, channels, groups);
+    const GroupNormPlan pl = groupnorm_plan(dtype, samples, positions, channels, groups, backward != 0);
     return (pl.group_floats + (backward ? 2 * (size_t)pl.part_rows * channels : 0)) * sizeof(float);
 }
 
@@ -262,7 +266,7 @@ static int group_norm(GroupNormArgs& a, int dtype, int weight_dtype, bool backwa
     if ((long long)a.channels > 256ll * 65535 || a.channels > (1 << 30)) return PRB_ERR_UNSUPPORTED;
     const size_t need = prb_group_norm_workspace_bytes(a.samples, a.positions, a.channels, a.groups, dtype, backward);
     if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < need)) return PRB_ERR_WORKSPACE;
-    const GroupNormPlan pl = groupnorm_plan(dtype, a.samples, a.positions, a.channels, a.groups);
+    const GroupNormPlan pl = groupnorm_plan(dtype, a.samples, a.positions, a.channels, a.groups, backward);
     a.group_part = reinterpret_cast<float*>(ws);
     a.partial = a.group_part + pl.group_floats;
     a.w_f32 = weight_dtype == PRB_F32;

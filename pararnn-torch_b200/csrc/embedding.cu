@@ -60,11 +60,18 @@ __global__ void __launch_bounds__(kT) embed_fwd(const __grid_constant__ EmbedArg
     }
 }
 
+// one atomic for all lanes of a warp that hold the same id: frequent tokens queue 32 times less
 __global__ void __launch_bounds__(kT) embed_count(const __grid_constant__ EmbedArgs a, int* counts, int* rank) {
     const long long t = (long long)blockIdx.x * kT + threadIdx.x;
-    if (t >= a.tokens) return;
-    const long long id = id_at(a, t);
-    rank[t] = (id >= 0 && id < a.vocab) ? atomicAdd(counts + id, 1) : -1;
+    const long long id = t < a.tokens ? id_at(a, t) : -1;
+    const bool in = id >= 0 && id < a.vocab;
+    const int key = in ? (int)id : -1;
+    const unsigned peers = __match_any_sync(0xffffffffu, key);
+    const int lane = threadIdx.x & 31, leader = __ffs(peers) - 1;
+    int first = 0;
+    if (in && lane == leader) first = atomicAdd(counts + key, __popc(peers));
+    first = __shfl_sync(0xffffffffu, first, leader);
+    if (t < a.tokens) rank[t] = in ? first + __popc(peers & ((1u << lane) - 1)) : -1;
 }
 
 // counters: [0] list cursor, [1] long segments, [2] pieces
@@ -177,22 +184,30 @@ __device__ __forceinline__ void row_sum(const EmbedArgs& a, int v, int n, int mi
     const int nv = a.channels / V;
     const Vec<T, V>* src = reinterpret_cast<const Vec<T, V>*>(a.dy);
     Vec<T, V>* dst = reinterpret_cast<Vec<T, V>*>(a.out) + (size_t)v * nv;
-    for (int i0 = 0; i0 < nv; i0 += 32) {
-        const int i = i0 + lane;
-        float acc[V] = {};
-#pragma unroll 4
+    constexpr int kCols = V == 8 ? 3 : 4;  // vectors of a lane per turn: their loads are in flight together
+    for (int i0 = 0; i0 < nv; i0 += 32 * kCols) {
+        float acc[kCols][V] = {};
+#pragma unroll 2
         for (int j = 0; j < n; ++j) {
-            const long long t = __shfl_sync(0xffffffffu, mine, j);
-            if (i < nv) {
-                const Vec<T, V> x = src[t * nv + i];
+            const Vec<T, V>* from = src + (long long)__shfl_sync(0xffffffffu, mine, j) * nv + i0 + lane;
+            Vec<T, V> x[kCols];
 #pragma unroll
-                for (int k = 0; k < V; ++k) acc[k] += static_cast<float>(x.v[k]);
-            }
+            for (int c = 0; c < kCols; ++c)
+                if (i0 + c * 32 + lane < nv) x[c] = from[c * 32];
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+                if (i0 + c * 32 + lane < nv) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) acc[c][k] += static_cast<float>(x[c].v[k]);
+                }
         }
-        if (i < nv) {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            const int i = i0 + c * 32 + lane;
+            if (i >= nv) break;
             Vec<T, V> y;
 #pragma unroll
-            for (int k = 0; k < V; ++k) st_f(&y.v[k], a.scale * acc[k]);
+            for (int k = 0; k < V; ++k) st_f(&y.v[k], a.scale * acc[c][k]);
             dst[i] = y;
         }
     }
@@ -232,15 +247,17 @@ __global__ void __launch_bounds__(kT) embed_sums(const __grid_constant__ EmbedAr
 template <typename T>
 __global__ void __launch_bounds__(kT) embed_join(const __grid_constant__ EmbedArgs a, const int* counters,
                                                  const LongSeg* segs, const float* partial) {
-    if ((int)blockIdx.x >= counters[1]) return;
-    const LongSeg sg = segs[blockIdx.x];
-    const int pieces = (sg.n + sg.piece_len - 1) / sg.piece_len;
-    T* dst = reinterpret_cast<T*>(a.out) + (size_t)sg.id * a.channels;
-    for (int c = blockIdx.y * kT + threadIdx.x; c < a.channels; c += kT * gridDim.y) {
-        float s = 0.f;
+    const int longs = counters[1];
+    for (int i = blockIdx.x; i < longs; i += gridDim.x) {
+        const LongSeg sg = segs[i];
+        const int pieces = (sg.n + sg.piece_len - 1) / sg.piece_len;
+        T* dst = reinterpret_cast<T*>(a.out) + (size_t)sg.id * a.channels;
+        for (int c = blockIdx.y * kT + threadIdx.x; c < a.channels; c += kT * gridDim.y) {
+            float s = 0.f;
 #pragma unroll 8
-        for (int k = 0; k < pieces; ++k) s += partial[(size_t)(sg.piece0 + k) * a.channels + c];
-        st_f(dst + c, a.scale * s);
+            for (int k = 0; k < pieces; ++k) s += partial[(size_t)(sg.piece0 + k) * a.channels + c];
+            st_f(dst + c, a.scale * s);
+        }
     }
 }
 
@@ -284,7 +301,7 @@ cudaError_t grad_t(const EmbedArgs& a, const EmbedPlan& pl, char* ws, cudaStream
                                                   pieces);
     if (longs) {
         const int cols = (a.channels + kT - 1) / kT;
-        embed_join<T><<<dim3(longs, cols < 64 ? cols : 64), kT, 0, s>>>(a, counters, segs, partial);
+        embed_join<T><<<dim3(longs < 2 * sm_count() ? longs : 2 * sm_count(), cols < 64 ? cols : 64), kT, 0, s>>>(a, counters, segs, partial);
     }
     return cudaGetLastError();
 }

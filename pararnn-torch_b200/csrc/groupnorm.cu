@@ -22,23 +22,47 @@ namespace prb {
 namespace {
 
 constexpr int kT = 256;
+// CTAs per SM of the persistent row kernels (one vector per lane) and of the slab kernels; the grids are
+// whole waves of them.  Holding the next row's data in registers while a row is worked on keeps
+// 24 - 32 KB per SM in flight.
+constexpr int kRowCtasFwd = 5, kRowCtasBwd = 3, kSlabCtas = 4;
 constexpr int kMaxLocal = kT + 2;  // groups that one CTA's channels can touch
+constexpr int kBatch = 4, kPair = 3;  // positions whose loads a thread issues together (one input, two inputs)
 
+// V neighbouring channels as they lie in memory; loads are issued well before their conversion
 template <typename T, int V>
 struct __align__(sizeof(T) * V) Pack {
     T v[V];
 };
 template <typename T, int V>
-__device__ __forceinline__ void load_v(float (&r)[V], const T* p) {
-    const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(p);
+__device__ __forceinline__ Pack<T, V> load_raw(const T* p) {
+    return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack(float (&r)[V], const Pack<T, V>& u) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = static_cast<float>(u.v[i]);
+        for (int i = 0; i < V / 2; ++i) {
+            r[2 * i] = __uint_as_float(w[i] << 16);
+            r[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = static_cast<float>(u.v[i]);
+    }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_v(T* p, const float (&r)[V]) {
     Pack<T, V> u;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(&u);
 #pragma unroll
-    for (int i = 0; i < V; ++i) st_f(&u.v[i], r[i]);
+        for (int i = 0; i < V / 2; ++i) w[i] = __floats2bfloat162_rn(r[2 * i], r[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) st_f(&u.v[i], r[i]);
+    }
     *reinterpret_cast<Pack<T, V>*>(p) = u;
 }
 __device__ __forceinline__ float affine(const void* p, int f32, int i, float none) {
@@ -93,98 +117,121 @@ __device__ __forceinline__ RowSlot row_slot(int groups) {
 }
 
 template <typename T, int V, int NV, int LANES, int ACT>
-__global__ void __launch_bounds__(kT) gn_rows_fwd(const __grid_constant__ GroupNormArgs p) {
+__global__ void __launch_bounds__(kT, NV == 1 ? kRowCtasFwd : 2) gn_rows_fwd(const __grid_constant__ GroupNormArgs p) {
     const RowSlot rs = row_slot<LANES>(p.groups);
     const int cg = p.channels / p.groups;
     float w[NV][V], b[NV][V];
+    bool in[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+        in[j] = rs.live && (j * LANES + rs.lane) * V < cg;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = (j * LANES + rs.lane) * V + i;
-            const bool in = rs.live && c < cg;
-            w[j][i] = in ? affine(p.w, p.w_f32, rs.g * cg + c, 1.f) : 0.f;
-            b[j][i] = in ? affine(p.b, p.w_f32, rs.g * cg + c, 0.f) : 0.f;
+            const int c = rs.g * cg + (j * LANES + rs.lane) * V + i;
+            w[j][i] = in[j] ? affine(p.w, p.w_f32, c, 1.f) : 0.f;
+            b[j][i] = in[j] ? affine(p.b, p.w_f32, c, 0.f) : 0.f;
         }
+    }
     const float inv = 1.f / cg;
-    for (long long r0 = (long long)blockIdx.x * rs.rows; r0 < p.samples; r0 += (long long)gridDim.x * rs.rows) {
-        const long long row = r0 + rs.sub;
-        const bool live = rs.live && row < p.samples;
-        const size_t at = (size_t)row * p.channels + (size_t)rs.g * cg;
+    const size_t step = (size_t)gridDim.x * rs.rows;
+    const size_t col = (size_t)rs.g * cg + rs.lane * V;
+    size_t row = (size_t)blockIdx.x * rs.rows + rs.sub;
+    Pack<T, V> raw[NV] = {};
+    auto fetch = [&](size_t r) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (in[j] && r < (size_t)p.samples)
+                raw[j] = load_raw<T, V>(reinterpret_cast<const T*>(p.x) + r * p.channels + col + j * LANES * V);
+    };
+    fetch(row);
+    // all threads of a CTA take the same number of turns: the shuffles need whole warps
+    for (size_t r0 = (size_t)blockIdx.x * rs.rows; r0 < (size_t)p.samples; r0 += step, row += step) {
         float x[NV][V];
         float s = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * LANES + rs.lane) * V;
-            if (live && c < cg) {
-                load_v<T, V>(x[j], reinterpret_cast<const T*>(p.x) + at + c);
+            unpack<T, V>(x[j], raw[j]);
+            if (in[j]) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) s += x[j][i];
             }
         }
+        fetch(row + step);
         const float mean = lane_sum<LANES>(s) * inv;
         float m2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (live && (j * LANES + rs.lane) * V < cg) {
+            if (in[j]) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float d = x[j][i] - mean;
-                    m2 = fmaf(d, d, m2);
+                    x[j][i] -= mean;
+                    m2 = fmaf(x[j][i], x[j][i], m2);
                 }
             }
         const float rstd = rsqrtf(lane_sum<LANES>(m2) * inv + p.eps);
-        if (!live) continue;
-        if (rs.lane == 0 && p.stats) p.stats[(size_t)row * p.groups + rs.g] = make_float2(mean, rstd);
+        if (!rs.live || row >= (size_t)p.samples) continue;
+        if (rs.lane == 0 && p.stats) p.stats[row * p.groups + rs.g] = make_float2(mean, rstd);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * LANES + rs.lane) * V;
-            if (c >= cg) continue;
-            float y[V];
+            if (!in[j]) continue;
 #pragma unroll
-            for (int i = 0; i < V; ++i) y[i] = act<ACT>(fmaf((x[j][i] - mean) * rstd, w[j][i], b[j][i]));
-            store_v<T, V>(reinterpret_cast<T*>(p.y) + at + c, y);
+            for (int i = 0; i < V; ++i) x[j][i] = act<ACT>(fmaf(x[j][i] * rstd, w[j][i], b[j][i]));
+            store_v<T, V>(reinterpret_cast<T*>(p.y) + row * p.channels + col + j * LANES * V, x[j]);
         }
     }
 }
 
 template <typename T, int V, int NV, int LANES, int ACT>
-__global__ void __launch_bounds__(kT) gn_rows_bwd(const __grid_constant__ GroupNormArgs p) {
+__global__ void __launch_bounds__(kT, NV == 1 ? kRowCtasBwd : 1) gn_rows_bwd(const __grid_constant__ GroupNormArgs p) {
     const RowSlot rs = row_slot<LANES>(p.groups);
     const int cg = p.channels / p.groups;
     float w[NV][V], b[NV][V], dw[NV][V] = {}, db[NV][V] = {};
+    bool in[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+        in[j] = rs.live && (j * LANES + rs.lane) * V < cg;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = (j * LANES + rs.lane) * V + i;
-            const bool in = rs.live && c < cg;
-            w[j][i] = in ? affine(p.w, p.w_f32, rs.g * cg + c, 1.f) : 0.f;
-            b[j][i] = in ? affine(p.b, p.w_f32, rs.g * cg + c, 0.f) : 0.f;
+            const int c = rs.g * cg + (j * LANES + rs.lane) * V + i;
+            w[j][i] = in[j] ? affine(p.w, p.w_f32, c, 1.f) : 0.f;
+            b[j][i] = in[j] ? affine(p.b, p.w_f32, c, 0.f) : 0.f;
         }
+    }
     const float inv = 1.f / cg;
-    for (long long r0 = (long long)blockIdx.x * rs.rows; r0 < p.samples; r0 += (long long)gridDim.x * rs.rows) {
-        const long long row = r0 + rs.sub;
-        const bool live = rs.live && row < p.samples;
-        const size_t at = (size_t)row * p.channels + (size_t)rs.g * cg;
-        float2 st = make_float2(0.f, 0.f);
-        if (live) st = p.stats[(size_t)row * p.groups + rs.g];
+    const size_t step = (size_t)gridDim.x * rs.rows;
+    const size_t col = (size_t)rs.g * cg + rs.lane * V;
+    size_t row = (size_t)blockIdx.x * rs.rows + rs.sub;
+    Pack<T, V> raw_x[NV] = {}, raw_d[NV] = {};
+    float2 st = make_float2(0.f, 0.f);
+    auto fetch = [&](size_t r) {
+        if (!rs.live || r >= (size_t)p.samples) return;
+        st = p.stats[r * p.groups + rs.g];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (in[j]) {
+                const size_t at = r * p.channels + col + j * LANES * V;
+                raw_x[j] = load_raw<T, V>(reinterpret_cast<const T*>(p.x) + at);
+                raw_d[j] = load_raw<T, V>(reinterpret_cast<const T*>(p.dy) + at);
+            }
+    };
+    fetch(row);
+    for (size_t r0 = (size_t)blockIdx.x * rs.rows; r0 < (size_t)p.samples; r0 += step, row += step) {
+        const bool live = rs.live && row < (size_t)p.samples;
+        const float2 ms = st;
         float h[NV][V], d[NV][V];  // xhat, then w du
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            unpack<T, V>(h[j], raw_x[j]);
+            unpack<T, V>(d[j], raw_d[j]);
+        }
+        fetch(row + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * LANES + rs.lane) * V;
-            if (live && c < cg) {
-                load_v<T, V>(h[j], reinterpret_cast<const T*>(p.x) + at + c);
-                load_v<T, V>(d[j], reinterpret_cast<const T*>(p.dy) + at + c);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            if (live && (j * LANES + rs.lane) * V < cg) {
+            if (live && in[j]) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    h[j][i] = (h[j][i] - st.x) * st.y;
+                    h[j][i] = (h[j][i] - ms.x) * ms.y;
                     const float du = d[j][i] * act_slope<ACT>(fmaf(h[j][i], w[j][i], b[j][i]));
                     dw[j][i] = fmaf(du, h[j][i], dw[j][i]);
                     db[j][i] += du;
@@ -199,12 +246,10 @@ __global__ void __launch_bounds__(kT) gn_rows_bwd(const __grid_constant__ GroupN
         if (!live) continue;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * LANES + rs.lane) * V;
-            if (c >= cg) continue;
-            float dx[V];
+            if (!in[j]) continue;
 #pragma unroll
-            for (int i = 0; i < V; ++i) dx[i] = st.y * (d[j][i] - s1 - h[j][i] * s2);
-            store_v<T, V>(reinterpret_cast<T*>(p.dx) + at + c, dx);
+            for (int i = 0; i < V; ++i) d[j][i] = ms.y * (d[j][i] - s1 - h[j][i] * s2);
+            store_v<T, V>(reinterpret_cast<T*>(p.dx) + row * p.channels + col + j * LANES * V, d[j]);
         }
     }
     // one row of partial sums per CTA: its rows in order of `sub`
@@ -219,9 +264,8 @@ __global__ void __launch_bounds__(kT) gn_rows_bwd(const __grid_constant__ GroupN
             red[1][threadIdx.x][i] = db[j][i];
         }
         __syncthreads();
-        const int c = (j * LANES + rs.lane) * V;
-        if (rs.live && rs.sub == 0 && c < cg) {
-            float* dst = p.partial + (size_t)blockIdx.x * 2 * p.channels + rs.g * cg + c;
+        if (rs.sub == 0 && in[j]) {
+            float* dst = p.partial + (size_t)blockIdx.x * 2 * p.channels + col + j * LANES * V;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float a0 = 0.f, a1 = 0.f;
@@ -297,7 +341,7 @@ __device__ __forceinline__ void group_blocks(const GroupNormArgs& p, int g, int&
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kT) gn_slab_stats(const __grid_constant__ GroupNormArgs p) {
+__global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_stats(const __grid_constant__ GroupNormArgs p) {
     __shared__ float sn[kT], sm[kT], sv[kT];
     const SlabSlot s = slab_slot<V>(p);
     const size_t n = p.sample0 + blockIdx.y;
@@ -305,19 +349,27 @@ __global__ void __launch_bounds__(kT) gn_slab_stats(const __grid_constant__ Grou
     // sums about the thread's first value, so that a large mean cancels nothing
     float pivot = 0.f, s1 = 0.f, s2 = 0.f, cnt = 0.f;
     if (s.live && s.p0 + s.sub < s.p1) {
-        float v[V];
-        load_v<T, V>(v, x + (size_t)(s.p0 + s.sub) * p.channels);
-        pivot = v[0];
-#pragma unroll 4
-        for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
-            load_v<T, V>(v, x + (size_t)q * p.channels);
+        pivot = static_cast<float>(x[(size_t)(s.p0 + s.sub) * p.channels]);
+        for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kBatch * s.rows) {
+            Pack<T, V> raw[kBatch];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float d = v[i] - pivot;
-                s1 += d;
-                s2 = fmaf(d, d, s2);
+            for (int e = 0; e < kBatch; ++e) {
+                const int q = min(q0 + e * s.rows, s.p1 - 1);
+                raw[e] = load_raw<T, V>(x + (size_t)q * p.channels);
             }
-            cnt += V;
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                if (q0 + e * s.rows >= s.p1) break;
+                float v[V];
+                unpack<T, V>(v, raw[e]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = v[i] - pivot;
+                    s1 += d;
+                    s2 = fmaf(d, d, s2);
+                }
+                cnt += V;
+            }
         }
     }
     const float m = cnt > 0.f ? s1 / cnt : 0.f;
@@ -346,7 +398,7 @@ __global__ void __launch_bounds__(kT) gn_slab_stats(const __grid_constant__ Grou
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kT) gn_slab_fwd(const __grid_constant__ GroupNormArgs p) {
+__global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_fwd(const __grid_constant__ GroupNormArgs p) {
     __shared__ float2 st[kMaxLocal];
     const SlabSlot s = slab_slot<V>(p);
     const size_t n = p.sample0 + blockIdx.y;
@@ -379,18 +431,28 @@ __global__ void __launch_bounds__(kT) gn_slab_fwd(const __grid_constant__ GroupN
         b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
     }
     const size_t base = n * p.positions * p.channels + s.c;
-#pragma unroll 4
-    for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
-        float v[V];
-        load_v<T, V>(v, reinterpret_cast<const T*>(p.x) + base + (size_t)q * p.channels);
+    for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kBatch * s.rows) {
+        Pack<T, V> raw[kBatch];
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = act<ACT>(fmaf((v[i] - ms.x) * ms.y, w[i], b[i]));
-        store_v<T, V>(reinterpret_cast<T*>(p.y) + base + (size_t)q * p.channels, v);
+        for (int e = 0; e < kBatch; ++e) {
+            const int q = min(q0 + e * s.rows, s.p1 - 1);
+            raw[e] = load_raw<T, V>(reinterpret_cast<const T*>(p.x) + base + (size_t)q * p.channels);
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int q = q0 + e * s.rows;
+            if (q >= s.p1) break;
+            float v[V];
+            unpack<T, V>(v, raw[e]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = act<ACT>(fmaf((v[i] - ms.x) * ms.y, w[i], b[i]));
+            store_v<T, V>(reinterpret_cast<T*>(p.y) + base + (size_t)q * p.channels, v);
+        }
     }
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kT) gn_slab_sums(const __grid_constant__ GroupNormArgs p) {
+__global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_sums(const __grid_constant__ GroupNormArgs p) {
     __shared__ float red[2][kT][V];
     __shared__ float gs[2][kT];
     const SlabSlot s = slab_slot<V>(p);
@@ -404,17 +466,27 @@ __global__ void __launch_bounds__(kT) gn_slab_sums(const __grid_constant__ Group
             w[i] = affine(p.w, p.w_f32, s.c + i, 1.f);
             b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
         }
-#pragma unroll 2
-        for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
-            float h[V], d[V];
-            load_v<T, V>(h, reinterpret_cast<const T*>(p.x) + base + (size_t)q * p.channels);
-            load_v<T, V>(d, reinterpret_cast<const T*>(p.dy) + base + (size_t)q * p.channels);
+        for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kPair * s.rows) {
+            Pack<T, V> raw_x[kPair], raw_d[kPair];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = (h[i] - ms.x) * ms.y;
-                const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
-                dw[i] = fmaf(du, h[i], dw[i]);
-                db[i] += du;
+            for (int e = 0; e < kPair; ++e) {
+                const size_t at = base + (size_t)min(q0 + e * s.rows, s.p1 - 1) * p.channels;
+                raw_x[e] = load_raw<T, V>(reinterpret_cast<const T*>(p.x) + at);
+                raw_d[e] = load_raw<T, V>(reinterpret_cast<const T*>(p.dy) + at);
+            }
+#pragma unroll
+            for (int e = 0; e < kPair; ++e) {
+                if (q0 + e * s.rows >= s.p1) break;
+                float h[V], d[V];
+                unpack<T, V>(h, raw_x[e]);
+                unpack<T, V>(d, raw_d[e]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    h[i] = (h[i] - ms.x) * ms.y;
+                    const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
+                    dw[i] = fmaf(du, h[i], dw[i]);
+                    db[i] += du;
+                }
             }
         }
     }
@@ -464,7 +536,7 @@ __global__ void __launch_bounds__(kT) gn_slab_sums(const __grid_constant__ Group
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kT) gn_slab_bwd(const __grid_constant__ GroupNormArgs p) {
+__global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_bwd(const __grid_constant__ GroupNormArgs p) {
     __shared__ float2 st[kMaxLocal];
     const SlabSlot s = slab_slot<V>(p);
     const size_t n = p.sample0 + blockIdx.y;
@@ -496,18 +568,29 @@ __global__ void __launch_bounds__(kT) gn_slab_bwd(const __grid_constant__ GroupN
         b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
     }
     const size_t base = n * p.positions * p.channels + s.c;
-#pragma unroll 2
-    for (int q = s.p0 + s.sub; q < s.p1; q += s.rows) {
-        float h[V], d[V];
-        load_v<T, V>(h, reinterpret_cast<const T*>(p.x) + base + (size_t)q * p.channels);
-        load_v<T, V>(d, reinterpret_cast<const T*>(p.dy) + base + (size_t)q * p.channels);
+    for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kPair * s.rows) {
+        Pack<T, V> raw_x[kPair], raw_d[kPair];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            h[i] = (h[i] - ms.x) * ms.y;
-            const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
-            d[i] = ms.y * (fmaf(du, w[i], -sums.x) - h[i] * sums.y);
+        for (int e = 0; e < kPair; ++e) {
+            const size_t at = base + (size_t)min(q0 + e * s.rows, s.p1 - 1) * p.channels;
+            raw_x[e] = load_raw<T, V>(reinterpret_cast<const T*>(p.x) + at);
+            raw_d[e] = load_raw<T, V>(reinterpret_cast<const T*>(p.dy) + at);
         }
-        store_v<T, V>(reinterpret_cast<T*>(p.dx) + base + (size_t)q * p.channels, d);
+#pragma unroll
+        for (int e = 0; e < kPair; ++e) {
+            const int q = q0 + e * s.rows;
+            if (q >= s.p1) break;
+            float h[V], d[V];
+            unpack<T, V>(h, raw_x[e]);
+            unpack<T, V>(d, raw_d[e]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                h[i] = (h[i] - ms.x) * ms.y;
+                const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
+                d[i] = ms.y * (fmaf(du, w[i], -sums.x) - h[i] * sums.y);
+            }
+            store_v<T, V>(reinterpret_cast<T*>(p.dx) + base + (size_t)q * p.channels, d);
+        }
     }
 }
 
@@ -534,7 +617,7 @@ __global__ void __launch_bounds__(1024) gn_reduce(const float* part, long long r
 }
 
 // ---------------------------------------------------------------------------------------- host
-constexpr long long kPieceBytes = 48ll << 20;  // half of L2: what a second pass still finds there
+constexpr long long kPieceBytes = 72ll << 20;  // what a second pass still finds in the 126 MB of L2
 
 template <typename T, int V, int NV, int LANES, int ACT>
 cudaError_t rows_t(const GroupNormArgs& a, bool backward, cudaStream_t s) {
@@ -592,7 +675,7 @@ cudaError_t run_v(const GroupNormArgs& a, const GroupNormPlan& pl, bool backward
 }  // namespace
 
 // A pure function of the shape, so that the size query and the launch agree.
-GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int channels, int groups) {
+GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int channels, int groups, bool backward) {
     GroupNormPlan pl{};
     const int cg = channels / groups, most = dtype == kF32 ? 4 : 8;
     // vectors of 16 bytes where a group holds whole ones, else of 2, else single channels
@@ -607,8 +690,9 @@ GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int ch
         const long long slots = (long long)groups * pl.lanes;
         const long long at_once = slots >= kT ? 1 : kT / slots;
         const long long wide = (slots + kT - 1) / kT;
-        // persistent CTAs: 8 per SM keep enough loads in flight, and one partial row each
-        long long ctas = (long long)sm * 8 / wide;
+        // one wave of persistent CTAs, each with one row of partial sums
+        const int per_sm = pl.nv > 1 ? (backward ? 1 : 2) : backward ? kRowCtasBwd : kRowCtasFwd;
+        long long ctas = (long long)sm * per_sm / wide;
         const long long full = (samples + at_once - 1) / at_once;
         ctas = ctas < 1 ? 1 : ctas > full ? full : ctas;
         pl.slabs = (int)ctas;
@@ -619,11 +703,11 @@ GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int ch
     const int slots = channels / pl.vec, per = slots < kT ? slots : kT;
     pl.blocks = (slots + kT - 1) / kT;
     const int at_once = kT / per;
-    // about 4 CTAs per SM over the piece of samples that one launch covers, 8 positions a thread at least
+    // one wave of CTAs over the piece of samples that one launch covers, 8 positions a thread at least
     const long long bytes = (long long)positions * channels * (dtype == kF32 ? 4 : 2);
-    long long n = kPieceBytes / bytes;
+    long long n = kPieceBytes / (backward ? 2 * bytes : bytes);
     n = n < 1 ? 1 : n > samples ? samples : n;
-    long long want = ((long long)sm * 4 + n * pl.blocks - 1) / (n * pl.blocks);
+    long long want = (long long)sm * kSlabCtas / (n * pl.blocks);
     const long long room = (positions + 8ll * at_once - 1) / (8ll * at_once);
     want = want < 1 ? 1 : want > room ? room : want;
     pl.slabs = (int)want;
@@ -633,7 +717,7 @@ GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int ch
 }
 
 cudaError_t launch_groupnorm(const GroupNormArgs& args, int dtype, bool backward, cudaStream_t s) {
-    GroupNormPlan pl = groupnorm_plan(dtype, args.samples, args.positions, args.channels, args.groups);
+    GroupNormPlan pl = groupnorm_plan(dtype, args.samples, args.positions, args.channels, args.groups, backward);
     GroupNormArgs a = args;
     a.slabs = pl.slabs;
     cudaError_t e;

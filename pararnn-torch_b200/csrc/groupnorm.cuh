@@ -23,7 +23,7 @@ struct GroupNormPlan {
     size_t group_floats;
 };
 
-GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int channels, int groups);
+GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int channels, int groups, bool backward);
 cudaError_t launch_groupnorm(const GroupNormArgs& a, int dtype, bool backward, cudaStream_t s);
 
 }  // namespace prb

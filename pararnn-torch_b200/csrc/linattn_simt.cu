@@ -217,12 +217,22 @@ __global__ void fold_states_kernel(const __grid_constant__ MixParams p, float* s
     const float w_full = w[0], w_last = w[1];
     const size_t own = ((size_t)seq * p.state_heads + hs) * p.state_elems + e;
     float run = s_in ? s_in[own] : 0.f;
-    for (int i = 0; i < n; ++i) {
-        const int seg = reverse ? n - 1 - i : i;
-        float* at = seg_states + ((size_t)(base + seg) * p.state_heads + hs) * p.state_elems + e;
-        const float u = *at;
-        *at = run;
-        run = fmaf(seg == n - 1 ? w_last : w_full, run, u);
+    constexpr int kAhead = 8;  // loads in flight
+    for (int i0 = 0; i0 < n; i0 += kAhead) {
+        float u[kAhead];
+        float* at[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = min(i0 + k, n - 1), seg = reverse ? n - 1 - i : i;
+            at[k] = seg_states + ((size_t)(base + seg) * p.state_heads + hs) * p.state_elems + e;
+            u[k] = *at[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (i0 + k >= n) break;
+            *at[k] = run;
+            run = fmaf((reverse ? i0 + k == 0 : i0 + k == n - 1) ? w_last : w_full, run, u[k]);
+        }
     }
     if (s_out) s_out[own] = run;
 }
