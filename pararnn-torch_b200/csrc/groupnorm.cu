@@ -302,28 +302,26 @@ __device__ __forceinline__ SlabSlot slab_slot(const GroupNormArgs& p) {
     s.p1 = (int)((long long)(blockIdx.x + 1) * p.positions / p.slabs);
     return s;
 }
-__device__ __forceinline__ void chan(float& n, float& mean, float& m2, float n2, float mean2, float m22) {
-    const float t = n + n2;
-    if (t == 0.f) return;
-    const float d = mean2 - mean, f = n2 / t;
-    mean = fmaf(d, f, mean);
-    m2 += m22 + d * d * n * f;
-    n = t;
-}
-__device__ __forceinline__ void warp_chan(float& n, float& mean, float& m2) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float n2 = __shfl_xor_sync(0xffffffffu, n, o), a = __shfl_xor_sync(0xffffffffu, mean, o),
-                    b = __shfl_xor_sync(0xffffffffu, m2, o);
-        // both lanes of a pair compute the same merge: order the operands by lane
-        if (threadIdx.x & o) {
-            float nn = n2, aa = a, bb = b;
-            chan(nn, aa, bb, n, mean, m2);
-            n = nn, mean = aa, m2 = bb;
-        } else {
-            chan(n, mean, m2, n2, a, b);
-        }
+// Joins (count, mean, M2) entries over a warp without a division per pair: the common mean first, then
+// every entry's M2 and its distance from that mean.  `entry(t)` gives entry t of `total`.
+template <typename F>
+__device__ __forceinline__ float3 warp_join(int total, const F& entry) {
+    const int lane = threadIdx.x & 31;
+    float n = 0.f, sum = 0.f;
+    for (int t = lane; t < total; t += 32) {
+        const float3 u = entry(t);
+        n += u.x;
+        sum = fmaf(u.x, u.y, sum);
     }
+    n = lane_sum<32>(n);
+    const float mean = n > 0.f ? lane_sum<32>(sum) / n : 0.f;
+    float m2 = 0.f;
+    for (int t = lane; t < total; t += 32) {
+        const float3 u = entry(t);
+        const float d = u.y - mean;
+        m2 += u.x > 0.f ? fmaf(u.x * d, d, u.z) : 0.f;
+    }
+    return make_float3(n, mean, lane_sum<32>(m2));
 }
 // groups that this CTA's channels touch
 template <int V>
@@ -385,15 +383,13 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_stats(const __grid_cons
         const int g = g0 + k;
         const int lo = max(0, g * cg / V - (int)blockIdx.z * kT), hi = min(per, (g + 1) * cg / V - (int)blockIdx.z * kT);
         const int width = hi - lo, total = width * s.rows;
-        float cn = 0.f, cm = 0.f, cv = 0.f;
-        for (int t = lane; t < total; t += 32) {
+        const float3 j = warp_join(total, [&](int t) {
             const int id = (t / width) * per + lo + t % width;
-            chan(cn, cm, cv, sn[id], sm[id], sv[id]);
-        }
-        warp_chan(cn, cm, cv);
+            return make_float3(sn[id], sm[id], sv[id]);
+        });
         if (lane == 0)
             reinterpret_cast<float4*>(p.group_part)[((n * p.slabs + blockIdx.x) * gridDim.z + blockIdx.z) * p.groups + g] =
-                make_float4(cn, cm, cv, 0.f);
+                make_float4(j.x, j.y, j.z, 0.f);
     }
 }
 
@@ -408,15 +404,13 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_fwd(const __grid_consta
     for (int k = warp; k < ng; k += kT / 32) {
         int b0, nb;
         group_blocks<V>(p, g0 + k, b0, nb);
-        float cn = 0.f, cm = 0.f, cv = 0.f;
-        for (int t = lane; t < p.slabs * nb; t += 32) {
+        const float3 j = warp_join(p.slabs * nb, [&](int t) {
             const float4 u = reinterpret_cast<const float4*>(
                 p.group_part)[((n * p.slabs + t / nb) * gridDim.z + b0 + t % nb) * p.groups + g0 + k];
-            chan(cn, cm, cv, u.x, u.y, u.z);
-        }
-        warp_chan(cn, cm, cv);
+            return make_float3(u.x, u.y, u.z);
+        });
         if (lane == 0) {
-            const float2 r = make_float2(cm, rsqrtf(cv / cn + p.eps));
+            const float2 r = make_float2(j.y, rsqrtf(j.z / j.x + p.eps));
             st[k] = r;
             if (blockIdx.x == 0 && p.stats && b0 == (int)blockIdx.z) p.stats[n * p.groups + g0 + k] = r;
         }
