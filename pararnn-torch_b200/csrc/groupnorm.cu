@@ -15,6 +15,8 @@
 //          because the host walks the samples in pieces of at most kPieceBytes.
 // Variances are merged as (count, mean, M2), never as sums of squares, and all partial sums are
 // added in a fixed order, so results repeat bit for bit.
+#include <type_traits>
+
 #include "groupnorm.cuh"
 
 namespace prb {
@@ -38,30 +40,65 @@ template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_raw(const T* p) {
     return *reinterpret_cast<const Pack<T, V>*>(p);
 }
+// V channels in fp32; pairs go through the packed fp32 instructions, which halves the issue slots that
+// bound these kernels (28 instructions per element without them, HBM needs about 10)
+template <int V>
+struct Vals {
+    float2 a[V / 2];
+};
+template <>
+struct Vals<1> {
+    float a[1];
+};
+__device__ __forceinline__ float2 op_add(float2 x, float2 y) { return __fadd2_rn(x, y); }
+__device__ __forceinline__ float2 op_mul(float2 x, float2 y) { return __fmul2_rn(x, y); }
+__device__ __forceinline__ float2 op_fma(float2 x, float2 y, float2 z) { return __ffma2_rn(x, y, z); }
+__device__ __forceinline__ float op_add(float x, float y) { return x + y; }
+__device__ __forceinline__ float op_mul(float x, float y) { return x * y; }
+__device__ __forceinline__ float op_fma(float x, float y, float z) { return fmaf(x, y, z); }
+__device__ __forceinline__ float2 op_ex2(float2 x) { return ex2_2(x); }
+__device__ __forceinline__ float op_ex2(float x) { return ex2_approx(x); }
+__device__ __forceinline__ float2 op_rcp(float2 x) { return rcp_2(x); }
+__device__ __forceinline__ float op_rcp(float x) { return rcp_f(x); }
+template <typename E>
+__device__ __forceinline__ E all(float x);
+template <>
+__device__ __forceinline__ float all<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float2 all<float2>(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float total(float x) { return x; }
+__device__ __forceinline__ float total(float2 x) { return x.x + x.y; }
+template <int V>
+constexpr int kN = V == 1 ? 1 : V / 2;  // elements of Vals
+template <int V>
+using Elem = std::conditional_t<V == 1, float, float2>;
+
 template <typename T, int V>
-__device__ __forceinline__ void unpack(float (&r)[V], const Pack<T, V>& u) {
-    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+__device__ __forceinline__ void unpack(Vals<V>& r, const Pack<T, V>& u) {
+    if constexpr (V == 1) {
+        r.a[0] = static_cast<float>(u.v[0]);
+    } else if constexpr (sizeof(T) == 2) {
         const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-            r[2 * i] = __uint_as_float(w[i] << 16);
-            r[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        for (int i = 0; i < V / 2; ++i)
+            r.a[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) r[i] = static_cast<float>(u.v[i]);
+        for (int i = 0; i < V / 2; ++i) r.a[i] = make_float2(u.v[2 * i], u.v[2 * i + 1]);
     }
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_v(T* p, const float (&r)[V]) {
+__device__ __forceinline__ void store_v(T* p, const Vals<V>& r) {
     Pack<T, V> u;
-    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    if constexpr (V == 1) {
+        st_f(&u.v[0], r.a[0]);
+    } else if constexpr (sizeof(T) == 2) {
         __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(&u);
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) w[i] = __floats2bfloat162_rn(r[2 * i], r[2 * i + 1]);
+        for (int i = 0; i < V / 2; ++i) w[i] = __floats2bfloat162_rn(r.a[i].x, r.a[i].y);
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) st_f(&u.v[i], r[i]);
+        for (int i = 0; i < V / 2; ++i) u.v[2 * i] = r.a[i].x, u.v[2 * i + 1] = r.a[i].y;
     }
     *reinterpret_cast<Pack<T, V>*>(p) = u;
 }
@@ -71,20 +108,47 @@ __device__ __forceinline__ float affine(const void* p, int f32, int i, float non
                : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p) + i));
 }
 
-template <int ACT>
-__device__ __forceinline__ float act(float u) {
-    if constexpr (ACT == kActSilu) return u * sigmoid_f(u);
-    if constexpr (ACT == kActGelu) return u * normcdff(u);
+__device__ __forceinline__ float gelu_cdf(float u) { return normcdff(u); }
+__device__ __forceinline__ float2 gelu_cdf(float2 u) { return make_float2(normcdff(u.x), normcdff(u.y)); }
+__device__ __forceinline__ float gelu_pdf(float u) { return 0.3989422804014327f * expf(-0.5f * u * u); }
+__device__ __forceinline__ float2 gelu_pdf(float2 u) { return make_float2(gelu_pdf(u.x), gelu_pdf(u.y)); }
+template <typename E>
+__device__ __forceinline__ E sigmoid_e(E u) {
+    return op_rcp(op_add(op_ex2(op_mul(u, all<E>(-1.4426950216293335f))), all<E>(1.f)));
+}
+template <int ACT, typename E>
+__device__ __forceinline__ E act(E u) {
+    if constexpr (ACT == kActSilu) return op_mul(u, sigmoid_e(u));
+    if constexpr (ACT == kActGelu) return op_mul(u, gelu_cdf(u));
     return u;
 }
-template <int ACT>
-__device__ __forceinline__ float act_slope(float u) {
+template <int ACT, typename E>
+__device__ __forceinline__ E act_slope(E u) {
     if constexpr (ACT == kActSilu) {
-        const float s = sigmoid_f(u);
-        return s * fmaf(u, 1.f - s, 1.f);
+        const E s = sigmoid_e(u);
+        return op_mul(s, op_fma(u, op_fma(s, all<E>(-1.f), all<E>(1.f)), all<E>(1.f)));
     }
-    if constexpr (ACT == kActGelu) return fmaf(u, 0.3989422804014327f * expf(-0.5f * u * u), normcdff(u));
-    return 1.f;
+    if constexpr (ACT == kActGelu) return op_fma(u, gelu_pdf(u), gelu_cdf(u));
+    return all<E>(1.f);
+}
+// weight or bias of V channels from c on
+template <int V>
+__device__ __forceinline__ Vals<V> affine_v(const void* p, int f32, int c, float none, bool in) {
+    Vals<V> r;
+    if constexpr (V == 1) {
+        r.a[0] = in ? affine(p, f32, c, none) : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            r.a[i] = in ? make_float2(affine(p, f32, c + 2 * i, none), affine(p, f32, c + 2 * i + 1, none))
+                        : make_float2(0.f, 0.f);
+    }
+    return r;
+}
+template <int V>
+__device__ __forceinline__ float at(const Vals<V>& r, int i) {
+    if constexpr (V == 1) return r.a[0];
+    else return i & 1 ? r.a[i / 2].y : r.a[i / 2].x;
 }
 
 template <int LANES>
@@ -120,17 +184,16 @@ template <typename T, int V, int NV, int LANES, int ACT>
 __global__ void __launch_bounds__(kT, NV == 1 ? kRowCtasFwd : 2) gn_rows_fwd(const __grid_constant__ GroupNormArgs p) {
     const RowSlot rs = row_slot<LANES>(p.groups);
     const int cg = p.channels / p.groups;
-    float w[NV][V], b[NV][V];
+    using E = Elem<V>;
+    constexpr int N = kN<V>;
+    Vals<V> w[NV], b[NV];
     bool in[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         in[j] = rs.live && (j * LANES + rs.lane) * V < cg;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = rs.g * cg + (j * LANES + rs.lane) * V + i;
-            w[j][i] = in[j] ? affine(p.w, p.w_f32, c, 1.f) : 0.f;
-            b[j][i] = in[j] ? affine(p.b, p.w_f32, c, 0.f) : 0.f;
-        }
+        const int c = rs.g * cg + (j * LANES + rs.lane) * V;
+        w[j] = affine_v<V>(p.w, p.w_f32, c, 1.f, in[j]);
+        b[j] = affine_v<V>(p.b, p.w_f32, c, 0.f, in[j]);
     }
     const float inv = 1.f / cg;
     const size_t step = (size_t)gridDim.x * rs.rows;
@@ -146,36 +209,37 @@ __global__ void __launch_bounds__(kT, NV == 1 ? kRowCtasFwd : 2) gn_rows_fwd(con
     fetch(row);
     // all threads of a CTA take the same number of turns: the shuffles need whole warps
     for (size_t r0 = (size_t)blockIdx.x * rs.rows; r0 < (size_t)p.samples; r0 += step, row += step) {
-        float x[NV][V];
-        float s = 0.f;
+        Vals<V> x[NV];
+        E s = all<E>(0.f);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             unpack<T, V>(x[j], raw[j]);
             if (in[j]) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) s += x[j][i];
+                for (int i = 0; i < N; ++i) s = op_add(s, x[j].a[i]);
             }
         }
         fetch(row + step);
-        const float mean = lane_sum<LANES>(s) * inv;
-        float m2 = 0.f;
+        const float mean = lane_sum<LANES>(total(s)) * inv;
+        E m2 = all<E>(0.f);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (in[j]) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x[j][i] -= mean;
-                    m2 = fmaf(x[j][i], x[j][i], m2);
+                for (int i = 0; i < N; ++i) {
+                    x[j].a[i] = op_add(x[j].a[i], all<E>(-mean));
+                    m2 = op_fma(x[j].a[i], x[j].a[i], m2);
                 }
             }
-        const float rstd = rsqrtf(lane_sum<LANES>(m2) * inv + p.eps);
+        const float rstd = rsqrtf(lane_sum<LANES>(total(m2)) * inv + p.eps);
         if (!rs.live || row >= (size_t)p.samples) continue;
         if (rs.lane == 0 && p.stats) p.stats[row * p.groups + rs.g] = make_float2(mean, rstd);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (!in[j]) continue;
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[j][i] = act<ACT>(fmaf(x[j][i] * rstd, w[j][i], b[j][i]));
+            for (int i = 0; i < N; ++i)
+                x[j].a[i] = act<ACT>(op_fma(op_mul(x[j].a[i], all<E>(rstd)), w[j].a[i], b[j].a[i]));
             store_v<T, V>(reinterpret_cast<T*>(p.y) + row * p.channels + col + j * LANES * V, x[j]);
         }
     }
@@ -185,17 +249,18 @@ template <typename T, int V, int NV, int LANES, int ACT>
 __global__ void __launch_bounds__(kT, NV == 1 ? kRowCtasBwd : 1) gn_rows_bwd(const __grid_constant__ GroupNormArgs p) {
     const RowSlot rs = row_slot<LANES>(p.groups);
     const int cg = p.channels / p.groups;
-    float w[NV][V], b[NV][V], dw[NV][V] = {}, db[NV][V] = {};
+    using E = Elem<V>;
+    constexpr int N = kN<V>;
+    Vals<V> w[NV], b[NV], dw[NV], db[NV];
     bool in[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         in[j] = rs.live && (j * LANES + rs.lane) * V < cg;
+        const int c = rs.g * cg + (j * LANES + rs.lane) * V;
+        w[j] = affine_v<V>(p.w, p.w_f32, c, 1.f, in[j]);
+        b[j] = affine_v<V>(p.b, p.w_f32, c, 0.f, in[j]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = rs.g * cg + (j * LANES + rs.lane) * V + i;
-            w[j][i] = in[j] ? affine(p.w, p.w_f32, c, 1.f) : 0.f;
-            b[j][i] = in[j] ? affine(p.b, p.w_f32, c, 0.f) : 0.f;
-        }
+        for (int i = 0; i < N; ++i) dw[j].a[i] = db[j].a[i] = all<E>(0.f);
     }
     const float inv = 1.f / cg;
     const size_t step = (size_t)gridDim.x * rs.rows;
@@ -218,37 +283,39 @@ __global__ void __launch_bounds__(kT, NV == 1 ? kRowCtasBwd : 1) gn_rows_bwd(con
     for (size_t r0 = (size_t)blockIdx.x * rs.rows; r0 < (size_t)p.samples; r0 += step, row += step) {
         const bool live = rs.live && row < (size_t)p.samples;
         const float2 ms = st;
-        float h[NV][V], d[NV][V];  // xhat, then w du
+        Vals<V> h[NV], d[NV];  // xhat, then w du
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             unpack<T, V>(h[j], raw_x[j]);
             unpack<T, V>(d[j], raw_d[j]);
         }
         fetch(row + step);
-        float s1 = 0.f, s2 = 0.f;
+        E s1 = all<E>(0.f), s2 = all<E>(0.f);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (live && in[j]) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    h[j][i] = (h[j][i] - ms.x) * ms.y;
-                    const float du = d[j][i] * act_slope<ACT>(fmaf(h[j][i], w[j][i], b[j][i]));
-                    dw[j][i] = fmaf(du, h[j][i], dw[j][i]);
-                    db[j][i] += du;
-                    d[j][i] = du * w[j][i];
-                    s1 += d[j][i];
-                    s2 = fmaf(d[j][i], h[j][i], s2);
+                for (int i = 0; i < N; ++i) {
+                    const E x = op_mul(op_add(h[j].a[i], all<E>(-ms.x)), all<E>(ms.y));
+                    const E du = op_mul(d[j].a[i], act_slope<ACT>(op_fma(x, w[j].a[i], b[j].a[i])));
+                    dw[j].a[i] = op_fma(du, x, dw[j].a[i]);
+                    db[j].a[i] = op_add(db[j].a[i], du);
+                    h[j].a[i] = x;
+                    d[j].a[i] = op_mul(du, w[j].a[i]);
+                    s1 = op_add(s1, d[j].a[i]);
+                    s2 = op_fma(d[j].a[i], x, s2);
                 }
             }
         }
-        s1 = lane_sum<LANES>(s1) * inv;
-        s2 = lane_sum<LANES>(s2) * inv;
+        const float m1 = lane_sum<LANES>(total(s1)) * inv, m2 = lane_sum<LANES>(total(s2)) * inv;
         if (!live) continue;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (!in[j]) continue;
 #pragma unroll
-            for (int i = 0; i < V; ++i) d[j][i] = ms.y * (d[j][i] - s1 - h[j][i] * s2);
+            for (int i = 0; i < N; ++i)
+                d[j].a[i] = op_mul(all<E>(ms.y),
+                                   op_fma(h[j].a[i], all<E>(-m2), op_add(d[j].a[i], all<E>(-m1))));
             store_v<T, V>(reinterpret_cast<T*>(p.dx) + row * p.channels + col + j * LANES * V, d[j]);
         }
     }
@@ -260,8 +327,8 @@ __global__ void __launch_bounds__(kT, NV == 1 ? kRowCtasBwd : 1) gn_rows_bwd(con
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            red[0][threadIdx.x][i] = dw[j][i];
-            red[1][threadIdx.x][i] = db[j][i];
+            red[0][threadIdx.x][i] = at(dw[j], i);
+            red[1][threadIdx.x][i] = at(db[j], i);
         }
         __syncthreads();
         if (rs.sub == 0 && in[j]) {
@@ -345,7 +412,9 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_stats(const __grid_cons
     const size_t n = p.sample0 + blockIdx.y;
     const T* x = reinterpret_cast<const T*>(p.x) + n * p.positions * p.channels + s.c;
     // sums about the thread's first value, so that a large mean cancels nothing
-    float pivot = 0.f, s1 = 0.f, s2 = 0.f, cnt = 0.f;
+    using E = Elem<V>;
+    E t1 = all<E>(0.f), t2 = all<E>(0.f);
+    float pivot = 0.f, cnt = 0.f;
     if (s.live && s.p0 + s.sub < s.p1) {
         pivot = static_cast<float>(x[(size_t)(s.p0 + s.sub) * p.channels]);
         for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kBatch * s.rows) {
@@ -358,19 +427,19 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_stats(const __grid_cons
 #pragma unroll
             for (int e = 0; e < kBatch; ++e) {
                 if (q0 + e * s.rows >= s.p1) break;
-                float v[V];
+                Vals<V> v;
                 unpack<T, V>(v, raw[e]);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float d = v[i] - pivot;
-                    s1 += d;
-                    s2 = fmaf(d, d, s2);
+                for (int i = 0; i < kN<V>; ++i) {
+                    const E d = op_add(v.a[i], all<E>(-pivot));
+                    t1 = op_add(t1, d);
+                    t2 = op_fma(d, d, t2);
                 }
                 cnt += V;
             }
         }
     }
-    const float m = cnt > 0.f ? s1 / cnt : 0.f;
+    const float s1 = total(t1), s2 = total(t2), m = cnt > 0.f ? s1 / cnt : 0.f;
     sn[threadIdx.x] = cnt;
     sm[threadIdx.x] = pivot + m;
     sv[threadIdx.x] = cnt > 0.f ? fmaxf(s2 - s1 * m, 0.f) + 0.f * s2 : 0.f;
@@ -418,12 +487,11 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_fwd(const __grid_consta
     __syncthreads();
     if (!s.live) return;
     const float2 ms = st[s.g - g0];
-    float w[V], b[V];
+    using E = Elem<V>;
+    Vals<V> w = affine_v<V>(p.w, p.w_f32, s.c, 1.f, true);
+    const Vals<V> b = affine_v<V>(p.b, p.w_f32, s.c, 0.f, true);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        w[i] = affine(p.w, p.w_f32, s.c + i, 1.f);
-        b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
-    }
+    for (int i = 0; i < kN<V>; ++i) w.a[i] = op_mul(w.a[i], all<E>(ms.y));
     const size_t base = n * p.positions * p.channels + s.c;
     for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kBatch * s.rows) {
         Pack<T, V> raw[kBatch];
@@ -436,10 +504,11 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_fwd(const __grid_consta
         for (int e = 0; e < kBatch; ++e) {
             const int q = q0 + e * s.rows;
             if (q >= s.p1) break;
-            float v[V];
+            Vals<V> v;
             unpack<T, V>(v, raw[e]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = act<ACT>(fmaf((v[i] - ms.x) * ms.y, w[i], b[i]));
+            for (int i = 0; i < kN<V>; ++i)
+                v.a[i] = act<ACT>(op_fma(op_add(v.a[i], all<E>(-ms.x)), w.a[i], b.a[i]));
             store_v<T, V>(reinterpret_cast<T*>(p.y) + base + (size_t)q * p.channels, v);
         }
     }
@@ -451,15 +520,13 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_sums(const __grid_const
     __shared__ float gs[2][kT];
     const SlabSlot s = slab_slot<V>(p);
     const size_t n = p.sample0 + blockIdx.y;
-    float w[V], b[V], dw[V] = {}, db[V] = {};
+    using E = Elem<V>;
+    Vals<V> w = affine_v<V>(p.w, p.w_f32, s.c, 1.f, s.live), b = affine_v<V>(p.b, p.w_f32, s.c, 0.f, s.live), dw, db;
+#pragma unroll
+    for (int i = 0; i < kN<V>; ++i) dw.a[i] = db.a[i] = all<E>(0.f);
     const size_t base = n * p.positions * p.channels + s.c;
     if (s.live) {
         const float2 ms = p.stats[n * p.groups + s.g];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            w[i] = affine(p.w, p.w_f32, s.c + i, 1.f);
-            b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
-        }
         for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kPair * s.rows) {
             Pack<T, V> raw_x[kPair], raw_d[kPair];
 #pragma unroll
@@ -471,23 +538,23 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_sums(const __grid_const
 #pragma unroll
             for (int e = 0; e < kPair; ++e) {
                 if (q0 + e * s.rows >= s.p1) break;
-                float h[V], d[V];
+                Vals<V> h, d;
                 unpack<T, V>(h, raw_x[e]);
                 unpack<T, V>(d, raw_d[e]);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    h[i] = (h[i] - ms.x) * ms.y;
-                    const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
-                    dw[i] = fmaf(du, h[i], dw[i]);
-                    db[i] += du;
+                for (int i = 0; i < kN<V>; ++i) {
+                    const E x = op_mul(op_add(h.a[i], all<E>(-ms.x)), all<E>(ms.y));
+                    const E du = op_mul(d.a[i], act_slope<ACT>(op_fma(x, w.a[i], b.a[i])));
+                    dw.a[i] = op_fma(du, x, dw.a[i]);
+                    db.a[i] = op_add(db.a[i], du);
                 }
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        red[0][threadIdx.x][i] = dw[i];
-        red[1][threadIdx.x][i] = db[i];
+        red[0][threadIdx.x][i] = at(dw, i);
+        red[1][threadIdx.x][i] = at(db, i);
     }
     __syncthreads();
     const int per = min(p.channels / V, kT);
@@ -503,8 +570,8 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_sums(const __grid_const
             }
             dst[i] = a0;
             dst[p.channels + i] = a1;
-            t1 = fmaf(w[i], a1, t1);
-            t2 = fmaf(w[i], a0, t2);
+            t1 = fmaf(at(w, i), a1, t1);
+            t2 = fmaf(at(w, i), a0, t2);
         }
     }
     gs[0][threadIdx.x] = t1;
@@ -555,12 +622,8 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_bwd(const __grid_consta
     __syncthreads();
     if (!s.live) return;
     const float2 ms = p.stats[n * p.groups + s.g], sums = st[s.g - g0];
-    float w[V], b[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        w[i] = affine(p.w, p.w_f32, s.c + i, 1.f);
-        b[i] = affine(p.b, p.w_f32, s.c + i, 0.f);
-    }
+    using E = Elem<V>;
+    const Vals<V> w = affine_v<V>(p.w, p.w_f32, s.c, 1.f, true), b = affine_v<V>(p.b, p.w_f32, s.c, 0.f, true);
     const size_t base = n * p.positions * p.channels + s.c;
     for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kPair * s.rows) {
         Pack<T, V> raw_x[kPair], raw_d[kPair];
@@ -574,14 +637,14 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_bwd(const __grid_consta
         for (int e = 0; e < kPair; ++e) {
             const int q = q0 + e * s.rows;
             if (q >= s.p1) break;
-            float h[V], d[V];
+            Vals<V> h, d;
             unpack<T, V>(h, raw_x[e]);
             unpack<T, V>(d, raw_d[e]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = (h[i] - ms.x) * ms.y;
-                const float du = d[i] * act_slope<ACT>(fmaf(h[i], w[i], b[i]));
-                d[i] = ms.y * (fmaf(du, w[i], -sums.x) - h[i] * sums.y);
+            for (int i = 0; i < kN<V>; ++i) {
+                const E x = op_mul(op_add(h.a[i], all<E>(-ms.x)), all<E>(ms.y));
+                const E du = op_mul(d.a[i], act_slope<ACT>(op_fma(x, w.a[i], b.a[i])));
+                d.a[i] = op_mul(all<E>(ms.y), op_fma(x, all<E>(-sums.y), op_fma(du, w.a[i], all<E>(-sums.x))));
             }
             store_v<T, V>(reinterpret_cast<T*>(p.dx) + base + (size_t)q * p.channels, d);
         }
