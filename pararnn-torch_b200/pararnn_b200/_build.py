@@ -1,7 +1,8 @@
-"""Build the C-ABI shared library ``libpararnn_b200.so`` for sm_100a with nvcc.
+"""Build the C-ABI shared library ``libpararnn_b200.so`` for sm_100a with nvcc, and the PyTorch
+binding of the token-model operators ``libpararnn_b200_torch.so`` on top of it with g++.
 
-The library is built in-tree next to this file so that it travels with the
-source tree.  ``python -m pararnn_b200._build`` rebuilds it.
+The libraries are built in-tree next to this file so that they travel with the
+source tree.  ``python -m pararnn_b200._build`` rebuilds them.
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 LIB = os.path.join(HERE, "libpararnn_b200.so")
+TORCH_LIB = os.path.join(HERE, "libpararnn_b200_torch.so")
 OBJ_DIR = os.path.join(CSRC, "build")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -25,13 +27,28 @@ def _newest_source_mtime() -> float:
     m = 0.0
     for root in (CSRC, os.path.join(os.path.dirname(os.path.dirname(HERE)), "include")):
         for f in os.listdir(root):
-            if f.endswith((".cu", ".cuh", ".h")):
+            if f.endswith((".cu", ".cuh", ".h", ".cpp")):
                 m = max(m, os.path.getmtime(os.path.join(root, f)))
     return m
 
 
 def is_fresh() -> bool:
-    return os.path.exists(LIB) and os.path.getmtime(LIB) >= _newest_source_mtime()
+    newest = _newest_source_mtime()
+    return all(os.path.exists(f) and os.path.getmtime(f) >= newest for f in (LIB, TORCH_LIB))
+
+
+def _torch_binding_command() -> list[str]:
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            "-I" + os.path.join(root, "include"),
+            "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            "-I" + os.path.join(cuda, "include"), os.path.join(CSRC, "torch_binding.cpp"), "-o", TORCH_LIB,
+            "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+            "-L" + HERE, "-lpararnn_b200", "-Wl,-rpath,$ORIGIN"]
 
 
 def _compile(src: str) -> str:
@@ -57,6 +74,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    r = subprocess.run(_torch_binding_command(), capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for torch_binding.cpp:\n{r.stdout}\n{r.stderr}")
     if verbose:
         print("built", LIB)
     return LIB

@@ -20,6 +20,7 @@ class ExtensionMissingError(RuntimeError):
 
 
 _lib = None
+_native = None
 
 _VOIDP = ctypes.c_void_p
 _INT = ctypes.c_int
@@ -113,6 +114,24 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+def native():
+    """The C++ operators of ``torch_binding.cpp`` (``torch.ops.pararnn_b200_native``)."""
+    global _native
+    if _native is None:
+        import torch
+
+        lib()
+        path = os.path.join(HERE, "libpararnn_b200_torch.so")
+        if not os.path.exists(path):
+            raise ExtensionMissingError(f"{path} not found: build it with `python -m pararnn_b200._build`")
+        try:
+            torch.ops.load_library(path)
+        except OSError as exc:  # pragma: no cover
+            raise ExtensionMissingError(f"cannot load {path}: {exc}") from exc
+        _native = torch.ops.pararnn_b200_native
+    return _native
 
 
 OPTIONS = {"kernel_family": 0, "picard_fused": 1, "newton_fused": 2, "spin_limit": 3}

@@ -12,39 +12,13 @@ and ``cells/para_rwkv7.py``; this mixer has no counterpart there.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch import Tensor
 
 from . import _lib as L
-from .ops import (_attention_devices, _check_cuda, _device_guard, _dtype_code, _once, _raise, _raw_stream, gather_h0,
-                  validate_cu_seqlens)
-from .token_ops import _p, _scratch
+from .ops import _attention_devices, _check_cuda, _dtype_code, gather_h0, validate_cu_seqlens
 
 MAX_HEAD_DIM = 128
-
-
-def _heads(t: Tensor):
-    """``(tensor to keep alive, prb_heads)``: ``t`` itself where the kernels can address it (unit channel
-    stride, no broadcast axes, for bf16 16-byte aligned rows), else a contiguous copy."""
-    if not t.is_contiguous():
-        shape, st = t.shape, t.stride()
-        copy = st[3] != 1 and shape[3] > 1
-        for s, n in zip(st[:3], shape[:3]):
-            # an axis of length 1 may carry any stride
-            copy |= n > 1 and (s == 0 or (t.dtype == torch.bfloat16 and s % 8 != 0))
-        if copy:
-            t = t.contiguous()
-    ptr = t.data_ptr()
-    if ptr % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        ptr = t.data_ptr()
-    _, n1, n2, n3 = t.shape
-    if t.is_contiguous():
-        return t, L.Heads(ptr, n1 * n2 * n3, n2 * n3, n3)
-    st = [s if n > 1 else n3 for s, n in zip(t.stride(), t.shape)]
-    return t, L.Heads(ptr, st[0], st[1], st[2])
 
 
 def _shapes(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor):
@@ -80,7 +54,7 @@ def _check_state(state: Tensor | None, shape: tuple[int, ...], name: str) -> Ten
         raise TypeError(f"{name} must be float32 (states are kept in 32 bits), got {state.dtype}")
     if tuple(state.shape) != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(state.shape)}")
-    return state.contiguous()
+    return state
 
 
 def _offsets(cu_seqlens: Tensor | None, batch: int, time: int, dev):
@@ -102,44 +76,30 @@ def _offsets(cu_seqlens: Tensor | None, batch: int, time: int, dev):
     return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous(), len(cs) - 1, longest
 
 
-_ref = ctypes.byref
-
-
 def _decay(log_decay: Tensor) -> Tensor:
-    return log_decay.to(torch.float32).contiguous()
+    return log_decay.detach().to(torch.float32).contiguous()
 
 
-def _maker(cu: Tensor | None):
-    """Checked offsets cover every token; those that a graph replays with may not, and tokens that no
-    sequence holds are left as they were: zeros."""
-    return torch.zeros if cu is not None and torch.cuda.is_current_stream_capturing() else torch.empty
+def _prepare(q, k, v, log_decay, state, cu_seqlens, scale):
+    """Checks, and the trailing arguments of the native operators: (cu, sequences, longest, scale, sparse)."""
+    B, T, Hq, Hkv, dk, dv = _shapes(q, k, v, log_decay)
+    _dtype_code(q)
+    dev = _check_cuda(q, k, v, log_decay, state)
+    cu, n_seq, longest = _offsets(cu_seqlens, B, T, dev)
+    _check_state(state, (n_seq, Hkv, dk, dv), "state")
+    _attention_devices.add(dev)
+    # checked offsets cover every token; those that a graph replays with may not, and tokens that no
+    # sequence holds give zeros
+    sparse = cu is not None and torch.cuda.is_current_stream_capturing()
+    return (B, T, Hq, Hkv, dk, dv), cu, n_seq, longest, dk ** -0.5 if scale is None else float(scale), sparse
 
 
 def linear_attention_fused(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor | None = None,
                            cu_seqlens: Tensor | None = None, *, scale: float | None = None,
                            want_state: bool = True):
     """``(o, final state or None)``: ``o (B,T,Hq,dv)`` in ``q.dtype``, states fp32 ``(n_seq,Hkv,dk,dv)``."""
-    B, T, Hq, Hkv, dk, dv = _shapes(q, k, v, log_decay)
-    code = _dtype_code(q)
-    dev = _check_cuda(q, k, v, log_decay, state)
-    cu, n_seq, longest = _offsets(cu_seqlens, B, T, dev)
-    s_in = _check_state(state, (n_seq, Hkv, dk, dv), "state")
-    scale = dk ** -0.5 if scale is None else float(scale)
-    (qv, qh), (kv, kh), (vv, vh) = _heads(q), _heads(k), _heads(v)
-    g = _decay(log_decay)
-    make = _maker(cu)
-    out = make((B, T, Hq, dv), dtype=q.dtype, device=dev)
-    s_out = torch.empty((n_seq, Hkv, dk, dv), dtype=torch.float32, device=dev) if want_state else None
-    lib = L.lib()
-    with _device_guard(dev):
-        n = lib.prb_linear_attention_workspace_bytes(B, T, n_seq, longest, Hq, Hkv, dk, dv, code, cu is not None, 0)
-        ws = _scratch(n, dev)
-        rc = lib.prb_linear_attention(_ref(qh), _ref(kh), _ref(vh), _p(g), _p(s_in), _p(cu), _p(out), _p(s_out), B, T,
-                                      n_seq, longest, Hq, Hkv, dk, dv, code, scale, _p(ws), n, _raw_stream(dev))
-    if rc:
-        _raise(rc, "linear_attention_fused")
-    _attention_devices.add(dev)
-    return out, s_out
+    _, cu, n_seq, longest, scale, sparse = _prepare(q, k, v, log_decay, state, cu_seqlens, scale)
+    return L.native().attention_fwd(q, k, v, _decay(log_decay), state, cu, n_seq, longest, scale, want_state, sparse)
 
 
 def linear_attention_reverse_vjp(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, grad_out: Tensor,
@@ -148,59 +108,14 @@ def linear_attention_reverse_vjp(q: Tensor, k: Tensor, v: Tensor, log_decay: Ten
                                  want_state: bool = False):
     """``(g_q, g_k, g_v, g_state or None)`` from the cotangents of the output and of the final state.
     Gradients of shared key / value heads are summed over their query heads in fp32."""
-    B, T, Hq, Hkv, dk, dv = _shapes(q, k, v, log_decay)
-    code = _dtype_code(q)
+    shape, cu, n_seq, longest, scale, sparse = _prepare(q, k, v, log_decay, state, cu_seqlens, scale)
+    B, T, Hq, Hkv, dk, dv = shape
     if tuple(grad_out.shape) != (B, T, Hq, dv):
         raise ValueError(f"grad_out must be {(B, T, Hq, dv)}, got {tuple(grad_out.shape)}")
-    dev = _check_cuda(q, k, v, log_decay, grad_out, state, grad_state)
-    cu, n_seq, longest = _offsets(cu_seqlens, B, T, dev)
-    s_in = _check_state(state, (n_seq, Hkv, dk, dv), "state")
-    gs = _check_state(grad_state, (n_seq, Hkv, dk, dv), "grad_state")
-    scale = dk ** -0.5 if scale is None else float(scale)
-    (qv, qh), (kv, kh), (vv, vh), (gv, gh) = _heads(q), _heads(k), _heads(v), _heads(grad_out.to(q.dtype))
-    g = _decay(log_decay)
-    make = _maker(cu)
-    g_q = make((B, T, Hq, dk), dtype=q.dtype, device=dev)
-    g_k = make((B, T, Hkv, dk), dtype=q.dtype, device=dev)
-    g_v = make((B, T, Hkv, dv), dtype=q.dtype, device=dev)
-    g_s = torch.empty((n_seq, Hkv, dk, dv), dtype=torch.float32, device=dev) if want_state else None
-    lib = L.lib()
-    with _device_guard(dev):
-        n = lib.prb_linear_attention_workspace_bytes(B, T, n_seq, longest, Hq, Hkv, dk, dv, code, cu is not None, 1)
-        ws = _scratch(n, dev)
-        rc = lib.prb_bwd_linear_attention(_ref(qh), _ref(kh), _ref(vh), _ref(gh), _p(g), _p(s_in), _p(gs), _p(cu),
-                                          _p(g_q), _p(g_k), _p(g_v), _p(g_s), B, T, n_seq, longest, Hq, Hkv, dk, dv,
-                                          code, scale, _p(ws), n, _raw_stream(dev))
-    if rc:
-        _raise(rc, "linear_attention_reverse_vjp")
-    _attention_devices.add(dev)
-    return g_q, g_k, g_v, g_s
-
-
-class _LinearAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, state, cu_seqlens, scale, want_state):
-        out, s_out = linear_attention_fused(q, k, v, log_decay, state, cu_seqlens, scale=scale,
-                                            want_state=want_state)
-        ctx.save_for_backward(q, k, v, log_decay, state, cu_seqlens)
-        ctx.scale = scale
-        ctx.set_materialize_grads(False)
-        return out, s_out
-
-    @staticmethod
-    def backward(ctx, grad_out, grad_state):
-        _once("linear_attention")
-        q, k, v, log_decay, state, cu = ctx.saved_tensors
-        if grad_out is None and grad_state is None:
-            return (None,) * 8
-        if grad_out is None:
-            grad_out = q.new_zeros(*q.shape[:3], v.shape[3])
-        g_q, g_k, g_v, g_s = linear_attention_reverse_vjp(
-            q, k, v, log_decay, grad_out, state, grad_state, cu, scale=ctx.scale,
-            want_state=ctx.needs_input_grad[4])
-        need = ctx.needs_input_grad
-        return (g_q if need[0] else None, g_k if need[1] else None, g_v if need[2] else None, None, g_s, None, None,
-                None)
+    _check_state(grad_state, (n_seq, Hkv, dk, dv), "grad_state")
+    _check_cuda(q, grad_out, grad_state)
+    return L.native().attention_bwd(q, k, v, _decay(log_decay), grad_out, state, grad_state, cu, n_seq, longest, scale,
+                                    want_state, sparse)
 
 
 def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor | None = None,
@@ -223,7 +138,9 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: 
             raise ValueError("block_table needs state as a pool (C, Hkv, dk, dv)")
         rows = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
         state = gather_h0(state, block_table, rows, (k.shape[2], k.shape[3], v.shape[3]))
-    out, s_out = _LinearAttention.apply(q, k, v, log_decay, state, cu_seqlens, scale, return_state)
+    _, cu, n_seq, longest, scale, sparse = _prepare(q, k, v, log_decay, state, cu_seqlens, scale)
+    out, s_out = L.native().attention(q, k, v, _decay(log_decay), state, cu, n_seq, longest, scale, return_state,
+                                      sparse)
     return (out, s_out) if return_state else out
 
 
@@ -269,24 +186,19 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
             raise ValueError(f"block_table must be ({B},), got {tuple(block_table.shape)}")
         if block_table.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"block_table must be int32 or int64, got {block_table.dtype}")
-    code = _dtype_code(q)
+    _dtype_code(q)
     dev = _check_cuda(q, k, v, log_decay, state)
     shape = (B, 1, Hq, dv) if timed else (B, Hq, dv)
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=dev)
     elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {shape} {q.dtype} on {dev}")
-    bt = None
-    if block_table is not None:
-        if not block_table.is_cuda and torch.cuda.is_current_stream_capturing():
+    if block_table is not None and not block_table.is_cuda:
+        if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a CUDA graph needs block_table on the device")
-        bt = block_table.to(dev).contiguous()
-    q, k, v, g = q.contiguous(), k.contiguous(), v.contiguous(), _decay(log_decay)
-    scale = dk ** -0.5 if scale is None else float(scale)
-    with _device_guard(dev):
-        rc = L.lib().prb_linear_attention_step(_p(q), _p(k), _p(v), _p(g), _p(state), _p(bt),
-                                               bt is not None and bt.dtype == torch.int64, _p(out), B,
-                                               state.shape[0], Hq, Hkv, dk, dv, code, scale, _raw_stream(dev))
-    if rc:
-        _raise(rc, "linear_attention_step")
+        block_table = block_table.to(dev)
+    elif block_table is not None:
+        _check_cuda(q, block_table)
+    L.native().attention_step(q, k, v, _decay(log_decay), state, block_table, dk ** -0.5 if scale is None else scale,
+                              out)
     return out

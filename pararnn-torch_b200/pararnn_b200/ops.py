@@ -68,33 +68,6 @@ def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_GUARD = _NoGuard()
-
-
-def _device_guard(device):
-    """``torch.cuda.device(device)`` where it changes something; small operators are called so often
-    that the switch to the device that is current anyway would be a tenth of their host time."""
-    return _NO_GUARD if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
-
-
-def _raw_stream(device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _once(name: str) -> None:
-    """Gradients of these operators are not differentiable themselves: refuse ``create_graph=True``."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"the gradient of {name} cannot be differentiated again (create_graph=True)")
-
-
 def _raise(code: int, what: str) -> None:
     if code == 0:
         return
