@@ -43,7 +43,7 @@ def _check_heads(Hq: int, Hkv: int, dk: int, dv: int, log_decay: Tensor) -> None
         raise ValueError(f"query heads ({Hq}) must be a multiple of key / value heads ({Hkv})")
     if not (1 <= dk <= MAX_HEAD_DIM and 1 <= dv <= MAX_HEAD_DIM):
         raise TypeError(f"the CUDA backend covers head sizes 1..{MAX_HEAD_DIM}, got dk={dk}, dv={dv}")
-    if tuple(log_decay.shape) != (Hkv,):
+    if log_decay.shape != (Hkv,):
         raise ValueError(f"log_decay must be ({Hkv},), one for each key / value head, got {tuple(log_decay.shape)}")
 
 
@@ -154,28 +154,30 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     ``(B,)`` a pool ``(C,Hkv,dk,dv)`` whose named slots are updated.  Slots outside the pool mark padding
     rows: they touch no state and their outputs are zero.  A slot that several rows name takes
     them in row order.  One launch, no allocation with ``out=``: CUDA graphs can capture it."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    # this call is the latency of a token: its checks are kept short
+    if (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or state.requires_grad) \
+            and torch.is_grad_enabled():
         raise RuntimeError("linear_attention_step has no backward: call it under torch.no_grad()")
     timed = q.dim() == 4
     if timed:
         if any(t.dim() != 4 or t.shape[1] != 1 for t in (q, k, v)):
             raise ValueError("linear_attention_step takes one token: time axes must have length 1")
         q, k, v = q[:, 0], k[:, 0], v[:, 0]
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise ValueError(f"{name} must be (B, heads, channels), got {tuple(t.shape)}")
-        if t.dtype != q.dtype:
-            raise TypeError(f"q, k, v must have one dtype, got {q.dtype} and {t.dtype} ({name})")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("q, k, v must be (B, heads, channels), got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k, v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     B, Hq, dk = q.shape
     Hkv, dv = k.shape[1], v.shape[2]
-    if tuple(k.shape) != (B, Hkv, dk) or tuple(v.shape) != (B, Hkv, dv):
+    if k.shape != (B, Hkv, dk) or v.shape != (B, Hkv, dv):
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
     _check_heads(Hq, Hkv, dk, dv, log_decay)
     if B < 1:
         raise ValueError("batch must be >= 1")
     if state.dtype != torch.float32:
         raise TypeError(f"state must be float32 (states are kept in 32 bits), got {state.dtype}")
-    if state.dim() != 4 or tuple(state.shape[1:]) != (Hkv, dk, dv) or state.shape[0] < 1:
+    if state.dim() != 4 or state.shape[1:] != (Hkv, dk, dv) or state.shape[0] < 1:
         raise ValueError(f"state must be (slots, {Hkv}, {dk}, {dv}), got {tuple(state.shape)}")
     if not state.is_contiguous():
         raise ValueError("linear_attention_step updates state in place: it must be contiguous")
@@ -191,7 +193,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     shape = (B, 1, Hq, dv) if timed else (B, Hq, dv)
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=dev)
-    elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+    elif out.shape != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {shape} {q.dtype} on {dev}")
     if block_table is not None and not block_table.is_cuda:
         if torch.cuda.is_current_stream_capturing():

@@ -19,6 +19,11 @@ Registered:
   as a scan op plus plain functions (``solvers/scan.py:126-203``, ``kernels/vjp_*.py``); here each
   is one op.
 
+* ``pararnn_b200::linear_attention_fused``, ``::reverse_linear_attention_vjp``,
+  ``::linear_attention_step``, ``::group_norm_fused``, ``::group_norm_vjp``, ``::embedding_fused``,
+  ``::embedding_vjp``: the token-model operators (no counterpart in the reference); the functional
+  entry points ``linear_attention``, ``group_norm`` and ``embedding`` are the differentiable ones.
+
 One difference in behaviour: the reference's ``newton_slstm_fused`` is called with a ``states``
 guess produced by ``slstm_picard_init``; here ``states=None`` makes the op run the frozen-gate warm
 start itself, with the number of Picard passes taken from ``set_default_picard_iters`` (the op
@@ -30,7 +35,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import head_ops, ops
+from . import attn_ops, head_ops, ops, token_ops
 
 _picard_default = 0
 
@@ -221,7 +226,96 @@ def _(states, wx, a_z, a_r, a_n, grad_states, h0=None):
             torch.empty(a_z.shape, **f32), torch.empty(wx.shape[0], d, **f32))
 
 
+# ------------------------------------------------------------------------------- token-model ops
+
+@torch.library.custom_op("pararnn_b200::linear_attention_fused", mutates_args=())
+def linear_attention_fused(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor | None = None,
+                           cu_seqlens: Tensor | None = None, *, scale: float | None = None) -> tuple[Tensor, Tensor]:
+    return attn_ops.linear_attention_fused(q, k, v, log_decay, state, cu_seqlens, scale=scale)
+
+
+def _states_like(q, k, v, cu_seqlens):
+    n = q.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    return torch.empty(n, k.shape[2], k.shape[3], v.shape[3], dtype=torch.float32, device=q.device)
+
+
+@linear_attention_fused.register_fake
+def _(q, k, v, log_decay, state=None, cu_seqlens=None, *, scale=None):
+    return q.new_empty(*q.shape[:3], v.shape[3]), _states_like(q, k, v, cu_seqlens)
+
+
+@torch.library.custom_op("pararnn_b200::reverse_linear_attention_vjp", mutates_args=())
+def reverse_linear_attention_vjp(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, grad_out: Tensor,
+                                 state: Tensor | None = None, grad_state: Tensor | None = None,
+                                 cu_seqlens: Tensor | None = None, *,
+                                 scale: float | None = None) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    return attn_ops.linear_attention_reverse_vjp(q, k, v, log_decay, grad_out, state, grad_state, cu_seqlens,
+                                                 scale=scale, want_state=True)
+
+
+@reverse_linear_attention_vjp.register_fake
+def _(q, k, v, log_decay, grad_out, state=None, grad_state=None, cu_seqlens=None, *, scale=None):
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=q.dtype, device=q.device),
+            torch.empty(v.shape, dtype=q.dtype, device=q.device), _states_like(q, k, v, cu_seqlens))
+
+
+@torch.library.custom_op("pararnn_b200::linear_attention_step", mutates_args=("state",))
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor,
+                          block_table: Tensor | None = None, *, scale: float | None = None) -> Tensor:
+    with torch.no_grad():
+        return attn_ops.linear_attention_step(q, k, v, log_decay, state, scale=scale, block_table=block_table)
+
+
+@linear_attention_step.register_fake
+def _(q, k, v, log_decay, state, block_table=None, *, scale=None):
+    return q.new_empty(*q.shape[:-1], v.shape[-1])
+
+
+@torch.library.custom_op("pararnn_b200::group_norm_fused", mutates_args=())
+def group_norm_fused(x: Tensor, num_groups: int, weight: Tensor | None = None, bias: Tensor | None = None,
+                     eps: float = 1e-5, activation: str | None = None) -> tuple[Tensor, Tensor]:
+    return token_ops.group_norm_fused(x, num_groups, weight, bias, eps, activation)
+
+
+@group_norm_fused.register_fake
+def _(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
+    return (torch.empty(x.shape, dtype=x.dtype, device=x.device),
+            torch.empty(x.shape[0], num_groups, 2, dtype=torch.float32, device=x.device))
+
+
+@torch.library.custom_op("pararnn_b200::group_norm_vjp", mutates_args=())
+def group_norm_vjp(x: Tensor, grad_y: Tensor, stats: Tensor, num_groups: int, weight: Tensor, bias: Tensor,
+                   activation: str | None = None) -> tuple[Tensor, Tensor, Tensor]:
+    return token_ops.group_norm_vjp(x, grad_y, stats, num_groups, weight, bias, activation)
+
+
+@group_norm_vjp.register_fake
+def _(x, grad_y, stats, num_groups, weight, bias, activation=None):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(weight), torch.empty_like(bias)
+
+
+@torch.library.custom_op("pararnn_b200::embedding_fused", mutates_args=())
+def embedding_fused(ids: Tensor, weight: Tensor, scale: float = 1.0) -> Tensor:
+    return token_ops.embedding_fused(ids, weight, scale)
+
+
+@embedding_fused.register_fake
+def _(ids, weight, scale=1.0):
+    return weight.new_empty(*ids.shape, weight.shape[1])
+
+
+@torch.library.custom_op("pararnn_b200::embedding_vjp", mutates_args=())
+def embedding_vjp(ids: Tensor, grad_out: Tensor, vocab: int, scale: float = 1.0) -> Tensor:
+    return token_ops.embedding_vjp(ids, grad_out, vocab, scale)
+
+
+@embedding_vjp.register_fake
+def _(ids, grad_out, vocab, scale=1.0):
+    return grad_out.new_empty(vocab, grad_out.shape[-1])
+
+
 OP_NAMES = ("newton_gru_fused", "newton_nlru_fused", "newton_cfc_fused", "newton_titans_fused", "newton_lstm_fused", "newton_slstm_fused",
             "newton_gru_head_fused",
             "reverse_gru_head_factor", "reverse_gru_vjp", "reverse_nlru_vjp", "reverse_slstm_vjp",
-            "reverse_gru_head_vjp")
+            "reverse_gru_head_vjp", "linear_attention_fused", "reverse_linear_attention_vjp", "linear_attention_step",
+            "group_norm_fused", "group_norm_vjp", "embedding_fused", "embedding_vjp")
