@@ -92,6 +92,7 @@ cudaError_t segment_states(MixParams p, const HeadView& b, const HeadView& c, in
     j.share_b = share;
     j.reverse = reverse;
     j.upd_scale = upd;
+    j.exact = s_out != nullptr;
     p.n_jobs = 1;
     cudaError_t e = launch_mix(p, a, true, s);
     if (e != cudaSuccess) return e;
@@ -154,6 +155,7 @@ int prb_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads
     j.share_b = 1;
     j.p_scale = j.row_scale = scale;
     j.upd_scale = 1.f;
+    j.exact = j.s_out != nullptr;
     p.n_jobs = 1;
     return done(launch_mix(p, a, false, s));
 }
@@ -224,6 +226,7 @@ int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_h
     jv.c = view(grad_out);
     jv.out = g_v;
     jv.s_out = seg ? nullptr : g_state;
+    jv.exact = jv.s_out != nullptr;
     jv.da = dk;
     jv.dc = dv;
     jv.s_row = dv;

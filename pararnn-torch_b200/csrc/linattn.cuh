@@ -43,6 +43,7 @@ struct MixJob {
     int share_a;         // heads of a that read one state head
     int share_b;         // heads of b and c that one head of a sums over
     int reverse;
+    int exact;           // the state is an output, not only an operand (tensor cores)
     float p_scale, row_scale, upd_scale;
 };
 

@@ -18,11 +18,12 @@
 // registers (setmaxnreg).
 //
 // Roundings: the scores and the state are rounded to bf16 once as operands, 2^-9 each, which is
-// what the bf16 output loses anyway.  The decayed b^T is split into two bf16 halves (2^-17): the state
-// it builds is returned in fp32 and may be read by thousands of later tokens.  With da = 128 the
-// halves follow one another along K; with da = 64 they fill the two halves of the 128 TMEM lanes, so
-// that the second half costs no further matrix instructions: threads 64-127 then carry the
-// state of the low halves, and S is the sum of the two.
+// what the bf16 output loses anyway.  The decayed b^T is split into two bf16 parts (2^-17), since the state
+// that it builds is read by thousands of later tokens, and into three (2^-24) where the state is returned
+// in fp32 (MixJob::exact): two parts leave an error of 1.3e-6, three 3e-7.  With da = 128 the
+// first two parts follow one another along K; with da = 64 they fill the two halves of the 128 TMEM
+// lanes, so that the second costs no further matrix instructions: threads 64-127 then carry the
+// state of the low parts, and S is the sum of the two.  The third part is one more piece behind them.
 //
 // b^T reaches TMEM through transposing ldmatrix loads: a fragment of 8 x 8 holds token pairs of one
 // channel, which is what a 16x128b TMEM store wants.  It is made in two halves of 64 tokens, so that
@@ -211,7 +212,7 @@ struct Control {
     // one per stage: their producers may be several visits ahead of (or behind) the others
     uint64_t full[4], empty[4], scanned[4], staged[4];
     // one visit or chunk at a time
-    uint64_t p_full[2], p_ready, b_ready[2], b_free[2], i_full, o_full, x_free, drain;
+    uint64_t p_full[2], p_ready, b_ready[3], b_free[3], i_full, o_full, x_free, drain;
     uint32_t tmem;
     int dead;
     int dirty[4];
@@ -311,8 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             mbar_init(&ct.staged[i], 8);
         }
         mbar_init(&ct.p_ready, 8);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&ct.p_full[i], 1);
+        mbar_init(&ct.p_full[0], 1);
+        mbar_init(&ct.p_full[1], 1);
+        for (int i = 0; i < 3; ++i) {
             mbar_init(&ct.b_ready[i], 4);
             mbar_init(&ct.b_free[i], 1);
         }
@@ -449,6 +451,15 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                     tc_commit(&ct.b_free[hf]);
                 }
                 if (!ok) break;
+                if (jb.exact) {
+                    if (!wait(ct, &ct.b_ready[2], par)) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        mma_ts(tmem + L::kColU, tmem + L::kColB + (kSplit || k < 4 ? k * 8 : 64 + (k - 4) * 8),
+                               dcd + (k * 2048 >> 4), kOut, true);
+                    tc_commit(&ct.b_free[2]);
+                }
                 if (!STATE_ONLY) {
                     if (!wait(ct, &ct.p_ready, par)) break;
                     tc_fence_after();
@@ -588,7 +599,8 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             const uint32_t tile = from + v.st * L::kStage;
 #pragma unroll 1
             for (int hf = 0; hf < L::kHalves; ++hf) {
-                if (it > 0 && !(ok = wait_warp(ct, &ct.b_free[hf], par ^ 1))) break;
+                // the third part of the last visit lay where the first piece goes
+                if (it > 0 && !(ok = wait_warp(ct, &ct.b_free[jb.exact && hf == 0 ? 2 : hf], par ^ 1))) break;
                 tc_fence_after();
                 constexpr int kGroups = kC / 8 / L::kHalves;
 #pragma unroll 1
@@ -628,8 +640,47 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 if (lane == 0) mbar_arrive(&ct.b_ready[hf]);
             }
             if (!ok) break;
+            if (jb.exact) {
+                // third part: b w in fp32 less the two parts, both differences exact
+                if (!wait_warp(ct, &ct.b_free[0], par)) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int tg = 0; tg < kC / 8; tg += 4) {
+                    uint32_t rest[2][8] = {};
+                    if (!low) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t f[4];
+                            ldmatrix_t(tile + (tg + e) * 1024, f);
+                            const uint2 w = ct.wb[(tg + e) * 4 + (lane & 3)];
+                            const int t = (tg + e) * 8 + 2 * (lane & 3);
+                            float2 wf;
+                            wf.x = t < n ? jb.upd_scale * ct.pw[reverse ? t + 1 : n - 1 - t] : 0.f;
+                            wf.y = t + 1 < n ? jb.upd_scale * ct.pw[reverse ? t + 2 : n - 2 - t] : 0.f;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const __nv_bfloat162 b = as_bf162(f[q]), wh = as_bf162(w.x);
+                                const __nv_bfloat162 h = __hmul2_rn(b, wh);
+                                const __nv_bfloat162 l = __hfma2(b, as_bf162(w.y), __hfma2(b, wh, __hneg2(h)));
+                                const float2 bf = __bfloat1622float2(b), hf = __bfloat1622float2(h),
+                                             lf = __bfloat1622float2(l);
+                                rest[q >> 1][2 * e + (q & 1)] =
+                                    pack_bf16((bf.x * wf.x - hf.x) - lf.x, (bf.y * wf.y - hf.y) - lf.y);
+                            }
+                        }
+                    }
+                    const uint32_t col = lanes + L::kColB + (kSplit || tg < 8 ? tg * 4 : 64 + (tg - 8) * 4);
+                    tmem_st_16x128b_x4(col, rest[0]);
+                    tmem_st_16x128b_x4(col + (16u << 16), rest[1]);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ct.b_ready[2]);
+            }
             if (v.g < share - 1) continue;
-            if (!wait_warp(ct, &ct.b_free[L::kHalves - 1], par)) break;  // U of the chunk is complete
+            // U of the chunk is complete
+            if (!wait_warp(ct, &ct.b_free[jb.exact ? 2 : L::kHalves - 1], par)) break;
             tc_fence_after();
             const float2 wn = make_float2(ct.pw[n], ct.pw[n]);
 #pragma unroll
