@@ -156,13 +156,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
+// registers per thread of the calling warpgroup, up or down from the 128 of the launch
 template <int N>
-__device__ __forceinline__ void regs_up() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_down() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+__device__ __forceinline__ void set_regs() {
+    if constexpr (N > 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
@@ -190,9 +188,33 @@ struct TcParams {
 
 constexpr uint32_t kCtlBytes = 2048;
 
-template <int DA, int DC, bool STATE_ONLY>
+// ------------------------------------------------------------------------------ decayed b^T
+// Weights of tokens 2 i and 2 i + 1 of a chunk of n tokens, 0 behind its end.
+__device__ __forceinline__ float2 weight_f32(const float* pw, int i, int n, int reverse, float scale) {
+    const int t = 2 * i;
+    return make_float2(t < n ? scale * pw[reverse ? t + 1 : n - 1 - t] : 0.f,
+                       t + 1 < n ? scale * pw[reverse ? t + 2 : n - 2 - t] : 0.f);
+}
+// the same as bf16 pairs: high and low parts
+__device__ __forceinline__ uint2 weight_pair(const float* pw, int i, int n, int reverse, float scale) {
+    const float2 w = weight_f32(pw, i, n, reverse, scale);
+    const uint32_t h = pack_bf16(w.x, w.y);
+    return make_uint2(h, pack_bf16(w.x - __uint_as_float(h << 16), w.y - __uint_as_float(h & 0xffff0000u)));
+}
+// Part 0, 1 or 2 of b w for a pair of tokens: high = rn(b wh), low = rn((b wh - high) + b wl), the bracket
+// exact; third = rn(b w - high - low) with b w in fp32 and exact differences.
+__device__ __forceinline__ uint32_t b_part(uint32_t b_bits, uint2 w, float2 wf, int kind) {
+    const __nv_bfloat162 b = as_bf162(b_bits), wh = as_bf162(w.x), h = __hmul2_rn(b, wh);
+    if (kind == 0) return as_u32(h);
+    const __nv_bfloat162 l = __hfma2(b, as_bf162(w.y), __hfma2(b, wh, __hneg2(h)));
+    if (kind == 1) return as_u32(l);
+    const float2 x = __bfloat1622float2(b), hf = __bfloat1622float2(h), lf = __bfloat1622float2(l);
+    return pack_bf16((x.x * wf.x - hf.x) - lf.x, (x.y * wf.y - hf.y) - lf.y);
+}
+
+template <int DA, int DC>
 struct Layout {
-    static constexpr uint32_t kA = STATE_ONLY ? 0 : DA / 64 * kPanel;
+    static constexpr uint32_t kA = DA / 64 * kPanel;
     static constexpr uint32_t kB = DA / 64 * kPanel;
     static constexpr uint32_t kCc = DC / 64 * kPanel;
     static constexpr uint32_t kStage = kA + kB + kCc;
@@ -217,27 +239,28 @@ struct Control {
     int dead;
     int dirty[4];
     float pw[kC + 1];              // w^0 .. w^128
-    float ps[kC];                  // p_scale w^0 .. w^127
+    float wd[64];                  // scores on the diagonal: p_scale times the factor of key - query + 31
     alignas(8) uint2 wb[kC / 2];   // upd_scale w^pos' of a token pair: bf16 pairs, high and low parts
     alignas(16) float wc[32];      // p_scale times the column factors of the score blocks off the diagonal
 };
 static_assert(sizeof(Control) <= kCtlBytes, "control block");
 
-// false: the limit ran out, or another warp's did
-__device__ __forceinline__ bool wait(Control& ct, uint64_t* bar, uint32_t parity) {
-    // one compact loop: the roles' code shares the instruction cache, and every visit passes a dozen waits
+// false: the limit ran out.  One compact loop: the roles' code shares the instruction cache, and every
+// visit passes a dozen waits.  The roles stop one after the other, each at its own wait.
+template <typename C>
+__device__ __forceinline__ bool wait(C& ct, uint64_t* bar, uint32_t parity) {
+    uint32_t left = kWaitLimit;
 #pragma unroll 1
-    for (uint32_t i = 0; i < kWaitLimit; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255) == 255 && *reinterpret_cast<volatile int*>(&ct.dead)) return false;
-    }
-    *reinterpret_cast<volatile int*>(&ct.dead) = 1;
-    g_status = kErrChainTimeout;
-    return false;
+    while (!mbar_try_wait(bar, parity))
+        if (--left == 0) {
+            ct.dead = 1;
+            return false;
+        }
+    return true;
 }
-
 // for whole warps: all lanes leave together
-__device__ __forceinline__ bool wait_warp(Control& ct, uint64_t* bar, uint32_t parity) {
+template <typename C>
+__device__ __forceinline__ bool wait_warp(C& ct, uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, wait(ct, bar, parity));
 }
 
@@ -256,7 +279,7 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* at, float (&v)[8]) {
 }
 // acc (8 channels from c0 of row i): the row's scores, rounded as the operand is, times c
 __device__ __forceinline__ void row_mix(const MixJob& jb, int row, long long t0, int head, int hb, int i, int j0,
-                                        int j1, int c0, const float* ps, float (&acc)[8]) {
+                                        int j1, int c0, const float* pw, float (&acc)[8]) {
     const __nv_bfloat16* a = token(jb.a, row, t0 + i, head);
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
@@ -269,16 +292,17 @@ __device__ __forceinline__ void row_mix(const MixJob& jb, int row, long long t0,
 #pragma unroll
             for (int q = 0; q < 8; ++q) s = fmaf(y[q], z[q], s);
         }
-        s = __bfloat162float(__float2bfloat16_rn(s * ps[j < i ? i - j : j - i]));
+        s = __bfloat162float(__float2bfloat16_rn(s * (jb.p_scale * pw[j < i ? i - j : j - i])));
         load8(token(jb.c, row, t0 + j, hb) + c0, y);
 #pragma unroll
         for (int q = 0; q < 8; ++q) acc[q] = fmaf(s, y[q], acc[q]);
     }
 }
 
-template <int DA, int DC, bool STATE_ONLY>
+// EXACT: some job of the launch returns its state (the third part costs the others instruction cache)
+template <int DA, int DC, bool EXACT>
 __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_constant__ TcParams tp) {
-    using L = Layout<DA, DC, STATE_ONLY>;
+    using L = Layout<DA, DC>;
     constexpr bool kSplit = DA == 64;  // low halves of b^T in lanes 64-127
     extern __shared__ unsigned char raw[];
     const uint32_t raw_at = smem_u32(raw), base = (raw_at + 1023) & ~1023u;
@@ -287,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     const MixParams& p = tp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // shares of the 512 x 128 registers of the launch: 128 S + 256 O + 128 M <= 65536
-    constexpr int kRegS = 208, kRegO = 112, kRegM = 64;
+    constexpr int kRegS = DC == 64 ? 152 : 208, kRegO = DC == 64 ? 144 : 112, kRegM = 64;
     static_assert(128 * kRegS + 256 * kRegO + 128 * kRegM <= kThreads * 128, "register shares");
 
     // unit fastest: the jobs and heads that read the same tokens run side by side and share them in L2
@@ -300,6 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         u -= n;
     }
     const MixJob& jb = p.job[ji];
+    const bool exact = EXACT && jb.exact;
     const int head = hs * (jb.heads / p.state_heads) + u;
     Seg seg;
     if (!locate(p.map, item, seg)) return;
@@ -307,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     if (tid == 0) {
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(&ct.full[i], 1);
-            mbar_init(&ct.empty[i], STATE_ONLY ? 1 : 2);
+            mbar_init(&ct.empty[i], 2);
             mbar_init(&ct.scanned[i], 1);
             mbar_init(&ct.staged[i], 8);
         }
@@ -328,7 +353,11 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     if (tid < kC + 1) {
         const float w = decay_pow(p.log_decay[hs], tid);
         ct.pw[tid] = w;
-        if (tid < kC) ct.ps[tid] = jb.p_scale * w;
+        // forwards w^(31 - j), backwards w^(j - 31); the other half lies behind the mask
+        if (tid < 32) {
+            ct.wd[jb.reverse ? 31 + tid : 31 - tid] = jb.p_scale * w;
+            ct.wd[jb.reverse ? 31 - tid : 31 + tid] = jb.p_scale * w;
+        }
         // forwards w^(31 - k), backwards w^k
         if (tid < 32) ct.wc[jb.reverse ? tid : 31 - tid] = jb.p_scale * w;
     }
@@ -361,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     auto x_col = [&](const Visit& v) { return tmem + L::kColX + (kTwice ? (v.m & 1) * 64 : 0); };
     auto offset = [&](const Visit& v) { return (reverse ? n_chunk - 1 - v.m : v.m) * kC; };
 
-    if (warp >= 12) regs_down<kRegM>();
+    if (warp >= 12) set_regs<kRegM>();
     if (warp == 12) {
         // ---- TMA
         if (lane == 0) {
@@ -378,8 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 // b first: the state warps start on it
                 for (int q = 0; q < DA / 64; ++q)
                     tma_load_4d(at + L::kA + q * kPanel, mb, full, q * 64, hb, t, seg.row);
-                if (!STATE_ONLY)
-                    for (int q = 0; q < DA / 64; ++q) tma_load_4d(at + q * kPanel, ma, full, q * 64, head, t, seg.row);
+                for (int q = 0; q < DA / 64; ++q) tma_load_4d(at + q * kPanel, ma, full, q * 64, head, t, seg.row);
                 for (int q = 0; q < DC / 64; ++q)
                     tma_load_4d(at + L::kA + L::kB + q * kPanel, mc, full, q * 64, hb, t, seg.row);
             }
@@ -405,11 +433,9 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 return true;
             };
             Visit v, ahead;
-            for (int it = kTwice && !STATE_ONLY ? -1 : 0; it < n_it; ++it) {
+            for (int it = kTwice ? -1 : 0; it < n_it; ++it) {
                 const uint32_t par = it & 1, mpar = v.m & 1;
-                if (STATE_ONLY) {
-                    if (!wait(ct, &ct.full[v.st], v.lap)) break;
-                } else if (kTwice) {
+                if (kTwice) {
                     // one visit ahead; the region is free when the product of visit it - 1 has ended
                     if (it + 1 < n_it) {
                         if (it > 0 && !wait(ct, &ct.o_full, par ^ 1)) break;
@@ -427,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
 #pragma unroll
                 for (int hf = 0; hf < L::kHalves; ++hf) {
                     if (!(ok = wait(ct, &ct.b_ready[hf], par))) break;
-                    if (!STATE_ONLY && hf == 0 && v.g == 0) {
+                    if (hf == 0 && v.g == 0) {
                         // twice: p_ready of the last chunk told that the epilogue before it has read this X
                         if (!kTwice && v.m > 0 && !(ok = wait(ct, &ct.x_free, mpar ^ 1))) break;
                         tc_fence_after();
@@ -445,13 +471,13 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                     for (int k = 0; k < 8 / L::kHalves; ++k) {
                         const uint64_t c = dcd + ((hf * 4 + k) * 2048 >> 4);
                         const uint32_t bt = tmem + L::kColB + hf * 32 + k * 8;
-                        mma_ts(tmem + L::kColU, bt, c, kOut, v.g > 0 || hf > 0 || k > 0);
+                        mma_ts(tmem + L::kColU, bt, c, kOut, (v.g > 0 && !exact) || hf > 0 || k > 0);
                         if (!kSplit) mma_ts(tmem + L::kColU, bt + 64, c, kOut, true);
                     }
                     tc_commit(&ct.b_free[hf]);
                 }
                 if (!ok) break;
-                if (jb.exact) {
+                if (exact) {
                     if (!wait(ct, &ct.b_ready[2], par)) break;
                     tc_fence_after();
 #pragma unroll
@@ -460,17 +486,15 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                                dcd + (k * 2048 >> 4), kOut, true);
                     tc_commit(&ct.b_free[2]);
                 }
-                if (!STATE_ONLY) {
-                    if (!wait(ct, &ct.p_ready, par)) break;
-                    tc_fence_after();
-                    if (!*reinterpret_cast<volatile int*>(&ct.dirty[v.st])) {
-                        const uint32_t from = tmem + L::kColP + p_buf(it) * 128;
+                if (!wait(ct, &ct.p_ready, par)) break;
+                tc_fence_after();
+                if (!*reinterpret_cast<volatile int*>(&ct.dirty[v.st])) {
+                    const uint32_t from = tmem + L::kColP + p_buf(it) * 128;
 #pragma unroll
-                        for (int k = 0; k < kC / 16; ++k)
-                            mma_ts(x_col(v), from + (k >> 1) * 32 + (k & 1) * 8, dcd + (k * 2048 >> 4), kOut, true);
-                    }
-                    tc_commit(&ct.o_full);
+                    for (int k = 0; k < kC / 16; ++k)
+                        mma_ts(x_col(v), from + (k >> 1) * 32 + (k & 1) * 8, dcd + (k * 2048 >> 4), kOut, true);
                 }
+                tc_commit(&ct.o_full);
                 tc_commit(&ct.empty[v.st]);
                 next(v);
             }
@@ -479,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         }
     } else if (warp == 14) {
         // ---- store: whole chunks leave through TMA, ragged ones the output warps have written themselves
-        if (!STATE_ONLY && lane == 0) {
+        if (lane == 0) {
             Visit v;
             for (int it = 0; it < n_it; ++it, next(v)) {
                 if (!wait(ct, &ct.staged[v.st], v.lap)) break;
@@ -498,41 +522,39 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         }
     } else if (warp == 15) {
         // ---- scan of c
-        if (!STATE_ONLY) {
-            Visit v;
-            for (int it = 0; it < n_it; ++it, next(v)) {
-                if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
-                const int rows = min(kC, seg.len - offset(v));
-                const unsigned char* tc = smem + v.st * L::kStage + L::kA + L::kB;
-                // 0 x inf and 0 x NaN are NaN
-                __nv_bfloat162 zero = __float2bfloat162_rn(0.f), sum[4] = {zero, zero, zero, zero};
+        Visit v;
+        for (int it = 0; it < n_it; ++it, next(v)) {
+            if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
+            const int rows = min(kC, seg.len - offset(v));
+            const unsigned char* tc = smem + v.st * L::kStage + L::kA + L::kB;
+            // 0 x inf and 0 x NaN are NaN
+            __nv_bfloat162 zero = __float2bfloat162_rn(0.f), sum[4] = {zero, zero, zero, zero};
 #pragma unroll 1
-                for (int q = 0; q < DC / 64; ++q)
+            for (int q = 0; q < DC / 64; ++q)
 #pragma unroll 4
-                    for (int i = lane; i < rows * 8; i += 32) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(tc + q * kPanel + i * 16);
-                        sum[0] = __hfma2(as_bf162(x.x), zero, sum[0]);
-                        sum[1] = __hfma2(as_bf162(x.y), zero, sum[1]);
-                        sum[2] = __hfma2(as_bf162(x.z), zero, sum[2]);
-                        sum[3] = __hfma2(as_bf162(x.w), zero, sum[3]);
-                    }
-                const float2 f = __bfloat1622float2(__hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3])));
-                bool bad = !(f.x + f.y == 0.f);
-                bad = __any_sync(0xffffffffu, bad);
-                if (lane == 0) {
-                    ct.dirty[v.st] = bad;
-                    mbar_arrive(&ct.scanned[v.st]);
+                for (int i = lane; i < rows * 8; i += 32) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(tc + q * kPanel + i * 16);
+                    sum[0] = __hfma2(as_bf162(x.x), zero, sum[0]);
+                    sum[1] = __hfma2(as_bf162(x.y), zero, sum[1]);
+                    sum[2] = __hfma2(as_bf162(x.z), zero, sum[2]);
+                    sum[3] = __hfma2(as_bf162(x.w), zero, sum[3]);
                 }
+            const float2 f = __bfloat1622float2(__hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3])));
+            bool bad = !(f.x + f.y == 0.f);
+            bad = __any_sync(0xffffffffu, bad);
+            if (lane == 0) {
+                ct.dirty[v.st] = bad;
+                mbar_arrive(&ct.scanned[v.st]);
             }
         }
     } else if (warp < 4) {
         // ---- state: thread r owns row r of S (da = 64: row r - 64 of the low halves from thread 64 on)
-        regs_up<kRegS>();
+        set_regs<kRegS>();
         const int r = tid;
         const uint32_t lanes = tmem + ((uint32_t)warp << 21);  // lane 32 * warp in bits 31-16
         float S[DC];
         {
-            const bool given = !STATE_ONLY && jb.s_in && r < jb.da;
+            const bool given = jb.s_in && r < jb.da;
             const float* from = given ? jb.s_in + sbase + (size_t)r * jb.s_row : nullptr;
             const int limit = given ? jb.dc : 0;
 #pragma unroll
@@ -554,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         for (int it = 0; it < n_it; ++it, next(v)) {
             const int n = min(kC, seg.len - offset(v));
             const uint32_t par = it & 1;
-            if (!STATE_ONLY && v.g == 0) {
+            if (v.g == 0) {
                 // S enters the chunk; the product with the last chunk's operand ended before that chunk's U
 #pragma unroll
                 for (int c = 0; c < DC; c += 8) {
@@ -582,17 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             if (n != table_n) {
                 // the decays of this chunk length (all chunks but the ragged one have the same)
                 asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (r < kC / 2) {
-                    float w[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int t = 2 * r + e;
-                        w[e] = t < n ? jb.upd_scale * ct.pw[reverse ? t + 1 : n - 1 - t] : 0.f;
-                    }
-                    const uint32_t h = pack_bf16(w[0], w[1]);
-                    ct.wb[r] = make_uint2(
-                        h, pack_bf16(w[0] - __uint_as_float(h << 16), w[1] - __uint_as_float(h & 0xffff0000u)));
-                }
+                if (r < kC / 2) ct.wb[r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 table_n = n;
             }
@@ -600,13 +612,13 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
 #pragma unroll 1
             for (int hf = 0; hf < L::kHalves; ++hf) {
                 // the third part of the last visit lay where the first piece goes
-                if (it > 0 && !(ok = wait_warp(ct, &ct.b_free[jb.exact && hf == 0 ? 2 : hf], par ^ 1))) break;
+                if (it > 0 && !(ok = wait_warp(ct, &ct.b_free[exact && hf == 0 ? 2 : hf], par ^ 1))) break;
                 tc_fence_after();
                 constexpr int kGroups = kC / 8 / L::kHalves;
 #pragma unroll 1
                 for (int tg = hf * kGroups; tg < hf * kGroups + kGroups; tg += 4) {
-                    // b w in two bf16 parts: high = rn(b wh), low = rn((b wh - high) + b wl), the bracket exact;
                     // registers of lanes 0-15 and 16-31 of the warp's 32 channels, token groups tg .. tg+3
+                    const float2 none = make_float2(0.f, 0.f);
                     uint32_t f[4][4], hi[2][8], lo[2][8];
                     uint2 w[4];
 #pragma unroll
@@ -618,13 +630,10 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const __nv_bfloat162 b = as_bf162(f[e][q]), wh = as_bf162(w[e].x);
-                            const __nv_bfloat162 h = __hmul2_rn(b, wh);
-                            hi[q >> 1][2 * e + (q & 1)] = as_u32(h);
-                            if (!kSplit || low) {
-                                const uint32_t l = as_u32(__hfma2(b, as_bf162(w[e].y), __hfma2(b, wh, __hneg2(h))));
-                                (kSplit ? hi : lo)[q >> 1][2 * e + (q & 1)] = l;
-                            }
+                            const int at = 2 * e + (q & 1);
+                            hi[q >> 1][at] = b_part(f[e][q], w[e], none, 0);
+                            if (!kSplit) lo[q >> 1][at] = b_part(f[e][q], w[e], none, 1);
+                            else if (low) hi[q >> 1][at] = b_part(f[e][q], w[e], none, 1);
                         }
                     const uint32_t col = lanes + L::kColB + tg * 4, low16 = 16u << 16;
                     tmem_st_16x128b_x4(col, hi[0]);
@@ -640,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 if (lane == 0) mbar_arrive(&ct.b_ready[hf]);
             }
             if (!ok) break;
-            if (jb.exact) {
+            if (exact) {
                 // third part: b w in fp32 less the two parts, both differences exact
                 if (!wait_warp(ct, &ct.b_free[0], par)) break;
                 tc_fence_after();
@@ -653,20 +662,9 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                             uint32_t f[4];
                             ldmatrix_t(tile + (tg + e) * 1024, f);
                             const uint2 w = ct.wb[(tg + e) * 4 + (lane & 3)];
-                            const int t = (tg + e) * 8 + 2 * (lane & 3);
-                            float2 wf;
-                            wf.x = t < n ? jb.upd_scale * ct.pw[reverse ? t + 1 : n - 1 - t] : 0.f;
-                            wf.y = t + 1 < n ? jb.upd_scale * ct.pw[reverse ? t + 2 : n - 2 - t] : 0.f;
+                            const float2 wf = weight_f32(ct.pw, (tg + e) * 4 + (lane & 3), n, reverse, jb.upd_scale);
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const __nv_bfloat162 b = as_bf162(f[q]), wh = as_bf162(w.x);
-                                const __nv_bfloat162 h = __hmul2_rn(b, wh);
-                                const __nv_bfloat162 l = __hfma2(b, as_bf162(w.y), __hfma2(b, wh, __hneg2(h)));
-                                const float2 bf = __bfloat1622float2(b), hf = __bfloat1622float2(h),
-                                             lf = __bfloat1622float2(l);
-                                rest[q >> 1][2 * e + (q & 1)] =
-                                    pack_bf16((bf.x * wf.x - hf.x) - lf.x, (bf.y * wf.y - hf.y) - lf.y);
-                            }
+                            for (int q = 0; q < 4; ++q) rest[q >> 1][2 * e + (q & 1)] = b_part(f[q], w, wf, 2);
                         }
                     }
                     const uint32_t col = lanes + L::kColB + (kSplit || tg < 8 ? tg * 4 : 64 + (tg - 8) * 4);
@@ -678,11 +676,13 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ct.b_ready[2]);
             }
-            if (v.g < share - 1) continue;
-            // U of the chunk is complete
-            if (!wait_warp(ct, &ct.b_free[jb.exact ? 2 : L::kHalves - 1], par)) break;
+            // U of the chunk is complete (or of the visit: the tensor core truncates when it adds up, so an exact
+            // state takes its visits one by one)
+            if (v.g < share - 1 && !exact) continue;
+            if (!wait_warp(ct, &ct.b_free[exact ? 2 : L::kHalves - 1], par)) break;
             tc_fence_after();
-            const float2 wn = make_float2(ct.pw[n], ct.pw[n]);
+            const float decay = v.g == 0 || !exact ? ct.pw[n] : 1.f;
+            const float2 wn = make_float2(decay, decay);
 #pragma unroll
             for (int c0 = 0; c0 < DC; c0 += 32) {
                 uint32_t x[32];
@@ -721,9 +721,9 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 }
             }
         }
-    } else {
+    } else if (warp < 12) {
         // ---- output: threads i and i + 128 own row i of the chunk
-        regs_down<kRegO>();
+        set_regs<kRegO>();
         const int i = (tid - 128) & 127, half = warp >= 8, w4 = warp & 3;
         const uint32_t lanes = tmem + ((uint32_t)w4 << 21);
         constexpr int kCols = DC / 2;  // output channels of a thread
@@ -759,16 +759,14 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                         }
                     } else {
                         // a masked score is replaced, not multiplied by 0: it may be inf or NaN
-                        const float* pw = reverse ? ct.ps - lane : ct.ps + lane;
-                        const int step = reverse ? 1 : -1;
+                        const float* wd = ct.wd + 31 - lane;
                         const uint32_t keep = reverse ? ~0u << lane : ~0u >> (31 - lane);
 #pragma unroll
                         for (int k = 0; k < 32; k += 2) {
-                            // decays of masked places are never read: the address stays on the diagonal there
-                            const bool in0 = keep >> k & 1, in1 = keep >> (k + 1) & 1;
-                            const float f0 = __uint_as_float(x[k]) * pw[(in0 ? k : lane) * step];
-                            const float f1 = __uint_as_float(x[k + 1]) * pw[(in1 ? k + 1 : lane) * step];
-                            h[k >> 1] = pack_bf16(in0 ? f0 : 0.f, in1 ? f1 : 0.f);
+                            const float f0 = keep >> k & 1 ? __uint_as_float(x[k]) : 0.f;
+                            const float f1 = keep >> (k + 1) & 1 ? __uint_as_float(x[k + 1]) : 0.f;
+                            const float2 f = __fmul2_rn(make_float2(f0, f1), make_float2(wd[k], wd[k + 1]));
+                            h[k >> 1] = pack_bf16(f.x, f.y);
                         }
                     }
                     if (reverse && n < kC) {
@@ -822,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                     float acc[8] = {};
                     if (i < n && c0 < jb.dc)
                         row_mix(jb, seg.row, seg.t0 + off, head, share > 1 ? head * share + v.g : hs, i, reverse ? i : 0,
-                                reverse ? n : i + 1, c0, ct.ps, acc);
+                                reverse ? n : i + 1, c0, ct.pw, acc);
                     __syncwarp();
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) + acc[k]);
@@ -877,27 +875,268 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             return true;
         };
         Visit v, ahead;
-        if (!STATE_ONLY) {
-            if (kTwice) {
-                for (int it = -1; it < n_it; ++it) {
-                    if (it >= 0 && !scale(it, v)) break;
-                    if (it + 1 < n_it) {
-                        if (!convert(it + 1, ahead)) break;
-                        next(ahead);
-                    }
-                    if (it < 0) continue;
-                    if (!finish(it, v)) break;
-                    next(v);
+        if (kTwice) {
+            for (int it = -1; it < n_it; ++it) {
+                if (it >= 0 && !scale(it, v)) break;
+                if (it + 1 < n_it) {
+                    if (!convert(it + 1, ahead)) break;
+                    next(ahead);
                 }
-            } else {
-                for (int it = 0; it < n_it; ++it, next(v))
-                    if (!convert(it, v) || !scale(it, v) || !finish(it, v)) break;
+                if (it < 0) continue;
+                if (!finish(it, v)) break;
+                next(v);
             }
+        } else {
+            for (int it = 0; it < n_it; ++it, next(v))
+                if (!convert(it, v) || !scale(it, v) || !finish(it, v)) break;
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && ct.dead) g_status = kErrChainTimeout;
+    if (warp == 13) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// The state-only sweep of a segment: U of every chunk and S = w^n S + U, from b and c alone.  Warps 4-7 and
+// 8-11 take turns in making the parts of the decayed b^T (two visits in flight), warps 0-3 carry S,
+// warp 12 loads, warp 13 issues the products.  TMEM columns: U 0-127, the parts of visit it from
+// 128 + (it & 1) * 192 on: da = 128: high, low, third part; da = 64: high | low, third part | 0.
+template <int DA, int DC>
+struct StateLayout {
+    static constexpr uint32_t kB = DA / 64 * kPanel, kStage = (DA + DC) / 64 * kPanel;
+    static constexpr int kStages = (int)(192 * 1024 / kStage) < 4 ? (int)(192 * 1024 / kStage) : 4;
+    static constexpr uint32_t kOffX = kStages * kStage;  // 64 x dc fp32: low rows on their way to the high ones
+    static constexpr uint32_t kOffCtl = kOffX + (DA == 64 ? 64 * DC * 4 : 0);
+    static constexpr uint32_t kBytes = kOffCtl + kCtlBytes + 1024;
+};
+struct StateControl {
+    uint64_t full[4], empty[4], b_ready[2], b_free[2], u_free, drain;
+    uint32_t tmem;
+    int dead;
+    float pw[kC + 1];
+    alignas(16) uint2 wb[2][kC / 2];   // per group: upd_scale w^pos' of a token pair, bf16 pairs, high and low
+};
+static_assert(sizeof(StateControl) <= kCtlBytes, "control block");
+
+template <int DA, int DC>
+__global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_constant__ TcParams tp) {
+    using L = StateLayout<DA, DC>;
+    constexpr bool kSplit = DA == 64;
+    extern __shared__ unsigned char raw[];
+    const uint32_t raw_at = smem_u32(raw), base = (raw_at + 1023) & ~1023u;
+    unsigned char* smem = raw + (base - raw_at);
+    StateControl& ct = *reinterpret_cast<StateControl*>(smem + L::kOffCtl);
+    const MixParams& p = tp.p;
+    const MixJob& jb = p.job[0];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kRegS = DC == 64 ? 152 : 208, kRegO = DC == 64 ? 144 : 112, kRegM = 64;
+    const int item = blockIdx.x % p.map.n_items, hs = blockIdx.x / p.map.n_items;
+    Seg seg;
+    if (!locate(p.map, item, seg)) return;
+    if (tid == 0) {
+        for (int i = 0; i < L::kStages; ++i) {
+            mbar_init(&ct.full[i], 1);
+            mbar_init(&ct.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ct.b_ready[i], 4);
+            mbar_init(&ct.b_free[i], 1);
+        }
+        mbar_init(&ct.u_free, 4);
+        mbar_init(&ct.drain, 1);
+        ct.dead = 0;
+        mbar_fence_init();
+    }
+    const int reverse = jb.reverse, exact = jb.exact;
+    if (tid < kC + 1) ct.pw[tid] = decay_pow(p.log_decay[hs], tid);
+    if (warp == 13) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ct.tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ct.tmem;
+    const int n_chunk = (seg.len + kC - 1) / kC, share = jb.share_b, n_it = n_chunk * share;
+    const size_t sbase = ((size_t)item * p.state_heads + hs) * p.state_elems;
+    struct Visit {
+        int m = 0, g = 0, st = 0;
+        uint32_t lap = 0;
+    };
+    auto next = [&](Visit& v) {
+        if (++v.st == L::kStages) v.st = 0, v.lap ^= 1;
+        if (++v.g == share) v.g = 0, ++v.m;
+    };
+    auto offset = [&](const Visit& v) { return (reverse ? n_chunk - 1 - v.m : v.m) * kC; };
+
+    if (warp >= 12) set_regs<kRegM>();
+    if (warp == 12) {
+        if (lane == 0) {
+            int it = 0;
+            for (Visit v; it < n_it; ++it, next(v)) {
+                if (it >= L::kStages && !wait(ct, &ct.empty[v.st], v.lap ^ 1)) break;
+                const uint32_t at = base + v.st * L::kStage;
+                const int t = seg.t0 + offset(v), hb = share > 1 ? hs * share + v.g : hs;
+                mbar_expect_tx(&ct.full[v.st], L::kStage);
+                for (int q = 0; q < DA / 64; ++q)
+                    tma_load_4d(at + q * kPanel, &tp.map[0][1], &ct.full[v.st], q * 64, hb, t, seg.row);
+                for (int q = 0; q < DC / 64; ++q)
+                    tma_load_4d(at + L::kB + q * kPanel, &tp.map[0][2], &ct.full[v.st], q * 64, hb, t, seg.row);
+            }
+            if (it < n_it) drain_ring(ct.full, L::kStages, it, kDrainLimit);
+        }
+    } else if (warp == 13) {
+        if (lane == 0) {
+            constexpr uint32_t kOut = instr_desc(DC, true);
+            Visit v;
+            for (int it = 0; it < n_it; ++it, next(v)) {
+                const int buf = it & 1;
+                if (!wait(ct, &ct.full[v.st], v.lap) || !wait(ct, &ct.b_ready[buf], (it >> 1) & 1)) break;
+                if (it > 0 && !wait(ct, &ct.u_free, (it - 1) & 1)) break;
+                tc_fence_after();
+                const uint64_t c = smem_desc(base + v.st * L::kStage + L::kB, kPanel);
+                const uint32_t bt = tmem + 128 + buf * 192;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    mma_ts(tmem, bt + k * 8, c + (k * 2048 >> 4), kOut, k > 0);
+                    if (!kSplit) mma_ts(tmem, bt + 64 + k * 8, c + (k * 2048 >> 4), kOut, true);
+                }
+                if (exact) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        mma_ts(tmem, bt + (kSplit ? 64 : 128) + k * 8, c + (k * 2048 >> 4), kOut, true);
+                }
+                tc_commit(&ct.b_free[buf]);
+                tc_commit(&ct.empty[v.st]);
+            }
+            tc_commit(&ct.drain);
+            mbar_wait_bounded(&ct.drain, 0, kWaitLimit);
+        }
+    } else if (warp < 4) {
+        // ---- state: thread r owns row r of S (da = 64: row r - 64 of the low parts from thread 64 on)
+        set_regs<kRegS>();
+        const int r = tid;
+        const uint32_t lanes = tmem + ((uint32_t)warp << 21);
+        float S[DC];
+#pragma unroll
+        for (int c = 0; c < DC; ++c) S[c] = 0.f;
+        Visit v;
+        for (int it = 0; it < n_it; ++it, next(v)) {
+            if (!wait_warp(ct, &ct.b_free[it & 1], (it >> 1) & 1)) break;
+            tc_fence_after();
+            const float decay = v.g == 0 ? ct.pw[min(kC, seg.len - offset(v))] : 1.f;
+            const float2 wn = make_float2(decay, decay);
+#pragma unroll
+            for (int c0 = 0; c0 < DC; c0 += 32) {
+                uint32_t x[32];
+                tmem_ld32(lanes + c0, x);
+                tc_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    const float2 s2 = __ffma2_rn(wn, make_float2(S[c0 + k], S[c0 + k + 1]),
+                                                 make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])));
+                    S[c0 + k] = s2.x;
+                    S[c0 + k + 1] = s2.y;
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ct.u_free);
+        }
+        if (kSplit) {
+            float* ex = reinterpret_cast<float*>(smem + L::kOffX);
+            if (r >= 64) {
+#pragma unroll
+                for (int c = 0; c < DC; ++c) ex[c * 64 + r - 64] = S[c];
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (r < 64) {
+#pragma unroll
+                for (int c = 0; c < DC; ++c) S[c] += ex[c * 64 + r];
+            }
+        }
+        if (r < jb.da) {
+            float* to = jb.s_out + sbase + (size_t)r * jb.s_row;
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                if (c < jb.dc) *to = S[c];
+                to += jb.s_col;
+            }
+        }
+    } else if (warp < 12) {
+        // ---- parts of the decayed b^T: group 0 the even visits, group 1 the odd ones
+        set_regs<kRegO>();
+        const int group = warp >= 8, w4 = warp & 3, r = (tid - 128) & 127;
+        const uint32_t lanes = tmem + ((uint32_t)w4 << 21);
+        const int d0 = (kSplit ? w4 & 1 : w4) * 32;
+        const bool low = kSplit && w4 >= 2;
+        const uint32_t from = base + (d0 >> 6) * kPanel + (lane & 7) * 128 +
+                              ((((d0 & 63) + 8 * (lane >> 3)) * 2) ^ ((lane & 7) << 4));
+        int table_n = -1;
+        Visit v;
+        for (int it = 0; it < n_it; ++it, next(v)) {
+            if ((it & 1) != group) continue;
+            const int n = min(kC, seg.len - offset(v));
+            if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
+            if (n < kC) {
+                unsigned char* tb = smem + v.st * L::kStage;
+                for (int i = n * 8 + r; i < kC * 8; i += 128)
+#pragma unroll
+                    for (int q = 0; q < (DA + DC) / 64; ++q)
+                        *reinterpret_cast<uint4*>(tb + q * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+            }
+            if (n != table_n) {
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
+                if (r < kC / 2) ct.wb[group][r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
+                table_n = n;
+            }
+            if (it > 1 && !wait_warp(ct, &ct.b_free[group], ((it >> 1) - 1) & 1)) break;
+            tc_fence_after();
+            const uint32_t tile = from + v.st * L::kStage, bt = lanes + 128 + group * 192;
+#pragma unroll 1
+            for (int tg = 0; tg < kC / 8; tg += 4) {
+                uint32_t f[4][4], part[2][8];
+                uint2 w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ldmatrix_t(tile + (tg + e) * 1024, f[e]);
+                    w[e] = ct.wb[group][(tg + e) * 4 + (lane & 3)];
+                }
+#pragma unroll
+                for (int which = 0; which < 3; ++which) {
+                    // da = 64: one store for high | low, one for the third part | 0
+                    if ((kSplit && which == 1) || (which == 2 && !exact)) continue;
+                    const int kind = kSplit && which == 0 && low ? 1 : which;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 wf = which == 2 ? weight_f32(ct.pw, (tg + e) * 4 + (lane & 3), n, reverse, jb.upd_scale)
+                                                     : make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            part[q >> 1][2 * e + (q & 1)] = kind == 2 && low ? 0u : b_part(f[e][q], w[e], wf, kind);
+                    }
+                    const uint32_t col = bt + (kSplit ? which / 2 : which) * 64 + tg * 4;
+                    tmem_st_16x128b_x4(col, part[0]);
+                    tmem_st_16x128b_x4(col + (16u << 16), part[1]);
+                }
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ct.b_ready[group]);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && ct.dead) g_status = kErrChainTimeout;
     if (warp == 13) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -919,33 +1158,32 @@ bool head_map(CUtensorMap* out, const HeadView& v, int d, int heads, int time, i
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DA, int DC, bool STATE_ONLY>
-cudaError_t launch_g(const TcParams& tp, cudaStream_t s) {
-    using L = Layout<DA, DC, STATE_ONLY>;
-    auto* fn = mix_tc_kernel<DA, DC, STATE_ONLY>;
+enum Sweep { kMix, kMixExact, kState };
+
+template <int DA, int DC, Sweep SWEEP>
+cudaError_t launch_d(const TcParams& tp, cudaStream_t s) {
+    void (*fn)(TcParams) = SWEEP == kState ? state_tc_kernel<DA, DC> : mix_tc_kernel<DA, DC, SWEEP == kMixExact>;
+    constexpr uint32_t bytes = SWEEP == kState ? StateLayout<DA, DC>::kBytes : Layout<DA, DC>::kBytes;
     // the attribute is a property of the function on the device: set once for each
     static bool ready[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64 || !ready[dev]) {
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
     const long long grid = (long long)tp.units * tp.p.map.n_items * tp.p.state_heads;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    fn<<<(unsigned)grid, kThreads, L::kBytes, s>>>(tp);
+    fn<<<(unsigned)grid, kThreads, bytes, s>>>(tp);
     return cudaGetLastError();
 }
-template <int DA, int DC>
-cudaError_t launch_d(const TcParams& tp, bool state_only, cudaStream_t s) {
-    return state_only ? launch_g<DA, DC, true>(tp, s) : launch_g<DA, DC, false>(tp, s);
-}
-cudaError_t launch_set(const TcParams& tp, bool state_only, cudaStream_t s) {
+template <Sweep SWEEP>
+cudaError_t launch_set(const TcParams& tp, cudaStream_t s) {
     const bool a = tp.p.job[0].da > 64, c = tp.p.job[0].dc > 64;
-    if (a) return c ? launch_d<128, 128>(tp, state_only, s) : launch_d<128, 64>(tp, state_only, s);
-    return c ? launch_d<64, 128>(tp, state_only, s) : launch_d<64, 64>(tp, state_only, s);
+    if (a) return c ? launch_d<128, 128, SWEEP>(tp, s) : launch_d<128, 64, SWEEP>(tp, s);
+    return c ? launch_d<64, 128, SWEEP>(tp, s) : launch_d<64, 64, SWEEP>(tp, s);
 }
 
 }  // namespace
@@ -997,7 +1235,11 @@ cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStr
             if (!state_only && !head_map(&tp.map[k][3], o, jb.dc, jb.heads, p.map.time, rows))
                 return cudaErrorInvalidValue;
         }
-        const cudaError_t e = launch_set(tp, state_only, s);
+        bool exact = false;
+        for (int k = 0; k < tp.p.n_jobs; ++k) exact |= tp.p.job[k].exact != 0;
+        const cudaError_t e = state_only ? launch_set<kState>(tp, s)
+                              : exact    ? launch_set<kMixExact>(tp, s)
+                                         : launch_set<kMix>(tp, s);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
