@@ -156,6 +156,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 // registers per thread of the calling warpgroup, up or down from the 128 of the launch
 template <int N>
 __device__ __forceinline__ void set_regs() {
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     }
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ct.tmem;
+    constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: they start at 0
 
     const int n_chunk = (seg.len + kC - 1) / kC, share = jb.share_b, n_it = n_chunk * share;
     const int reverse = jb.reverse;
@@ -414,59 +419,62 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             if (it < n_it) drain_ring(ct.full, L::kStages, it, kDrainLimit);
         }
     } else if (warp == 13) {
-        // ---- MMA
-        if (lane == 0) {
-            constexpr uint32_t kScores = instr_desc(kC, false), kOut = instr_desc(DC, true);
-            // scores of visit it (stage v.st); false: a wait ran out
-            auto scores = [&](int it, const Visit& v) {
-                if (!wait(ct, &ct.full[v.st], v.lap)) return false;
-                tc_fence_after();
-                const uint32_t sa = base + v.st * L::kStage;
-                const uint64_t da = smem_desc(sa, 16), db = smem_desc(sa + L::kA, 16);
-                const uint32_t to = tmem + L::kColP + p_buf(it) * 128;
+        // ---- MMA: the whole warp walks and waits, so that addresses and descriptors stay in uniform registers;
+        // one elected lane issues
+        constexpr uint32_t kScores = instr_desc(kC, false), kOut = instr_desc(DC, true);
+        // scores of visit it (stage v.st); false: a wait ran out
+        auto scores = [&](int it, const Visit& v) {
+            if (!wait_warp(ct, &ct.full[v.st], v.lap)) return false;
+            tc_fence_after();
+            const uint32_t sa = base + v.st * L::kStage;
+            const uint64_t da = smem_desc(sa, 16), db = smem_desc(sa + L::kA, 16);
+            const uint32_t to = tmem + L::kColP + p_buf(it) * 128;
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < DA / 16; ++k) {
                     const uint64_t off = ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
                     mma_ss(to, da + off, db + off, kScores, k > 0);
                 }
                 tc_commit(&ct.p_full[p_buf(it)]);
-                return true;
-            };
-            Visit v, ahead;
-            for (int it = kTwice ? -1 : 0; it < n_it; ++it) {
-                const uint32_t par = it & 1, mpar = v.m & 1;
-                if (kTwice) {
-                    // one visit ahead; the region is free when the product of visit it - 1 has ended
-                    if (it + 1 < n_it) {
-                        if (it > 0 && !wait(ct, &ct.o_full, par ^ 1)) break;
-                        if (!scores(it + 1, ahead)) break;
-                        next(ahead);
-                    }
-                    if (it < 0) continue;
-                } else {
-                    if (it > 0 && !wait(ct, &ct.o_full, par ^ 1)) break;
-                    if (!scores(it, v)) break;
+            }
+            __syncwarp();
+            return true;
+        };
+        Visit v, ahead;
+        for (int it = kTwice ? -1 : 0; it < n_it; ++it) {
+            const uint32_t par = it & 1, mpar = v.m & 1;
+            if (kTwice) {
+                // one visit ahead; the region is free when the product of visit it - 1 has ended
+                if (it + 1 < n_it) {
+                    if (it > 0 && !wait_warp(ct, &ct.o_full, par ^ 1)) break;
+                    if (!scores(it + 1, ahead)) break;
+                    next(ahead);
                 }
-                const uint32_t sa = base + v.st * L::kStage;
-                const uint64_t dcd = smem_desc(sa + L::kA + L::kB, kPanel);
-                bool ok = true;
+                if (it < 0) continue;
+            } else {
+                if (it > 0 && !wait_warp(ct, &ct.o_full, par ^ 1)) break;
+                if (!scores(it, v)) break;
+            }
+            const uint32_t sa = base + v.st * L::kStage;
+            const uint64_t dcd = smem_desc(sa + L::kA + L::kB, kPanel);
+            bool ok = true;
 #pragma unroll
-                for (int hf = 0; hf < L::kHalves; ++hf) {
-                    if (!(ok = wait(ct, &ct.b_ready[hf], par))) break;
-                    if (hf == 0 && v.g == 0) {
-                        // twice: p_ready of the last chunk told that the epilogue before it has read this X
-                        if (!kTwice && v.m > 0 && !(ok = wait(ct, &ct.x_free, mpar ^ 1))) break;
-                        tc_fence_after();
+            for (int hf = 0; hf < L::kHalves; ++hf) {
+                if (!(ok = wait_warp(ct, &ct.b_ready[hf], par))) break;
+                const bool first = hf == 0 && v.g == 0;
+                // twice: p_ready of the last chunk told that the epilogue before it has read this X
+                if (first && !kTwice && v.m > 0 && !(ok = wait_warp(ct, &ct.x_free, mpar ^ 1))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    if (first) {
                         const uint64_t da = smem_desc(sa, 16), ds = smem_desc(base + L::kOffS, 128 * 128);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const uint64_t off =
-                                kSplit ? (k & 3) * 32 >> 4 : ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
+                            const uint64_t off = kSplit ? (k & 3) * 32 >> 4 : ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
                             mma_ss(x_col(v), da + off, ds + (k * 2048 >> 4), kOut, k > 0);
                         }
                         tc_commit(&ct.i_full);
                     }
-                    tc_fence_after();
 #pragma unroll
                     for (int k = 0; k < 8 / L::kHalves; ++k) {
                         const uint64_t c = dcd + ((hf * 4 + k) * 2048 >> 4);
@@ -476,19 +484,26 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                     }
                     tc_commit(&ct.b_free[hf]);
                 }
-                if (!ok) break;
-                if (exact) {
-                    if (!wait(ct, &ct.b_ready[2], par)) break;
-                    tc_fence_after();
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (exact) {
+                if (!wait_warp(ct, &ct.b_ready[2], par)) break;
+                tc_fence_after();
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         mma_ts(tmem + L::kColU, tmem + L::kColB + (kSplit || k < 4 ? k * 8 : 64 + (k - 4) * 8),
                                dcd + (k * 2048 >> 4), kOut, true);
                     tc_commit(&ct.b_free[2]);
                 }
-                if (!wait(ct, &ct.p_ready, par)) break;
-                tc_fence_after();
-                if (!*reinterpret_cast<volatile int*>(&ct.dirty[v.st])) {
+                __syncwarp();
+            }
+            if (!wait_warp(ct, &ct.p_ready, par)) break;
+            tc_fence_after();
+            const bool skip = *reinterpret_cast<volatile int*>(&ct.dirty[v.st]) != 0;
+            if (elect_one()) {
+                if (!skip) {
                     const uint32_t from = tmem + L::kColP + p_buf(it) * 128;
 #pragma unroll
                     for (int k = 0; k < kC / 16; ++k)
@@ -496,11 +511,13 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 }
                 tc_commit(&ct.o_full);
                 tc_commit(&ct.empty[v.st]);
-                next(v);
             }
-            tc_commit(&ct.drain);
-            mbar_wait_bounded(&ct.drain, 0, kWaitLimit);
+            __syncwarp();
+            next(v);
         }
+        if (elect_one()) tc_commit(&ct.drain);
+        __syncwarp();
+        mbar_wait_bounded(&ct.drain, 0, kWaitLimit);
     } else if (warp == 14) {
         // ---- store: whole chunks leave through TMA, ragged ones the output warps have written themselves
         if (lane == 0) {
@@ -961,7 +978,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
     }
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ct.tmem;
+    constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: they start at 0
     const int n_chunk = (seg.len + kC - 1) / kC, share = jb.share_b, n_it = n_chunk * share;
     const size_t sbase = ((size_t)item * p.state_heads + hs) * p.state_elems;
     struct Visit {
@@ -991,16 +1008,16 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
             if (it < n_it) drain_ring(ct.full, L::kStages, it, kDrainLimit);
         }
     } else if (warp == 13) {
-        if (lane == 0) {
-            constexpr uint32_t kOut = instr_desc(DC, true);
-            Visit v;
-            for (int it = 0; it < n_it; ++it, next(v)) {
-                const int buf = it & 1;
-                if (!wait(ct, &ct.full[v.st], v.lap) || !wait(ct, &ct.b_ready[buf], (it >> 1) & 1)) break;
-                if (it > 0 && !wait(ct, &ct.u_free, (it - 1) & 1)) break;
-                tc_fence_after();
-                const uint64_t c = smem_desc(base + v.st * L::kStage + L::kB, kPanel);
-                const uint32_t bt = tmem + 128 + buf * 192;
+        constexpr uint32_t kOut = instr_desc(DC, true);
+        Visit v;
+        for (int it = 0; it < n_it; ++it, next(v)) {
+            const int buf = it & 1;
+            if (!wait_warp(ct, &ct.full[v.st], v.lap) || !wait_warp(ct, &ct.b_ready[buf], (it >> 1) & 1)) break;
+            if (it > 0 && !wait_warp(ct, &ct.u_free, (it - 1) & 1)) break;
+            tc_fence_after();
+            const uint64_t c = smem_desc(base + v.st * L::kStage + L::kB, kPanel);
+            const uint32_t bt = tmem + 128 + buf * 192;
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     mma_ts(tmem, bt + k * 8, c + (k * 2048 >> 4), kOut, k > 0);
@@ -1014,9 +1031,11 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
                 tc_commit(&ct.b_free[buf]);
                 tc_commit(&ct.empty[v.st]);
             }
-            tc_commit(&ct.drain);
-            mbar_wait_bounded(&ct.drain, 0, kWaitLimit);
+            __syncwarp();
         }
+        if (elect_one()) tc_commit(&ct.drain);
+        __syncwarp();
+        mbar_wait_bounded(&ct.drain, 0, kWaitLimit);
     } else if (warp < 4) {
         // ---- state: thread r owns row r of S (da = 64: row r - 64 of the low parts from thread 64 on)
         set_regs<kRegS>();
