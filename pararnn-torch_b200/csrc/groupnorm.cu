@@ -25,11 +25,12 @@ namespace {
 
 constexpr int kT = 256;
 // CTAs per SM of the persistent row kernels (one vector per lane) and of the slab kernels; the grids are
-// whole waves of them.  Holding the next row's data in registers while a row is worked on keeps
-// 24 - 32 KB per SM in flight.
-constexpr int kRowCtasFwd = 5, kRowCtasBwd = 3, kSlabCtas = 4;
+// whole waves of them.  Few CTAs with many loads in flight per thread beat many with few: on 32768 x 1024
+// bf16 the forward takes 31.6 us at 4 CTAs, 34 at 5, 37 at 6 and 44 at 8 (spills); on 16 x 4096 x 256 the
+// slab kernels take 77 us (forward and backward) at 2 CTAs and 8 loads, 86 at 4 and 4, 115 at 6 and 4.
+constexpr int kRowCtasFwd = 4, kRowCtasBwd = 3, kSlabCtas = 2;
 constexpr int kMaxLocal = kT + 2;  // groups that one CTA's channels can touch
-constexpr int kBatch = 4, kPair = 3;  // positions whose loads a thread issues together (one input, two inputs)
+constexpr int kBatch = 8, kPair = 8;  // positions whose loads a thread issues together (one input, two inputs)
 
 // V neighbouring channels as they lie in memory; loads are issued well before their conversion
 template <typename T, int V>

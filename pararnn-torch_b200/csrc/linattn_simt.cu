@@ -5,7 +5,8 @@
 //
 // This is the fp32 path: the four products are FFMA work (4 x 4 outputs per thread, operands as
 // float4 from shared memory), which bounds it; tensor cores would round the operands to fewer bits
-// than an fp32 caller asked for.
+// than an fp32 caller asked for.  The next chunk travels from global memory to registers while a
+// chunk is worked on, and with da <= 64 two CTAs share an SM.
 #include "linattn.cuh"
 
 namespace prb {
@@ -17,24 +18,47 @@ constexpr int kN = 64;      // output channels per CTA
 constexpr int kPitch = 68;  // floats per shared-memory row: float4-aligned, rows 4 banks apart
 constexpr int kThreads = 256;
 
+template <int D>
 struct Smem {
-    float at[kMaxHeadDim][kPitch];  // a, transposed: [channel][token]
-    float bt[kMaxHeadDim][kPitch];
+    float at[D][kPitch];  // a, transposed: [channel][token]
+    float bt[D][kPitch];
     float c[kC][kPitch];
-    float s[kMaxHeadDim][kPitch];   // state slice
+    float s[D][kPitch];   // state slice
     float pt[kC][kPitch];           // scores, transposed: [key][query]
     float pw[kC + 1];
 };
 
-// rows [t0, t0 + n) of one head into dst[channel][token], zeros outside
-template <typename TIO>
-__device__ void load_t(float (*dst)[kPitch], const HeadView& v, int row, int t0, int n, int h, int d, int d_pad) {
-    const TIO* base = reinterpret_cast<const TIO*>(v.p) + row * v.sb + (long long)t0 * v.st + h * v.sh;
-    const int tok = threadIdx.x & 7, quad = threadIdx.x >> 3;
-    for (int t = tok; t < kC; t += 8)
-        for (int ch = quad; ch < d_pad; ch += kThreads / 8)
-            dst[ch][t] = (t < n && ch < d) ? ld_f(base + (long long)t * v.st + ch) : 0.f;
-}
+// A 64-token tile of one head on its way through registers: warp w holds tokens w, w + 8, ..., lane l
+// the channels l, l + 32, ...; zeros outside.
+template <typename TIO, int D>
+struct Tile {
+    float v[kC / 8][D / 32];
+    __device__ __forceinline__ void fetch(const HeadView& view, int row, int t0, int n, int h, int c0, int d) {
+        const TIO* base = reinterpret_cast<const TIO*>(view.p) + row * view.sb + (long long)t0 * view.st + h * view.sh + c0;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < kC / 8; ++i)
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+                const int t = warp + 8 * i, ch = lane + 32 * k;
+                v[i][k] = (t < n && ch < d) ? ld_f(base + (long long)t * view.st + ch) : 0.f;
+            }
+    }
+    __device__ __forceinline__ void put_t(float (*dst)[kPitch]) const {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < kC / 8; ++i)
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) dst[lane + 32 * k][warp + 8 * i] = v[i][k];
+    }
+    __device__ __forceinline__ void put(float (*dst)[kPitch]) const {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < kC / 8; ++i)
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) dst[warp + 8 * i][lane + 32 * k] = v[i][k];
+    }
+};
 
 // acc[r][q] += sum_k x[k][r] y[k][q], 4 x 4
 __device__ __forceinline__ void mma44(float (&acc)[4][4], const float* x, const float* y) {
@@ -46,10 +70,10 @@ __device__ __forceinline__ void mma44(float (&acc)[4][4], const float* x, const 
         for (int q = 0; q < 4; ++q) acc[r][q] = fmaf(a[r], b[q], acc[r][q]);
 }
 
-template <typename TIO, bool STATE_ONLY>
-__global__ void __launch_bounds__(kThreads) mix_simt_kernel(const __grid_constant__ MixParams p) {
+template <typename TIO, bool STATE_ONLY, int D>
+__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1) mix_simt_kernel(const __grid_constant__ MixParams p) {
     extern __shared__ __align__(16) unsigned char raw[];
-    Smem& sm = *reinterpret_cast<Smem*>(raw);
+    Smem<D>& sm = *reinterpret_cast<Smem<D>*>(raw);
     int y = blockIdx.y, ji = 0;
     for (; ji + 1 < p.n_jobs; ++ji) {
         const int n = p.job[ji].heads * ((p.job[ji].dc + kN - 1) / kN);
@@ -75,23 +99,29 @@ __global__ void __launch_bounds__(kThreads) mix_simt_kernel(const __grid_constan
     }
     __syncthreads();
     const int n_chunk = (seg.len + kC - 1) / kC;
+    Tile<TIO, D> ra, rb;
+    Tile<TIO, kN> rc;
+    auto fetch = [&](int m, int gi) {
+        if (m >= n_chunk) return;
+        const int off = (jb.reverse ? n_chunk - 1 - m : m) * kC;
+        const int n = min(kC, seg.len - off), t0 = seg.t0 + off;
+        const int hb = jb.share_b > 1 ? head * jb.share_b + gi : hs;
+        if (!STATE_ONLY && gi == 0) ra.fetch(jb.a, seg.row, t0, n, head, 0, da);
+        rb.fetch(jb.b, seg.row, t0, n, hb, 0, da);
+        rc.fetch(jb.c, seg.row, t0, n, hb, c0, dcw);
+    };
+    fetch(0, 0);
     for (int m = 0; m < n_chunk; ++m) {
         const int off = (jb.reverse ? n_chunk - 1 - m : m) * kC;
         const int n = min(kC, seg.len - off), t0 = seg.t0 + off;
         float acc[4][4] = {};
         for (int gi = 0; gi < jb.share_b; ++gi) {
-            const int hb = jb.share_b > 1 ? head * jb.share_b + gi : hs;
-            if (!STATE_ONLY && gi == 0) load_t<TIO>(sm.at, jb.a, seg.row, t0, n, head, da, da_pad);
-            load_t<TIO>(sm.bt, jb.b, seg.row, t0, n, hb, da, da_pad);
-            {
-                const TIO* base = reinterpret_cast<const TIO*>(jb.c.p) + seg.row * jb.c.sb + (long long)t0 * jb.c.st +
-                                  hb * jb.c.sh + c0;
-                for (int i = tid; i < kC * kN; i += kThreads) {
-                    const int t = i / kN, q = i % kN;
-                    sm.c[t][q] = (t < n && q < dcw) ? ld_f(base + (long long)t * jb.c.st + q) : 0.f;
-                }
-            }
+            if (!STATE_ONLY && gi == 0) ra.put_t(sm.at);
+            rb.put_t(sm.bt);
+            rc.put(sm.c);
             __syncthreads();
+            if (gi + 1 < jb.share_b) fetch(m, gi + 1);
+            else fetch(m + 1, 0);
             if (!STATE_ONLY) {
                 float pr[4][4] = {};
                 for (int d = 0; d < da_pad; ++d) mma44(pr, &sm.at[d][ty * 4], &sm.bt[d][tx * 4]);
@@ -177,15 +207,22 @@ __global__ void __launch_bounds__(kThreads) mix_simt_kernel(const __grid_constan
     }
 }
 
-template <typename TIO, bool STATE_ONLY>
+template <typename TIO, bool STATE_ONLY, int D>
 cudaError_t launch_t(const MixParams& p, cudaStream_t s) {
     int ny = 0;
     for (int j = 0; j < p.n_jobs; ++j) ny += p.job[j].heads * ((p.job[j].dc + kN - 1) / kN);
-    cudaError_t e = cudaFuncSetAttribute(mix_simt_kernel<TIO, STATE_ONLY>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem));
+    cudaError_t e = cudaFuncSetAttribute(mix_simt_kernel<TIO, STATE_ONLY, D>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>));
     if (e != cudaSuccess) return e;
-    mix_simt_kernel<TIO, STATE_ONLY><<<dim3(p.map.n_items, ny), kThreads, sizeof(Smem), s>>>(p);
+    mix_simt_kernel<TIO, STATE_ONLY, D><<<dim3(p.map.n_items, ny), kThreads, sizeof(Smem<D>), s>>>(p);
     return cudaGetLastError();
+}
+template <typename TIO>
+cudaError_t launch_d(const MixParams& p, bool state_only, cudaStream_t s) {
+    bool wide = false;
+    for (int j = 0; j < p.n_jobs; ++j) wide |= p.job[j].da > 64;
+    if (wide) return state_only ? launch_t<TIO, true, 128>(p, s) : launch_t<TIO, false, 128>(p, s);
+    return state_only ? launch_t<TIO, true, 64>(p, s) : launch_t<TIO, false, 64>(p, s);
 }
 
 // One thread per state element and (sequence, head): walks the sequence's segments in order.
@@ -240,8 +277,7 @@ __global__ void fold_states_kernel(const __grid_constant__ MixParams p, float* s
 }  // namespace
 
 cudaError_t launch_mix_simt(const MixParams& p, int dtype, bool state_only, cudaStream_t s) {
-    if (dtype == kF32) return state_only ? launch_t<float, true>(p, s) : launch_t<float, false>(p, s);
-    return state_only ? launch_t<__nv_bfloat16, true>(p, s) : launch_t<__nv_bfloat16, false>(p, s);
+    return dtype == kF32 ? launch_d<float>(p, state_only, s) : launch_d<__nv_bfloat16>(p, state_only, s);
 }
 
 cudaError_t launch_fold_states(const MixParams& p, float* seg_states, const float* s_in, float* s_out, bool reverse,
