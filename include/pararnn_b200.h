@@ -67,7 +67,8 @@ const char* prb_error_string(int code);
  * kernel family or a wait limit so that small test shapes reach code that normally serves large
  * ones.  Not thread-safe; call it while no other call of this library is in progress.  Every
  * option's default is what production calls use.
- *   PRB_OPT_KERNEL_FAMILY  -1 choose by shape (default), 0 look-back kernels, 2 pipelined kernels
+ *   PRB_OPT_KERNEL_FAMILY  -1 choose by shape (default), 0 look-back kernels, 2 pipelined kernels;
+ *                          0 also keeps linear attention on the CUDA cores
  *   PRB_OPT_PICARD_FUSED    1 (default) / 0: all Picard passes in one sweep when the shape allows
  *   PRB_OPT_NEWTON_FUSED    1 (default) / 0: all Newton iterations in one sweep when it allows
  *   PRB_OPT_SPIN_LIMIT      polls after which a look-back wait gives up and reports

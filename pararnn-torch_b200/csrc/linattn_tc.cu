@@ -191,7 +191,7 @@ struct TcParams {
     int units;              // heads of all jobs per state head
 };
 
-constexpr uint32_t kCtlBytes = 2048;
+constexpr uint32_t kCtlBytes = 2048, kMaxSmem = 227 * 1024;
 
 // ------------------------------------------------------------------------------ decayed b^T
 // Weights of tokens 2 i and 2 i + 1 of a chunk of n tokens, 0 behind its end.
@@ -228,6 +228,7 @@ struct Layout {
     static constexpr uint32_t kOffS = kStages * kStage;
     static constexpr uint32_t kOffCtl = kOffS + kS;
     static constexpr uint32_t kBytes = kOffCtl + kCtlBytes + 1024;  // alignment slack
+    static_assert(kBytes <= kMaxSmem && kStages >= 2, "shared memory");
     // TMEM columns: scores (fp32, then bf16 in place), X, U, decayed b^T
     static constexpr bool kTwice = DA == 64 && DC == 64;
     static constexpr int kHalves = DA == 64 ? 1 : 2;  // pieces in which b^T is made
@@ -416,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 for (int q = 0; q < DC / 64; ++q)
                     tma_load_4d(at + L::kA + L::kB + q * kPanel, mc, full, q * 64, hb, t, seg.row);
             }
-            if (it < n_it) drain_ring(ct.full, L::kStages, it, kDrainLimit);
+            // also when another role gave up: no copy may land after the CTA has left
+            drain_ring(ct.full, L::kStages, it, kDrainLimit);
         }
     } else if (warp == 13) {
         // ---- MMA: the whole warp walks and waits, so that addresses and descriptors stay in uniform registers;
@@ -925,19 +927,23 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
 template <int DA, int DC>
 struct StateLayout {
     static constexpr uint32_t kB = DA / 64 * kPanel, kStage = (DA + DC) / 64 * kPanel;
-    static constexpr int kStages = (int)(192 * 1024 / kStage) < 4 ? (int)(192 * 1024 / kStage) : 4;
-    static constexpr uint32_t kOffX = kStages * kStage;  // 64 x dc fp32: low rows on their way to the high ones
-    static constexpr uint32_t kOffCtl = kOffX + (DA == 64 ? 64 * DC * 4 : 0);
-    static constexpr uint32_t kBytes = kOffCtl + kCtlBytes + 1024;
+    static constexpr uint32_t kX = DA == 64 ? 64 * DC * 4 : 0;  // low rows on their way to the high ones
+    static constexpr int kFit = (int)((kMaxSmem - kX - 4096 - 1024) / kStage), kStages = kFit < 4 ? kFit : 4;
+    static constexpr uint32_t kOffX = kStages * kStage;
+    static constexpr uint32_t kOffCtl = kOffX + kX;
+    static constexpr uint32_t kBytes = kOffCtl + 4096 + 1024;
+    static_assert(kBytes <= kMaxSmem && kStages >= 2, "shared memory");
 };
 struct StateControl {
     uint64_t full[4], empty[4], b_ready[2], b_free[2], u_free, drain;
     uint32_t tmem;
     int dead;
     float pw[kC + 1];
-    alignas(16) uint2 wb[2][kC / 2];   // per group: upd_scale w^pos' of a token pair, bf16 pairs, high and low
+    // per group: upd_scale w^pos' of a token pair, as bf16 pairs (high and low) and in fp32
+    alignas(16) uint2 wb[2][kC / 2];
+    alignas(16) float2 wf[2][kC / 2];
 };
-static_assert(sizeof(StateControl) <= kCtlBytes, "control block");
+static_assert(sizeof(StateControl) <= 4096, "control block");
 
 template <int DA, int DC>
 __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_constant__ TcParams tp) {
@@ -1005,7 +1011,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
                 for (int q = 0; q < DC / 64; ++q)
                     tma_load_4d(at + L::kB + q * kPanel, &tp.map[0][2], &ct.full[v.st], q * 64, hb, t, seg.row);
             }
-            if (it < n_it) drain_ring(ct.full, L::kStages, it, kDrainLimit);
+            drain_ring(ct.full, L::kStages, it, kDrainLimit);
         }
     } else if (warp == 13) {
         constexpr uint32_t kOut = instr_desc(DC, true);
@@ -1112,7 +1118,10 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
             }
             if (n != table_n) {
                 asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
-                if (r < kC / 2) ct.wb[group][r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
+                if (r < kC / 2) {
+                    ct.wb[group][r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
+                    ct.wf[group][r] = weight_f32(ct.pw, r, n, reverse, jb.upd_scale);
+                }
                 asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
                 table_n = n;
             }
@@ -1135,8 +1144,8 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
                     const int kind = kSplit && which == 0 && low ? 1 : which;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float2 wf = which == 2 ? weight_f32(ct.pw, (tg + e) * 4 + (lane & 3), n, reverse, jb.upd_scale)
-                                                     : make_float2(0.f, 0.f);
+                        float2 wf = make_float2(0.f, 0.f);
+                        if (which == 2) wf = ct.wf[group][(tg + e) * 4 + (lane & 3)];
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
                             part[q >> 1][2 * e + (q & 1)] = kind == 2 && low ? 0u : b_part(f[e][q], w[e], wf, kind);

@@ -70,6 +70,7 @@ struct AttnCall {
     }
 };
 AttnCall attn_call(const Tensor& q, const Tensor& k, const Tensor& v, bool packed, int64_t n_seq, int64_t longest) {
+    TORCH_CHECK_VALUE(q.size(0) < (1ll << 31) && q.size(1) < (1ll << 31), "batch and time must fit in 32 bits");
     return AttnCall{(int)q.size(0), (int)q.size(1), (int)n_seq,     (int)longest, (int)q.size(2),
                     (int)k.size(2), (int)q.size(3), (int)v.size(3), code(q),      packed};
 }
@@ -176,13 +177,18 @@ void attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
 
 // ------------------------------------------------------------------------------------- group norm
 
+void norm_sizes(const Tensor& x, int64_t& n, int64_t& c, int64_t& p) {
+    n = x.size(0), c = x.size(-1), p = x.numel() / (n * c);
+    TORCH_CHECK_VALUE(c < (1ll << 31) && p < (1ll << 31), "channels and positions must fit in 32 bits");
+}
 int weight_code(const Tensor& w, const Tensor& b) { return w.defined() ? code(w) : b.defined() ? code(b) : PRB_F32; }
 
 std::tuple<Tensor, Tensor> norm_fwd(const Tensor& x, int64_t groups, const OptTensor& w_, const OptTensor& b_,
                                     double eps, int64_t act, bool want_stats) {
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor xc = aligned(x), w = plain(get(w_)), b = plain(get(b_));
-    const int64_t n = x.size(0), c = x.size(-1), p = x.numel() / (n * c);
+    int64_t n, c, p;
+    norm_sizes(x, n, c, p);
     Tensor y = at::empty_like(xc);
     Tensor stats = want_stats ? at::empty({n, groups, 2}, x.options().dtype(at::kFloat)) : Tensor();
     const size_t need = prb_group_norm_workspace_bytes(n, (int)p, (int)c, (int)groups, code(x), 0);
@@ -198,7 +204,8 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(const Tensor& x, const Tensor& gy_, 
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor xc = aligned(x), gy = aligned(gy_.to(x.scalar_type())), w = plain(get(w_)), b = plain(get(b_)),
                  stats = stats_.contiguous();
-    const int64_t n = x.size(0), c = x.size(-1), p = x.numel() / (n * c);
+    int64_t n, c, p;
+    norm_sizes(x, n, c, p);
     Tensor gx = at::empty_like(xc);
     Tensor gw = w.defined() && want_params ? at::empty_like(w) : Tensor();
     Tensor gb = b.defined() && want_params ? at::empty_like(b) : Tensor();
@@ -242,6 +249,7 @@ Tensor norm(const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t gro
 
 Tensor embed_fwd(const Tensor& ids, const Tensor& table, double scale) {
     const c10::cuda::CUDAGuard guard(table.device());
+    TORCH_CHECK_VALUE(table.size(0) < (1ll << 31) && table.size(1) < (1ll << 31), "weight's sizes must fit in 32 bits");
     const Tensor idc = ids.contiguous(), w = table.contiguous();
     std::vector<int64_t> shape = ids.sizes().vec();
     shape.push_back(w.size(1));
@@ -256,6 +264,7 @@ Tensor embed_bwd(const Tensor& ids, const Tensor& grad, int64_t vocab, double sc
     const c10::cuda::CUDAGuard guard(grad.device());
     const Tensor idc = ids.contiguous(), g = grad.contiguous();
     const int64_t c = g.size(-1);
+    TORCH_CHECK_VALUE(vocab < (1ll << 31) && c < (1ll << 31), "vocab and channels must fit in 32 bits");
     if (ids.numel() == 0) return at::zeros({vocab, c}, g.options());
     Tensor out = at::empty({vocab, c}, g.options());
     const size_t need = prb_bwd_embedding_workspace_bytes(ids.numel(), (int)vocab, (int)c);

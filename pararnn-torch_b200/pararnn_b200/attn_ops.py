@@ -136,6 +136,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: 
     if block_table is not None:
         if state is None or state.dim() != 4:
             raise ValueError("block_table needs state as a pool (C, Hkv, dk, dv)")
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("block_table is checked on the host, which a CUDA graph cannot do: pass state's rows")
         rows = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
         state = gather_h0(state, block_table, rows, (k.shape[2], k.shape[3], v.shape[3]))
     _, cu, n_seq, longest, scale, sparse = _prepare(q, k, v, log_decay, state, cu_seqlens, scale)
@@ -195,6 +197,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         out = torch.empty(shape, dtype=q.dtype, device=dev)
     elif out.shape != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {shape} {q.dtype} on {dev}")
+    elif out.data_ptr() in (q.data_ptr(), k.data_ptr()):
+        raise ValueError("out must not be q or k: other heads still read them")
     if block_table is not None and not block_table.is_cuda:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a CUDA graph needs block_table on the device")

@@ -58,6 +58,14 @@ class LinearAttention(nn.Module):
         spread = torch.linspace(3.0, 9.0, n_kv_heads, device=device)
         self.register_buffer("log_decay", torch.log1p(-torch.exp2(-spread)).float())
 
+    def _apply(self, fn, *args, **kw):
+        # the schedule stays in float32 when the module is cast
+        kept = self.log_decay
+        super()._apply(fn, *args, **kw)
+        if self.log_decay.dtype != kept.dtype and not self.log_decay.is_meta:
+            self.log_decay = kept.to(self.log_decay.device)
+        return self
+
     def zero_state(self, rows: int) -> Tensor:
         return torch.zeros(rows, self.n_kv_heads, self.d_key, self.d_value, device=self.W_qkv.weight.device)
 

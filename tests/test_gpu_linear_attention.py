@@ -402,3 +402,53 @@ def test_first_call_of_a_fresh_thread():
     th.join()
     torch.cuda.synchronize()
     assert torch.equal(got[0][0], want[0]) and torch.equal(got[0][1], want[1])
+
+
+@pytest.mark.parametrize("dk,dv", [(128, 64), (64, 128), (128, 128), (40, 96)])
+@pytest.mark.parametrize("share", [1, 3])
+def test_segments_of_every_tile_shape(dk, dv, share):
+    """Rows long enough to be cut into segments, in every combination of 64- and 128-channel tiles: the state
+    sweep, the fold and the sweep from the segments' states, forwards and backwards, against the 64-bit recurrence."""
+    dtype, T = torch.bfloat16, 2300
+    q, k, v, do, g, s0, ds = make(1, T, share, 1, dk, dv, dtype, seed=dk + share, decay=-3e-3)
+    o, last = attention_oracle(q, k, v, g, s0)
+    mag_o, mag_s = attention_oracle(q.abs(), k.abs(), v.abs(), g, s0.abs())
+    args = [cuda(x, dtype) for x in (q, k, v)] + [g.cuda()]
+    got_o, got_s = la.linear_attention_fused(*args, s0.float().cuda())
+    near(got_o, o, bound(dtype, dk, T, mag_o, o), "o")
+    near(got_s, last, state_bound(dtype, dk, T, mag_s), "state")
+    want = attention_grads(q, k, v, g, do, s0, ds)
+    mags = attention_grads(q.abs(), k.abs(), v.abs(), g, do.abs(), s0.abs(), ds.abs())
+    got = la.linear_attention_reverse_vjp(*args, cuda(do, dtype), s0.float().cuda(), ds.float().cuda(),
+                                          want_state=True)
+    for name, a, w, m in zip(("dq", "dk", "dv"), got, want, mags):
+        near(a, w, bound(dtype, 128 * share, T, m, w), name)
+    near(got[3], want[3], state_bound(dtype, dk * share, T, mags[3]), "dstate")
+    # a state's terms are held to 2^-24 (three parts of the decayed key) and added in at most 24 truncating
+    # steps of 2^-23 a visit and one rounding a visit: 2^-18 of the sum of their sizes, against the 2^-17
+    # that two parts alone would leave
+    assert float(((got_s.double().cpu() - last).abs() / mag_s).max()) <= 2 ** -18
+
+
+def test_both_kernel_families_agree_in_bf16(prb_options):
+    """The tensor-core sweeps against the CUDA-core ones on the same bf16 inputs, at head sizes that both take."""
+    q, k, v, do, g, s0, ds = make(2, 333, 4, 2, 64, 96, torch.bfloat16, seed=21)
+    args = [cuda(x, torch.bfloat16) for x in (q, k, v)] + [g.cuda()]
+    more = (cuda(do, torch.bfloat16), s0.float().cuda(), ds.float().cuda())
+    a = la.linear_attention_fused(*args, s0.float().cuda()) + la.linear_attention_reverse_vjp(*args, *more, want_state=True)
+    prb_options("kernel_family", "lookback")
+    b = la.linear_attention_fused(*args, s0.float().cuda()) + la.linear_attention_reverse_vjp(*args, *more, want_state=True)
+    o, last = attention_oracle(q, k, v, g, s0)
+    mag_o, mag_s = attention_oracle(q.abs(), k.abs(), v.abs(), g, s0.abs())
+    for got in (a, b):
+        near(got[0], o, bound(torch.bfloat16, 64, 333, mag_o, o), "o")
+        near(got[1], last, state_bound(torch.bfloat16, 64, 333, mag_s), "state")
+    for x, y in zip(a, b):
+        assert float((x.double() - y.double()).norm() / y.double().norm()) <= 2 ** -7
+
+
+def test_step_refuses_an_output_that_other_heads_still_read():
+    x = torch.randn(2, 2, 64, device="cuda")
+    with pytest.raises(ValueError, match="out"):
+        prb.linear_attention_step(x, x.clone(), x.clone(), torch.zeros(2, device="cuda"),
+                                  torch.zeros(2, 2, 64, 64, device="cuda"), out=x)

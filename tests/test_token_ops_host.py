@@ -183,6 +183,8 @@ def test_layers_are_built_and_refuse_what_they_cannot_do():
     assert layer.log_decay.shape == (2,) and bool((layer.log_decay < 0).all())
     assert "log_decay" in layer.state_dict() and not layer.log_decay.requires_grad
     assert layer.zero_state(3).shape == (3, 2, 16, 32)
+    schedule = layer.log_decay.clone()
+    assert torch.equal(layer.bfloat16().log_decay, schedule) and layer.W_o.weight.dtype == torch.bfloat16
     for bad in (dict(n_heads=3), dict(n_heads=4, n_kv_heads=3)):
         with pytest.raises(ValueError):
             prb.LinearAttention(64, **bad)
