@@ -20,22 +20,24 @@ struct AttnShape {
 
 // Segments of the time axis.  One CTA walks a segment of one head (and of one block of 64 value channels on
 // the CUDA cores), so few (sequence, head) pairs leave SMs idle; cutting costs a second read of two
-// inputs (the state sweep) and two more launches, some 12 us.  A segment has at least as many tokens as
-// take about as long: 8 chunks of 128 on the tensor cores, 2 of 64 on the CUDA cores (of which two CTAs
-// share an SM up to 64 channels).  2 x 1021 tokens, 8 heads in fp32: cut in 4: 73 us, in 8: 60.
+// inputs (the state sweep) and two more launches, some 12 us.  So nothing up to 8 chunks of 128 (fp32: 2) is
+// cut, and a segment has at least 2 (fp32: 1; there two CTAs share an SM up to 64 channels).  Forward, 8 heads:
+// 2048 tokens of 64 channels uncut 39.7 us, in pieces of at least 8 chunks 38.5, of 4 27.8, of 2 22.6; 4096 of
+// 128: 100, 65.6, 50.6, 46.7; 32768 of 128: 772 uncut, 117 cut; 5 packed prompts of 739 tokens with their
+// states: 22 uncut, 34 cut; fp32 2 x 1021 in 4 pieces 73, in 8 60.
 SegMap plan_segments(const AttnShape& s, const int* cu, bool backward) {
     SegMap m{};
     m.cu = cu;
     m.n_seq = s.n_seq;
     m.time = s.time;
     const bool simt = s.dtype == PRB_F32, narrow = s.dk <= 64 && (s.dv <= 64 || !backward);
-    const int chunk = 128, sm = sm_count() * (simt && narrow ? 2 : 1), least = simt ? chunk : 8 * chunk;
+    const int chunk = 128, sm = sm_count() * (simt && narrow ? 2 : 1), least = simt ? chunk : 2 * chunk;
     const int blocks_v = simt ? (s.dv + 63) / 64 : 1, blocks_k = simt ? (s.dk + 63) / 64 : 1;
     const long long jobs =
         backward ? (long long)s.hq * blocks_k + s.hkv * (blocks_k + blocks_v) : (long long)s.hq * blocks_v;
     const long long tokens = cu ? s.time : (long long)s.rows * s.time;
     long long len = s.max_len;
-    if ((long long)s.n_seq * jobs < sm) {
+    if (s.max_len > (simt ? 2 : 8) * chunk && (long long)s.n_seq * jobs < sm) {
         // rectangular: as many equal segments as one wave holds; packed: an even share of all tokens
         const long long cuts = sm / (s.n_seq * jobs);
         len = cu ? (tokens * jobs + sm - 1) / sm : (s.time + cuts - 1) / cuts;

@@ -10,8 +10,10 @@
 //   place   pos[offset[id_t] + rank_t] = t
 //   order   one CTA per long list: a bitmap over the positions puts them in order
 //   sums    a warp per row sorts its <= 32 positions with shuffles and adds; a long list is cut into
-//           pieces of max(64, sqrt n) positions, a CTA each, whose sums go to the workspace
+//           pieces of max(128, sqrt n) positions, a CTA each, whose sums go to the workspace
 //   join    the pieces of a long list, in order
+// 32768 natural-text ids into 50304 x 768 bf16: 61 us, of which the one pass over the 127 MB takes 35 and the
+// six short launches around it the rest; the lookup itself takes 12 us (8.4 TB/s, part of it from L2).
 // Frequent tokens (a padding id, the head of a natural-text distribution) are thereby spread over
 // many CTAs instead of queueing on one row.
 #include "embedding.cuh"
@@ -22,9 +24,10 @@ namespace {
 
 constexpr int kT = 256;
 constexpr int kShort = 32;
-constexpr int kPiece = 64;
+constexpr int kPiece = 128;  // 32768 natural-text ids, 768 channels: 61 us, 65 with pieces of 64
 constexpr int kOrderT = 512;
 constexpr int kWindowWords = 8192;  // 262144 positions per bitmap
+constexpr int kFew = 2048, kFewRows = 4;  // tokens, and rows per CTA, up to which one launch does it all
 
 struct LongSeg {
     int id, off, n, piece0, piece_len;
@@ -261,6 +264,106 @@ __global__ void __launch_bounds__(kT) embed_join(const __grid_constant__ EmbedAr
     }
 }
 
+// Few tokens: every CTA reads all ids, keeps those of its own rows in the order of their positions, and writes
+// its rows.  One launch instead of seven short ones: 1531 tokens, 997 x 257 fp32 take 6.7 us against 17.5.
+// With many rows per CTA the lists are walked too often (2048 tokens, 50304 rows: 39 us against 30).  A
+// row with many positions is split over the CTA's warps in order, the parts are added in order.
+template <typename T, int V>
+__global__ void __launch_bounds__(kT) embed_few(const __grid_constant__ EmbedArgs a, int rows_per_cta) {
+    __shared__ int list_pos[kFew], list_row[kFew], warp_sum[kT / 32];
+    __shared__ int mine[kFew];
+    __shared__ float part[kT / 32][32 * V];
+    const int v0 = blockIdx.x * rows_per_cta, v1 = min(a.vocab, v0 + rows_per_cta);
+    const int n_tok = (int)a.tokens, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kPer = kFew / kT;  // neighbouring tokens of a thread
+    int row[kPer], cnt = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int t = threadIdx.x * kPer + i;
+        const long long id = t < n_tok ? id_at(a, t) : -1;
+        row[i] = id >= v0 && id < v1 ? (int)id : -1;
+        cnt += row[i] >= 0;
+    }
+    int inc = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    int at = inc - cnt, n_list = 0;
+    for (int i = 0; i < kT / 32; ++i) {
+        if (i < warp) at += warp_sum[i];
+        n_list += warp_sum[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (row[i] >= 0) {
+            list_row[at] = row[i];
+            list_pos[at++] = threadIdx.x * kPer + i;
+        }
+    __syncthreads();
+    const int nv = a.channels / V;
+    const Vec<T, V>* src = reinterpret_cast<const Vec<T, V>*>(a.dy);
+    for (int v = v0; v < v1; ++v) {
+        // positions of the row, in order; every warp counts, one writes
+        int n = 0;
+        for (int i0 = 0; i0 < n_list; i0 += 32) {
+            const bool hit = i0 + lane < n_list && list_row[i0 + lane] == v;
+            const unsigned b = __ballot_sync(0xffffffffu, hit);
+            if (hit && warp == 0) mine[n + __popc(b & ((1u << lane) - 1))] = list_pos[i0 + lane];
+            n += __popc(b);
+        }
+        __syncthreads();
+        Vec<T, V>* dst = reinterpret_cast<Vec<T, V>*>(a.out) + (size_t)v * nv;
+        if (n <= kShort) {
+            for (int i = threadIdx.x; i < nv; i += kT) {
+                float acc[V] = {};
+#pragma unroll 4
+                for (int k = 0; k < n; ++k) {
+                    const Vec<T, V> x = src[(size_t)mine[k] * nv + i];
+#pragma unroll
+                    for (int q = 0; q < V; ++q) acc[q] += static_cast<float>(x.v[q]);
+                }
+                Vec<T, V> y;
+#pragma unroll
+                for (int q = 0; q < V; ++q) st_f(&y.v[q], a.scale * acc[q]);
+                dst[i] = y;
+            }
+        } else {
+            const int k0 = n * warp / (kT / 32), k1 = n * (warp + 1) / (kT / 32);
+            for (int i0 = 0; i0 < nv; i0 += 32) {
+                float acc[V] = {};
+                if (i0 + lane < nv) {
+#pragma unroll 8
+                    for (int k = k0; k < k1; ++k) {
+                        const Vec<T, V> x = src[(size_t)mine[k] * nv + i0 + lane];
+#pragma unroll
+                        for (int q = 0; q < V; ++q) acc[q] += static_cast<float>(x.v[q]);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < V; ++q) part[warp][lane * V + q] = acc[q];
+                __syncthreads();
+                if (warp == 0 && i0 + lane < nv) {
+                    Vec<T, V> y;
+#pragma unroll
+                    for (int q = 0; q < V; ++q) {
+                        float s = 0.f;
+#pragma unroll
+                        for (int w = 0; w < kT / 32; ++w) s += part[w][lane * V + q];
+                        st_f(&y.v[q], a.scale * s);
+                    }
+                    dst[i0 + lane] = y;
+                }
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+    }
+}
+
 template <typename T>
 int vec_of(const EmbedArgs& a, const void* p, const void* q) {
     const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q);
@@ -278,6 +381,11 @@ cudaError_t fwd_t(const EmbedArgs& a, cudaStream_t s) {
 
 template <typename T, int V>
 cudaError_t grad_t(const EmbedArgs& a, const EmbedPlan& pl, char* ws, cudaStream_t s) {
+    const int ctas = 4 * sm_count(), per = (a.vocab + ctas - 1) / ctas;
+    if (a.tokens <= kFew && per <= kFewRows) {
+        embed_few<T, V><<<(a.vocab + per - 1) / per, kT, 0, s>>>(a, per);
+        return cudaGetLastError();
+    }
     int* counters = reinterpret_cast<int*>(ws + pl.counters);
     int* counts = reinterpret_cast<int*>(ws + pl.counts);
     int* offsets = reinterpret_cast<int*>(ws + pl.offsets);
