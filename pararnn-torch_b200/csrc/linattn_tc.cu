@@ -26,8 +26,8 @@
 // state of the low parts, and S is the sum of the two.  The third part is one more piece behind them.
 //
 // b^T reaches TMEM through transposing ldmatrix loads: a fragment of 8 x 8 holds token pairs of one
-// channel, which is what a 16x128b TMEM store wants.  It is made in two halves of 64 tokens, so that
-// one half is written while the matrix unit reads the other.  The decay of a score off the diagonal
+// channel, which is what a 16x128b TMEM store wants.  With da = 128 it is made in two halves of 64 tokens, so
+// that one half is written while the matrix unit reads the other.  The decay of a score off the diagonal
 // 32 x 32 blocks is a product of a row and a column factor.
 //
 // With da = dc = 64 there is room for the scores and X twice (kTwice): the scores of visit i + 1 are made
@@ -39,6 +39,12 @@
 // A masked score is 0, and 0 x inf = NaN: a chunk whose c holds an inf or a NaN skips the product with c
 // on the tensor cores; its rows are summed over the positions that they may see (row_mix),
 // so that nothing behind the mask can reach them.
+//
+// Measured: forward 16 x 4096, 8 heads of 64: 77 us, 16 x 2048, 8 heads of 128: 59 us, against 41 us of memory traffic
+// at the copy rate for both; with backward 294 and 224 against 82 (its three jobs read 9 inputs where one
+// pass would read 4).  A chunk takes 4300 resp. 5600 cycles: the MMA warp's walk over the barriers, with the
+// tensor pipe active for 22 resp. 40 % of the time.  128 tokens per chunk because tcgen05 works on 128 rows;
+// one CTA per SM because the TMEM regions and two to four stages of tiles fill one.
 //
 // Every wait has a limit; a CTA whose wait runs out raises g_status, lets its copies and matrix
 // products in flight end, frees its TMEM and leaves.
