@@ -409,7 +409,8 @@ cudaError_t grad_t(const EmbedArgs& a, const EmbedPlan& pl, char* ws, cudaStream
                                                   pieces);
     if (longs) {
         const int cols = (a.channels + kT - 1) / kT;
-        embed_join<T><<<dim3(longs < 2 * sm_count() ? longs : 2 * sm_count(), cols < 64 ? cols : 64), kT, 0, s>>>(a, counters, segs, partial);
+        const dim3 grid(longs < 2 * sm_count() ? longs : 2 * sm_count(), cols < 64 ? cols : 64);
+        embed_join<T><<<grid, kT, 0, s>>>(a, counters, segs, partial);
     }
     return cudaGetLastError();
 }

@@ -7,7 +7,7 @@
 // float4 from shared memory), which bounds it; tensor cores would round the operands to fewer bits
 // than an fp32 caller asked for.  The next chunk travels from global memory to registers while a
 // chunk is worked on, and with da <= 64 two CTAs share an SM.  2 x 1021 tokens, 8 query and 2 key heads of
-// 64 / 96 channels: 60 us in 8 segments (state sweep 11, fold 4, outputs 45).
+// 64 / 96 channels: 60 us in 8 segments (kernels traced one by one: state sweep 11, fold 3, outputs 47).
 #include "linattn.cuh"
 
 namespace prb {

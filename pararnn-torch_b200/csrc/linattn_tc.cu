@@ -33,8 +33,8 @@
 // With da = dc = 64 there is room for the scores and X twice (kTwice): the scores of visit i + 1 are made
 // and converted while the matrix unit works on X of visit i.  With 128 channels the four
 // regions fill all 512 columns.  The state warps publish S, read U and write b^T in program order, so
-// one barrier (b_ready) tells the MMA thread all three; every further barrier would cost it some 200
-// cycles a visit.
+// one barrier (b_ready) tells the MMA thread all three; every further barrier would cost it 200 -
+// 230 cycles a visit (read from clocks in the loop, which add to what they time).
 //
 // A masked score is 0, and 0 x inf = NaN: a chunk whose c holds an inf or a NaN skips the product with c
 // on the tensor cores; its rows are summed over the positions that they may see (row_mix),
@@ -42,8 +42,9 @@
 //
 // Measured: forward 16 x 4096, 8 heads of 64: 77 us, 16 x 2048, 8 heads of 128: 59 us, against 41 us of memory traffic
 // at the copy rate for both; with backward 294 and 224 against 82 (its three jobs read 9 inputs where one
-// pass would read 4).  A chunk takes 4300 resp. 5600 cycles: the MMA warp's walk over the barriers, with the
-// tensor pipe active for 22 resp. 40 % of the time.  128 tokens per chunk because tcgen05 works on 128 rows;
+// pass would read 4).  A chunk takes 2.4 resp. 3.7 us (time over chunks, start-up included) where the copy rate
+// would allow 1.3 resp. 2.6: the MMA warp's walk over the barriers, with the tensor pipe active for 22
+// resp. 40 % of the cycles.  128 tokens per chunk because tcgen05 works on 128 rows;
 // one CTA per SM because the TMEM regions and two to four stages of tiles fill one.
 //
 // Every wait has a limit; a CTA whose wait runs out raises g_status, lets its copies and matrix
