@@ -627,9 +627,11 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                         *reinterpret_cast<uint4*>(tb + q * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
             }
+            // every warp reads all rows of its channels below: the zeroes of the other warps have to be there, in
+            // each visit of a ragged chunk (share_b > 1 visits it once for each query head)
+            if (n < kC || n != table_n) asm volatile("bar.sync 1, 128;" ::: "memory");
             if (n != table_n) {
                 // the decays of this chunk length (all chunks but the ragged one have the same)
-                asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (r < kC / 2) ct.wb[r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 table_n = n;
@@ -1123,8 +1125,9 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
                         *reinterpret_cast<uint4*>(tb + q * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
             }
+            // as in mix_tc_kernel: no warp reads the rows before all of them are zero
+            if (n < kC || n != table_n) asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
             if (n != table_n) {
-                asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
                 if (r < kC / 2) {
                     ct.wb[group][r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
                     ct.wf[group][r] = weight_f32(ct.pw, r, n, reverse, jb.upd_scale);
