@@ -231,7 +231,9 @@ struct NormNode : torch::autograd::Function<NormNode> {
         once("group_norm");
         const variable_list s = ctx->get_saved_variables();
         auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-        const bool nw = s[1].defined() && ctx->needs_input_grad(1), nb = s[2].defined() && ctx->needs_input_grad(2);
+        // edges count the tensors that were given: without a weight the bias is edge 1
+        const bool has_w = s[1].defined(), nw = has_w && ctx->needs_input_grad(1),
+                   nb = s[2].defined() && ctx->needs_input_grad(has_w ? 2 : 1);
         auto [gx, gw, gb] = norm_bwd(s[0], grads[0], s[3], ctx->saved_data["groups"].toInt(), opt(s[1]), opt(s[2]),
                                      ctx->saved_data["act"].toInt(), nw || nb);
         variable_list r(6);
