@@ -39,6 +39,11 @@ void once(const char* name) {
 Tensor scratch(size_t bytes, const Tensor& like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
+// A kernel has written `t` through its pointer: autograd is told, so that a node which saved `t` refuses its
+// backward pass instead of reading the new values.
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Tensor plain(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 Tensor aligned(const Tensor& t) {
     Tensor c = t.contiguous();
@@ -173,6 +178,8 @@ void attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
                                     (int)state.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)v.size(2),
                                     code(q), (float)scale, stream(q)),
           "linear_attention_step");
+    written(state);
+    written(out);
 }
 
 // ------------------------------------------------------------------------------------- group norm
