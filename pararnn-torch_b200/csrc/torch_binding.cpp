@@ -169,8 +169,29 @@ std::tuple<Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Ten
     return {r[0], r.size() > 1 ? r[1] : Tensor()};
 }
 
+// Memory that a call writes must hold nothing else that it reads or writes: other CTAs (heads, slices of the value
+// channels, the one that applies a repeated slot's rows) may still be at it.
+void apart(const Tensor& w, const char* w_name, const Tensor& t, const char* name) {
+    // a tensor that is not contiguous is copied before the launch
+    if (!t.defined() || !t.is_contiguous() || t.numel() == 0 || w.numel() == 0) return;
+    const uintptr_t w0 = reinterpret_cast<uintptr_t>(w.data_ptr()), t0 = reinterpret_cast<uintptr_t>(t.data_ptr());
+    TORCH_CHECK_VALUE(w0 + w.nbytes() <= t0 || t0 + t.nbytes() <= w0, w_name, " must not share memory with ", name);
+}
+
 void attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& state,
                     const OptTensor& table_, double scale, const Tensor& out) {
+    apart(out, "out", q, "q");
+    apart(out, "out", k, "k");
+    // a value is read by the CTA that writes the output in its place, so out may be v where the heads are the same
+    if (out.data_ptr() != v.data_ptr() || q.size(1) != k.size(1)) apart(out, "out", v, "v");
+    apart(out, "out", decay, "log_decay");
+    apart(out, "out", state, "state");
+    apart(out, "out", get(table_), "block_table");
+    apart(state, "state", q, "q");
+    apart(state, "state", k, "k");
+    apart(state, "state", v, "v");
+    apart(state, "state", decay, "log_decay");
+    apart(state, "state", get(table_), "block_table");
     const c10::cuda::CUDAGuard guard(q.device());
     const Tensor qc = q.contiguous(), kc = k.contiguous(), vc = v.contiguous(), table = plain(get(table_));
     check(prb_linear_attention_step(ptr(qc), ptr(kc), ptr(vc), (const float*)ptr(decay), (float*)ptr(state), ptr(table),

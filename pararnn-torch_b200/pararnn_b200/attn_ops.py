@@ -155,7 +155,9 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     result then has too); ``state`` is a contiguous float32 ``(B,Hkv,dk,dv)``, or with ``block_table``
     ``(B,)`` a pool ``(C,Hkv,dk,dv)`` whose named slots are updated.  Slots outside the pool mark padding
     rows: they touch no state and their outputs are zero.  A slot that several rows name takes
-    them in row order.  One launch, no allocation with ``out=``: CUDA graphs can capture it."""
+    them in row order.  ``out`` and ``state`` share no memory with one another or with an input (``out``
+    may be ``v`` itself where ``Hq = Hkv``).  One launch, no allocation with ``out=``: CUDA graphs can
+    capture it."""
     # this call is the latency of a token: its checks are kept short
     if (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or state.requires_grad) \
             and torch.is_grad_enabled():

@@ -1,0 +1,86 @@
+"""What the token-model operators refuse about memory and sizes, on the CPU: the checks of the native operators come
+before any CUDA work."""
+
+import pytest
+import torch
+
+from pararnn_b200 import _lib
+
+ROWS, D = 3, 8
+
+
+def step(q, k, v, decay, state, out, table=None):
+    _lib.native().attention_step(q, k, v, decay, state, table, 1.0, out)
+
+
+def parts(hq=2, hkv=2):
+    return dict(q=torch.zeros(ROWS, hq, D), k=torch.zeros(ROWS, hkv, D), v=torch.zeros(ROWS, hkv, D),
+                decay=torch.zeros(hkv), state=torch.zeros(ROWS, hkv, D, D), out=torch.zeros(ROWS, hq, D))
+
+
+@pytest.mark.parametrize("name", ["q", "k"])
+@pytest.mark.parametrize("shift", [-5, -1, 0, 1, 7, ROWS * 2 * D - 1])
+def test_step_refuses_an_output_anywhere_inside_an_input(name, shift):
+    n = ROWS * 2 * D
+    flat = torch.zeros(3 * n)
+    a = parts()
+    a[name] = flat[n:2 * n].view(ROWS, 2, D)
+    a["out"] = flat[n + shift:2 * n + shift].view(ROWS, 2, D)
+    with pytest.raises(ValueError, match=f"out must not share memory with {name}"):
+        step(**a)
+
+
+def test_step_takes_a_neighbouring_output_and_v_itself():
+    """No refusal: the call gets as far as the device, which the CPU does not have."""
+    n = ROWS * 2 * D
+    flat = torch.zeros(3 * n)
+    a = parts()
+    a["q"], a["out"] = flat[n:2 * n].view(ROWS, 2, D), flat[:n].view(ROWS, 2, D)
+    with pytest.raises(RuntimeError) as e:
+        step(**a)
+    assert "share memory" not in str(e.value)
+    a = parts()
+    a["out"] = a["v"]
+    with pytest.raises(RuntimeError) as e:
+        step(**a)
+    assert "share memory" not in str(e.value)
+    # slices of one buffer that are not contiguous are copied first
+    fused = torch.zeros(ROWS, 6, D)
+    a = parts()
+    a["q"], a["k"], a["v"] = fused[:, :2], fused[:, 2:4], fused[:, 4:]
+    a["out"] = fused.view(-1)[:n].view(ROWS, 2, D)
+    with pytest.raises(RuntimeError) as e:
+        step(**a)
+    assert "share memory" not in str(e.value)
+
+
+def test_step_refuses_v_at_an_offset_or_with_other_heads():
+    n = ROWS * 2 * D
+    flat = torch.zeros(4 * n)
+    a = parts()
+    a["v"], a["out"] = flat[:n].view(ROWS, 2, D), flat[D:n + D].view(ROWS, 2, D)
+    with pytest.raises(ValueError, match="with v"):
+        step(**a)
+    a = parts(hq=4)
+    a["v"], a["out"] = flat[:n].view(ROWS, 2, D), flat[:2 * n].view(ROWS, 4, D)
+    with pytest.raises(ValueError, match="with v"):
+        step(**a)
+
+
+def test_step_refuses_states_decays_and_tables_in_written_memory():
+    pool = torch.zeros(ROWS * 2 * D * D + 64)
+    a = parts()
+    a["state"] = pool[64:].view(ROWS, 2, D, D)
+    for name, match in (("out", "out must not share memory with state"), ("q", "state must not share memory with q"),
+                        ("v", "state must not share memory with v")):
+        b = dict(a)
+        b[name] = pool[50:50 + ROWS * 2 * D].view(ROWS, 2, D)
+        with pytest.raises(ValueError, match=match):
+            step(**b)
+    a = parts()
+    a["decay"] = a["out"].view(-1)[4:6]
+    with pytest.raises(ValueError, match="log_decay"):
+        step(**a)
+    a = parts()
+    with pytest.raises(ValueError, match="block_table"):
+        step(**a, table=a["out"].view(-1)[2:2 + ROWS].view(torch.int32))
