@@ -36,6 +36,10 @@ void once(const char* name) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the gradient of ", name,
                 " cannot be differentiated again (create_graph=True)");
 }
+// the C ABI counts rows, heads and slots in 32 bits
+void narrow(std::initializer_list<int64_t> sizes, const char* what) {
+    for (const int64_t n : sizes) TORCH_CHECK_VALUE(n < (1ll << 31), what, " must fit in 32 bits, got ", n);
+}
 Tensor scratch(size_t bytes, const Tensor& like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
@@ -75,7 +79,7 @@ struct AttnCall {
     }
 };
 AttnCall attn_call(const Tensor& q, const Tensor& k, const Tensor& v, bool packed, int64_t n_seq, int64_t longest) {
-    TORCH_CHECK_VALUE(q.size(0) < (1ll << 31) && q.size(1) < (1ll << 31), "batch and time must fit in 32 bits");
+    narrow({q.size(0), q.size(1), q.size(2), k.size(2), n_seq}, "batch, time and heads");
     return AttnCall{(int)q.size(0), (int)q.size(1), (int)n_seq,     (int)longest, (int)q.size(2),
                     (int)k.size(2), (int)q.size(3), (int)v.size(3), code(q),      packed};
 }
@@ -84,9 +88,9 @@ AttnCall attn_call(const Tensor& q, const Tensor& k, const Tensor& v, bool packe
 std::tuple<Tensor, Tensor> attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay,
                                          const OptTensor& state_, const OptTensor& cu_, int64_t n_seq,
                                          int64_t longest, double scale, bool want_state, bool sparse) {
+    const AttnCall c = attn_call(q, k, v, cu_.has_value(), n_seq, longest);
     const c10::cuda::CUDAGuard guard(q.device());
     const Tensor state = plain(get(state_)), cu = get(cu_);
-    const AttnCall c = attn_call(q, k, v, cu.defined(), n_seq, longest);
     prb_heads hq, hk, hv;
     const Tensor qc = heads(q, hq), kc = heads(k, hk), vc = heads(v, hv);
     Tensor out = at::empty({c.rows, c.time, c.hq, c.dv}, q.options());
@@ -106,9 +110,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_bwd(const Tensor& q, const 
                                                          const OptTensor& state_, const OptTensor& grad_state_,
                                                          const OptTensor& cu_, int64_t n_seq, int64_t longest,
                                                          double scale, bool want_state, bool sparse) {
+    const AttnCall c = attn_call(q, k, v, cu_.has_value(), n_seq, longest);
     const c10::cuda::CUDAGuard guard(q.device());
     const Tensor state = plain(get(state_)), gs = plain(get(grad_state_)), cu = get(cu_);
-    const AttnCall c = attn_call(q, k, v, cu.defined(), n_seq, longest);
     prb_heads hq, hk, hv, hg;
     const Tensor qc = heads(q, hq), kc = heads(k, hk), vc = heads(v, hv), gc = heads(grad_.to(q.scalar_type()), hg);
     Tensor g_q = at::empty({c.rows, c.time, c.hq, c.dk}, q.options());
@@ -180,6 +184,7 @@ void apart(const Tensor& w, const char* w_name, const Tensor& t, const char* nam
 
 void attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& state,
                     const OptTensor& table_, double scale, const Tensor& out) {
+    narrow({q.size(0), q.size(1), k.size(1), state.size(0)}, "rows, heads and slots");
     apart(out, "out", q, "q");
     apart(out, "out", k, "k");
     // a value is read by the CTA that writes the output in its place, so out may be v where the heads are the same

@@ -84,3 +84,30 @@ def test_step_refuses_states_decays_and_tables_in_written_memory():
     a = parts()
     with pytest.raises(ValueError, match="block_table"):
         step(**a, table=a["out"].view(-1)[2:2 + ROWS].view(torch.int32))
+
+
+def meta(*shape, dtype=torch.float32):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+BIG = 2 ** 32 + 3  # 3 in 32 bits
+
+
+@pytest.mark.parametrize("change", [
+    dict(state=(BIG, 1, 1, 1)), dict(q=(BIG, 1, 1), k=(BIG, 1, 1), v=(BIG, 1, 1), out=(BIG, 1, 1)),
+    dict(q=(1, BIG, 1), out=(1, BIG, 1)),
+])
+def test_step_refuses_sizes_that_32_bits_would_cut(change):
+    shapes = dict(q=(1, 1, 1), k=(1, 1, 1), v=(1, 1, 1), decay=(1,), state=(3, 1, 1, 1), out=(1, 1, 1))
+    shapes.update(change)
+    with pytest.raises(ValueError, match="32 bits"):
+        step(**{n: meta(*s) for n, s in shapes.items()}, table=meta(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("shape", [(BIG, 1, 1, 1), (1, BIG, 1, 1), (1, 1, BIG, 1)])
+def test_sequences_refuse_sizes_that_32_bits_would_cut(shape):
+    x, g = meta(*shape), meta(shape[2])
+    with pytest.raises(ValueError, match="32 bits"):
+        _lib.native().attention_fwd(x, x, x, g, None, None, shape[0], shape[1], 1.0, False, False)
+    with pytest.raises(ValueError, match="32 bits"):
+        _lib.native().attention_bwd(x, x, x, g, x, None, None, None, shape[0], shape[1], 1.0, False, False)
