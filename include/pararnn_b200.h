@@ -71,8 +71,9 @@ const char* prb_error_string(int code);
  *                          0 also keeps linear attention on the CUDA cores
  *   PRB_OPT_PICARD_FUSED    1 (default) / 0: all Picard passes in one sweep when the shape allows
  *   PRB_OPT_NEWTON_FUSED    1 (default) / 0: all Newton iterations in one sweep when it allows
- *   PRB_OPT_SPIN_LIMIT      polls after which a look-back wait gives up and reports
- *                           PRB_STATUS_CHAIN_TIMEOUT; <= 0 restores the default */
+ *   PRB_OPT_SPIN_LIMIT      polls after which a look-back wait, or a wait of the linear attention
+ *                           sweeps, gives up and reports PRB_STATUS_CHAIN_TIMEOUT; <= 0
+ *                           restores the default */
 enum { PRB_OPT_KERNEL_FAMILY = 0, PRB_OPT_PICARD_FUSED = 1, PRB_OPT_NEWTON_FUSED = 2, PRB_OPT_SPIN_LIMIT = 3 };
 int prb_debug_set(int option, long long value);
 

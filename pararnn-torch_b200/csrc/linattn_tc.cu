@@ -196,6 +196,7 @@ struct TcParams {
     MixParams p;
     CUtensorMap map[3][4];  // [job][a, b, c, out]
     int units;              // heads of all jobs per state head
+    uint32_t wait_limit;    // polls after which a wait gives up
 };
 
 constexpr uint32_t kCtlBytes = 2048, kMaxSmem = 227 * 1024;
@@ -247,7 +248,7 @@ struct Control {
     // one per stage: their producers may be several visits ahead of (or behind) the others
     uint64_t full[4], empty[4], scanned[4], staged[4];
     // one visit or chunk at a time
-    uint64_t p_full[2], p_ready, b_ready[3], b_free[3], i_full, o_full, x_free, drain;
+    uint64_t p_full[2], p_ready, b_ready[3], b_free[3], i_full, o_full, x_free, drain, group;
     uint32_t tmem;
     int dead;
     int dirty[4];
@@ -261,8 +262,8 @@ static_assert(sizeof(Control) <= kCtlBytes, "control block");
 // false: the limit ran out.  One compact loop: the roles' code shares the instruction cache, and every
 // visit passes a dozen waits.  The roles stop one after the other, each at its own wait.
 template <typename C>
-__device__ __forceinline__ bool wait(C& ct, uint64_t* bar, uint32_t parity) {
-    uint32_t left = kWaitLimit;
+__device__ __forceinline__ bool wait(C& ct, uint32_t limit, uint64_t* bar, uint32_t parity) {
+    uint32_t left = limit;
 #pragma unroll 1
     while (!mbar_try_wait(bar, parity))
         if (--left == 0) {
@@ -273,8 +274,34 @@ __device__ __forceinline__ bool wait(C& ct, uint64_t* bar, uint32_t parity) {
 }
 // for whole warps: all lanes leave together
 template <typename C>
-__device__ __forceinline__ bool wait_warp(C& ct, uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, wait(ct, bar, parity));
+__device__ __forceinline__ bool wait_warp(C& ct, uint32_t limit, uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait(ct, limit, bar, parity));
+}
+// The four warps of a group meet inside their loop, which one of them may have left after a wait of its own
+// that ran out: a barrier with the same limit in the place of bar.sync, which would wait for that warp for ever.
+template <typename C>
+__device__ __forceinline__ bool meet(C& ct, uint32_t limit, uint64_t* bar) {
+    __syncwarp();
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) {
+        uint64_t phase;
+        asm volatile("mbarrier.arrive.shared::cta.b64 %0, [%1];" : "=l"(phase) : "r"(smem_u32(bar)) : "memory");
+        uint32_t left = limit;
+#pragma unroll 1
+        do {
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok)
+                : "r"(smem_u32(bar)), "l"(phase)
+                : "memory");
+        } while (!ok && --left);
+        if (!ok) ct.dead = 1;
+    }
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __syncwarp();
+    return ok != 0;
 }
 
 // The rows that hold something not finite read their operands again from global memory.
@@ -322,6 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     unsigned char* smem = raw + (base - raw_at);
     Control& ct = *reinterpret_cast<Control*>(smem + L::kOffCtl);
     const MixParams& p = tp.p;
+    const uint32_t limit = tp.wait_limit;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // shares of the 512 x 128 registers of the launch: 128 S + 256 O + 128 M <= 65536
     constexpr int kRegS = DC == 64 ? 152 : 208, kRegO = DC == 64 ? 144 : 112, kRegM = 64;
@@ -360,6 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         mbar_init(&ct.o_full, 1);
         mbar_init(&ct.x_free, 8);
         mbar_init(&ct.drain, 1);
+        mbar_init(&ct.group, 4);
         ct.dead = 0;
         mbar_fence_init();
     }
@@ -412,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             const CUtensorMap* mc = &tp.map[ji][2];
             int it = 0;
             for (Visit v; it < n_it; ++it, next(v)) {
-                if (it >= L::kStages && !wait(ct, &ct.empty[v.st], v.lap ^ 1)) break;
+                if (it >= L::kStages && !wait(ct, limit, &ct.empty[v.st], v.lap ^ 1)) break;
                 const uint32_t at = base + v.st * L::kStage;
                 const int t = seg.t0 + offset(v), hb = share > 1 ? head * share + v.g : hs;
                 uint64_t* full = &ct.full[v.st];
@@ -433,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         constexpr uint32_t kScores = instr_desc(kC, false), kOut = instr_desc(DC, true);
         // scores of visit it (stage v.st); false: a wait ran out
         auto scores = [&](int it, const Visit& v) {
-            if (!wait_warp(ct, &ct.full[v.st], v.lap)) return false;
+            if (!wait_warp(ct, limit, &ct.full[v.st], v.lap)) return false;
             tc_fence_after();
             const uint32_t sa = base + v.st * L::kStage;
             const uint64_t da = smem_desc(sa, 16), db = smem_desc(sa + L::kA, 16);
@@ -455,13 +484,13 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             if (kTwice) {
                 // one visit ahead; the region is free when the product of visit it - 1 has ended
                 if (it + 1 < n_it) {
-                    if (it > 0 && !wait_warp(ct, &ct.o_full, par ^ 1)) break;
+                    if (it > 0 && !wait_warp(ct, limit, &ct.o_full, par ^ 1)) break;
                     if (!scores(it + 1, ahead)) break;
                     next(ahead);
                 }
                 if (it < 0) continue;
             } else {
-                if (it > 0 && !wait_warp(ct, &ct.o_full, par ^ 1)) break;
+                if (it > 0 && !wait_warp(ct, limit, &ct.o_full, par ^ 1)) break;
                 if (!scores(it, v)) break;
             }
             const uint32_t sa = base + v.st * L::kStage;
@@ -469,10 +498,10 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             bool ok = true;
 #pragma unroll
             for (int hf = 0; hf < L::kHalves; ++hf) {
-                if (!(ok = wait_warp(ct, &ct.b_ready[hf], par))) break;
+                if (!(ok = wait_warp(ct, limit, &ct.b_ready[hf], par))) break;
                 const bool first = hf == 0 && v.g == 0;
                 // twice: p_ready of the last chunk told that the epilogue before it has read this X
-                if (first && !kTwice && v.m > 0 && !(ok = wait_warp(ct, &ct.x_free, mpar ^ 1))) break;
+                if (first && !kTwice && v.m > 0 && !(ok = wait_warp(ct, limit, &ct.x_free, mpar ^ 1))) break;
                 tc_fence_after();
                 if (elect_one()) {
                     if (first) {
@@ -497,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             }
             if (!ok) break;
             if (exact) {
-                if (!wait_warp(ct, &ct.b_ready[2], par)) break;
+                if (!wait_warp(ct, limit, &ct.b_ready[2], par)) break;
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
@@ -508,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 }
                 __syncwarp();
             }
-            if (!wait_warp(ct, &ct.p_ready, par)) break;
+            if (!wait_warp(ct, limit, &ct.p_ready, par)) break;
             tc_fence_after();
             const bool skip = *reinterpret_cast<volatile int*>(&ct.dirty[v.st]) != 0;
             if (elect_one()) {
@@ -532,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         if (lane == 0) {
             Visit v;
             for (int it = 0; it < n_it; ++it, next(v)) {
-                if (!wait(ct, &ct.staged[v.st], v.lap)) break;
+                if (!wait(ct, limit, &ct.staged[v.st], v.lap)) break;
                 const int off = offset(v);
                 if (v.g == share - 1 && seg.len - off >= kC) {
                     for (int q = 0; q < DC / 64; ++q)
@@ -550,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         // ---- scan of c
         Visit v;
         for (int it = 0; it < n_it; ++it, next(v)) {
-            if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
+            if (!wait_warp(ct, limit, &ct.full[v.st], v.lap)) break;
             const int rows = min(kC, seg.len - offset(v));
             const unsigned char* tc = smem + v.st * L::kStage + L::kA + L::kB;
             // 0 x inf and 0 x NaN are NaN
@@ -582,11 +611,11 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         {
             const bool given = jb.s_in && r < jb.da;
             const float* from = given ? jb.s_in + sbase + (size_t)r * jb.s_row : nullptr;
-            const int limit = given ? jb.dc : 0;
+            const int n_col = given ? jb.dc : 0;
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
                 S[c] = 0.f;
-                if (c < limit) S[c] = __ldg(from);
+                if (c < n_col) S[c] = __ldg(from);
                 from += jb.s_col;
             }
         }
@@ -597,8 +626,11 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         const uint32_t from = base + L::kA + (d0 >> 6) * kPanel + (lane & 7) * 128 +
                               ((((d0 & 63) + 8 * (lane >> 3)) * 2) ^ ((lane & 7) << 4));
         bool ok = true;
-        int table_n = -1;
         Visit v;
+        // the table of the first chunk; no warp has passed a wait yet, so all four reach this barrier
+        int table_n = min(kC, seg.len - offset(v));
+        if (r < kC / 2) ct.wb[r] = weight_pair(ct.pw, r, table_n, reverse, jb.upd_scale);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
         for (int it = 0; it < n_it; ++it, next(v)) {
             const int n = min(kC, seg.len - offset(v));
             const uint32_t par = it & 1;
@@ -616,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
                 }
                 fence_proxy_async();
             }
-            if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
+            if (!wait_warp(ct, limit, &ct.full[v.st], v.lap)) break;
             if (n < kC) {
                 // tokens of the next sequence behind the last one of this: no value of theirs may reach a
                 // product, not even as 0 x inf
@@ -629,18 +661,18 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             }
             // every warp reads all rows of its channels below: the zeroes of the other warps have to be there, in
             // each visit of a ragged chunk (share_b > 1 visits it once for each query head)
-            if (n < kC || n != table_n) asm volatile("bar.sync 1, 128;" ::: "memory");
+            if ((n < kC || n != table_n) && !meet(ct, limit, &ct.group)) break;
             if (n != table_n) {
                 // the decays of this chunk length (all chunks but the ragged one have the same)
                 if (r < kC / 2) ct.wb[r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (!meet(ct, limit, &ct.group)) break;
                 table_n = n;
             }
             const uint32_t tile = from + v.st * L::kStage;
 #pragma unroll 1
             for (int hf = 0; hf < L::kHalves; ++hf) {
                 // the third part of the last visit lay where the first piece goes
-                if (it > 0 && !(ok = wait_warp(ct, &ct.b_free[exact && hf == 0 ? 2 : hf], par ^ 1))) break;
+                if (it > 0 && !(ok = wait_warp(ct, limit, &ct.b_free[exact && hf == 0 ? 2 : hf], par ^ 1))) break;
                 tc_fence_after();
                 constexpr int kGroups = kC / 8 / L::kHalves;
 #pragma unroll 1
@@ -679,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             if (!ok) break;
             if (exact) {
                 // third part: b w in fp32 less the two parts, both differences exact
-                if (!wait_warp(ct, &ct.b_free[0], par)) break;
+                if (!wait_warp(ct, limit, &ct.b_free[0], par)) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int tg = 0; tg < kC / 8; tg += 4) {
@@ -707,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             // U of the chunk is complete (or of the visit: the tensor core truncates when it adds up, so an exact
             // state takes its visits one by one)
             if (v.g < share - 1 && !exact) continue;
-            if (!wait_warp(ct, &ct.b_free[exact ? 2 : L::kHalves - 1], par)) break;
+            if (!wait_warp(ct, limit, &ct.b_free[exact ? 2 : L::kHalves - 1], par)) break;
             tc_fence_after();
             const float decay = v.g == 0 || !exact ? ct.pw[n] : 1.f;
             const float2 wn = make_float2(decay, decay);
@@ -759,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         // scores of visit it: masked, decayed, to bf16 in place
         auto convert = [&](int it, const Visit& v) {
             const int n = min(kC, seg.len - offset(v));
-            if (!wait_warp(ct, &ct.p_full[p_buf(it)], p_par(it))) return false;
+            if (!wait_warp(ct, limit, &ct.p_full[p_buf(it)], p_par(it))) return false;
             tc_fence_after();
 #pragma unroll 1
             for (int jc = half; jc < 4; jc += 2) {  // blocks alternate, so that both halves have work
@@ -813,10 +845,10 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         auto scale = [&](int it, const Visit& v) {
             const int off = offset(v), n = min(kC, seg.len - off);
             const uint32_t mpar = v.m & 1;
-            if (!wait_warp(ct, &ct.scanned[v.st], v.lap)) return false;
+            if (!wait_warp(ct, limit, &ct.scanned[v.st], v.lap)) return false;
             const bool dirty = *reinterpret_cast<volatile int*>(&ct.dirty[v.st]) != 0;
             if (v.g == 0) {
-                if (!wait_warp(ct, &ct.i_full, mpar)) return false;
+                if (!wait_warp(ct, limit, &ct.i_full, mpar)) return false;
                 tc_fence_after();
                 const float rw = i < n ? jb.row_scale * ct.pw[reverse ? n - 1 - i : i + 1] : 0.f;
                 const float2 rw2 = make_float2(rw, rw);
@@ -866,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
         };
         auto finish = [&](int it, const Visit& v) {
             // every visit waits: p_ready of the next one tells the MMA thread that this product has ended
-            if (!wait_warp(ct, &ct.o_full, it & 1)) return false;
+            if (!wait_warp(ct, limit, &ct.o_full, it & 1)) return false;
             if (v.g < share - 1) return true;
             const int off = offset(v), n = min(kC, seg.len - off);
             tc_fence_after();
@@ -918,6 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
             for (int it = 0; it < n_it; ++it, next(v))
                 if (!convert(it, v) || !scale(it, v) || !finish(it, v)) break;
         }
+        tc_wait_st();  // of a visit that was given up: nothing may be under way when TMEM is freed
     }
     __syncwarp();
     tc_fence_before();
@@ -944,11 +977,11 @@ struct StateLayout {
     static_assert(kBytes <= kMaxSmem && kStages >= 2, "shared memory");
 };
 struct StateControl {
-    uint64_t full[4], empty[4], b_ready[2], b_free[2], u_free, drain;
+    uint64_t full[4], empty[4], b_ready[2], b_free[2], u_free, drain, group[2];
     uint32_t tmem;
     int dead;
     float pw[kC + 1];
-    // per group: upd_scale w^pos' of a token pair, as bf16 pairs (high and low) and in fp32
+    // upd_scale w^pos' of a token pair, as bf16 pairs (high and low) and in fp32: a whole chunk, the ragged one
     alignas(16) uint2 wb[2][kC / 2];
     alignas(16) float2 wf[2][kC / 2];
 };
@@ -964,6 +997,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
     StateControl& ct = *reinterpret_cast<StateControl*>(smem + L::kOffCtl);
     const MixParams& p = tp.p;
     const MixJob& jb = p.job[0];
+    const uint32_t limit = tp.wait_limit;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int kRegS = DC == 64 ? 152 : 208, kRegO = DC == 64 ? 144 : 112, kRegM = 64;
     const int item = blockIdx.x % p.map.n_items, hs = blockIdx.x / p.map.n_items;
@@ -980,6 +1014,8 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
         }
         mbar_init(&ct.u_free, 4);
         mbar_init(&ct.drain, 1);
+        mbar_init(&ct.group[0], 4);
+        mbar_init(&ct.group[1], 4);
         ct.dead = 0;
         mbar_fence_init();
     }
@@ -1011,7 +1047,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
         if (lane == 0) {
             int it = 0;
             for (Visit v; it < n_it; ++it, next(v)) {
-                if (it >= L::kStages && !wait(ct, &ct.empty[v.st], v.lap ^ 1)) break;
+                if (it >= L::kStages && !wait(ct, limit, &ct.empty[v.st], v.lap ^ 1)) break;
                 const uint32_t at = base + v.st * L::kStage;
                 const int t = seg.t0 + offset(v), hb = share > 1 ? hs * share + v.g : hs;
                 mbar_expect_tx(&ct.full[v.st], L::kStage);
@@ -1027,8 +1063,8 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
         Visit v;
         for (int it = 0; it < n_it; ++it, next(v)) {
             const int buf = it & 1;
-            if (!wait_warp(ct, &ct.full[v.st], v.lap) || !wait_warp(ct, &ct.b_ready[buf], (it >> 1) & 1)) break;
-            if (it > 0 && !wait_warp(ct, &ct.u_free, (it - 1) & 1)) break;
+            if (!wait_warp(ct, limit, &ct.full[v.st], v.lap) || !wait_warp(ct, limit, &ct.b_ready[buf], (it >> 1) & 1)) break;
+            if (it > 0 && !wait_warp(ct, limit, &ct.u_free, (it - 1) & 1)) break;
             tc_fence_after();
             const uint64_t c = smem_desc(base + v.st * L::kStage + L::kB, kPanel);
             const uint32_t bt = tmem + 128 + buf * 192;
@@ -1061,7 +1097,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
         for (int c = 0; c < DC; ++c) S[c] = 0.f;
         Visit v;
         for (int it = 0; it < n_it; ++it, next(v)) {
-            if (!wait_warp(ct, &ct.b_free[it & 1], (it >> 1) & 1)) break;
+            if (!wait_warp(ct, limit, &ct.b_free[it & 1], (it >> 1) & 1)) break;
             tc_fence_after();
             const float decay = v.g == 0 ? ct.pw[min(kC, seg.len - offset(v))] : 1.f;
             const float2 wn = make_float2(decay, decay);
@@ -1111,12 +1147,18 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
         const bool low = kSplit && w4 >= 2;
         const uint32_t from = base + (d0 >> 6) * kPanel + (lane & 7) * 128 +
                               ((((d0 & 63) + 8 * (lane >> 3)) * 2) ^ ((lane & 7) << 4));
-        int table_n = -1;
+        // one table for each group to fill; no warp has passed a wait yet: all eight reach this barrier
+        if (r < kC / 2) {
+            const int n = group ? seg.len % kC : kC;
+            ct.wb[group][r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
+            ct.wf[group][r] = weight_f32(ct.pw, r, n, reverse, jb.upd_scale);
+        }
+        asm volatile("bar.sync 2, 256;" ::: "memory");
         Visit v;
         for (int it = 0; it < n_it; ++it, next(v)) {
             if ((it & 1) != group) continue;
             const int n = min(kC, seg.len - offset(v));
-            if (!wait_warp(ct, &ct.full[v.st], v.lap)) break;
+            if (!wait_warp(ct, limit, &ct.full[v.st], v.lap)) break;
             if (n < kC) {
                 unsigned char* tb = smem + v.st * L::kStage;
                 for (int i = n * 8 + r; i < kC * 8; i += 128)
@@ -1126,16 +1168,9 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
                 fence_proxy_async();
             }
             // as in mix_tc_kernel: no warp reads the rows before all of them are zero
-            if (n < kC || n != table_n) asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
-            if (n != table_n) {
-                if (r < kC / 2) {
-                    ct.wb[group][r] = weight_pair(ct.pw, r, n, reverse, jb.upd_scale);
-                    ct.wf[group][r] = weight_f32(ct.pw, r, n, reverse, jb.upd_scale);
-                }
-                asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
-                table_n = n;
-            }
-            if (it > 1 && !wait_warp(ct, &ct.b_free[group], ((it >> 1) - 1) & 1)) break;
+            if (n < kC && !meet(ct, limit, &ct.group[group])) break;
+            const int tab = n < kC;
+            if (it > 1 && !wait_warp(ct, limit, &ct.b_free[group], ((it >> 1) - 1) & 1)) break;
             tc_fence_after();
             const uint32_t tile = from + v.st * L::kStage, bt = lanes + 128 + group * 192;
 #pragma unroll 1
@@ -1145,7 +1180,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     ldmatrix_t(tile + (tg + e) * 1024, f[e]);
-                    w[e] = ct.wb[group][(tg + e) * 4 + (lane & 3)];
+                    w[e] = ct.wb[tab][(tg + e) * 4 + (lane & 3)];
                 }
 #pragma unroll
                 for (int which = 0; which < 3; ++which) {
@@ -1155,7 +1190,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float2 wf = make_float2(0.f, 0.f);
-                        if (which == 2) wf = ct.wf[group][(tg + e) * 4 + (lane & 3)];
+                        if (which == 2) wf = ct.wf[tab][(tg + e) * 4 + (lane & 3)];
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
                             part[q >> 1][2 * e + (q & 1)] = kind == 2 && low ? 0u : b_part(f[e][q], w[e], wf, kind);
@@ -1255,6 +1290,7 @@ cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStr
         if (!left[j0]) continue;
         TcParams tp;
         tp.p = p;
+        tp.wait_limit = options().spin_limit < kWaitLimit ? options().spin_limit : kWaitLimit;
         tp.p.n_jobs = 0;
         tp.units = 0;
         for (int j = j0; j < p.n_jobs; ++j) {

@@ -1,0 +1,51 @@
+"""Bounded waits of the linear attention sweeps that run out: every role of the CTA leaves, the launch ends, the status
+word says so, and the next calls are right.  The limit is lowered through the library's test hook to a single poll,
+which no wait for a tile survives; nothing is made to hang."""
+
+import pytest
+import torch
+
+from pararnn_b200 import _lib
+from pararnn_b200 import attn_ops as la
+
+pytestmark = pytest.mark.gpu
+
+
+def problem(B, T, share, dk, dv, lens=None):
+    g = torch.Generator().manual_seed(T + dk + dv)
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v, do = (n(B, T, h, d).to("cuda", torch.bfloat16)
+                   for h, d in ((2 * share, dk), (2, dk), (2, dv), (2 * share, dv)))
+    cu = None if lens is None else torch.tensor([0] + lens).cumsum(0)
+    rows = B if lens is None else len(lens)
+    s0, ds = (n(rows, 2, dk, dv).cuda() for _ in range(2))
+    return (q, k, v, torch.tensor([-0.01, -0.2], device="cuda")), do, s0, ds, cu
+
+
+def run(p, want_state):
+    args, do, s0, ds, cu = p
+    r = la.linear_attention_fused(*args, s0, cu, want_state=want_state)
+    return r + la.linear_attention_reverse_vjp(*args, do, s0, ds, cu, want_state=want_state)
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (128, 64), (64, 128)])
+@pytest.mark.parametrize("want_state", [False, True])
+@pytest.mark.parametrize("shape", [dict(B=2, T=700, share=1), dict(B=1, T=2500, share=3),  # whole, in segments
+                                   dict(B=1, T=500, share=2, lens=[130, 1, 200, 169]),
+                                   dict(B=1, T=3000, share=3, lens=[2100, 900])])
+def test_a_wait_that_runs_out_ends_the_launch_and_is_reported(shape, dk, dv, want_state, prb_options):
+    lib = _lib.lib()
+    p = problem(dk=dk, dv=dv, **shape)
+    want = run(p, want_state)
+    torch.cuda.synchronize()
+    assert lib.prb_linear_attention_status(1) == 0
+    prb_options("spin_limit", 1)
+    run(p, want_state)
+    torch.cuda.synchronize()
+    prb_options("spin_limit", 0)
+    assert lib.prb_linear_attention_status(0) == 1 and lib.prb_linear_attention_status(1) == 1
+    assert lib.prb_linear_attention_status(1) == 0
+    for a, b in zip(run(p, want_state), want):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+    torch.cuda.synchronize()
+    assert lib.prb_linear_attention_status(1) == 0
