@@ -444,7 +444,8 @@ int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_h
 
 /* 0, or PRB_STATUS_CHAIN_TIMEOUT when a bounded device wait of an earlier prb_linear_attention or
  * prb_bwd_linear_attention call has run out on the current device (that call's results are not
- * valid).  Waits for the device; clear != 0 resets it. */
+ * valid).  Waits for all streams of the device, so not while one of them is being captured;
+ * clear != 0 resets it; PRB_ERR_LAUNCH when the device reports an error. */
 int prb_linear_attention_status(int clear);
 
 /* One token per row on a pool of fp32 states (slots,kv_heads,dk,dv), updated in place.  q (rows,q_heads,dk),

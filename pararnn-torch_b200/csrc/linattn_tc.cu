@@ -1321,6 +1321,8 @@ cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStr
 
 int linattn_status(int clear) {
     int v = 0;
+    // the copy alone would not wait for sweeps on non-blocking streams
+    if (cudaDeviceSynchronize() != cudaSuccess) return kErrLaunch;
     if (cudaMemcpyFromSymbol(&v, g_status, sizeof(int)) != cudaSuccess) return kErrLaunch;
     if (v && clear) {
         const int zero = 0;

@@ -134,6 +134,8 @@ def _check_attention() -> None:
         _attention_devices.discard(dev)
         with torch.cuda.device(dev):
             status = L.lib().prb_linear_attention_status(1)
+        if status < 0:
+            _raise(status, "prb_linear_attention_status")
         if status != 0:
             raise RuntimeError("pararnn_b200: a bounded device-side wait ran out in an earlier linear attention "
                                f"call on {dev} (status {status}); the results of that call are not valid")

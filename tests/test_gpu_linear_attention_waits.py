@@ -49,3 +49,20 @@ def test_a_wait_that_runs_out_ends_the_launch_and_is_reported(shape, dk, dv, wan
         assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
     torch.cuda.synchronize()
     assert lib.prb_linear_attention_status(1) == 0
+
+
+def test_the_status_waits_for_sweeps_on_other_streams(prb_options):
+    """torch's streams are non-blocking: a read on the legacy stream alone would not see what has not run yet."""
+    lib = _lib.lib()
+    p = problem(2, 700, 1, 64, 64)
+    run(p, False)
+    torch.cuda.synchronize()
+    assert lib.prb_linear_attention_status(1) == 0
+    side = torch.cuda.Stream()
+    prb_options("spin_limit", 1)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # about 10 ms
+        run(p, False)
+    prb_options("spin_limit", 0)
+    assert lib.prb_linear_attention_status(1) == 1
+    assert side.query()
