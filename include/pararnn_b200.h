@@ -447,6 +447,9 @@ int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_h
  * valid).  Waits for all streams of the device, so not while one of them is being captured;
  * clear != 0 resets it; PRB_ERR_LAUNCH when the device reports an error. */
 int prb_linear_attention_status(int clear);
+/* The same without waiting: the sweeps that have reported by now.  Reads a word of host memory, may be called
+ * at any time; the PyTorch binding does so in every call. */
+int prb_linear_attention_poll(int clear);
 
 /* One token per row on a pool of fp32 states (slots,kv_heads,dk,dv), updated in place.  q (rows,q_heads,dk),
  * k (rows,kv_heads,dk), v (rows,kv_heads,dv), out (rows,q_heads,dv) contiguous.  block_table (int32 or

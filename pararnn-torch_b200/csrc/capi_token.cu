@@ -240,6 +240,7 @@ int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_h
 }
 
 int prb_linear_attention_status(int clear) { return linattn_status(clear); }
+int prb_linear_attention_poll(int clear) { return linattn_poll(clear); }
 
 int prb_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, float* state,
                               const void* block_table, int table_is_int64, void* out, int rows, int slots, int q_heads,

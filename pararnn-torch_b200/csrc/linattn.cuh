@@ -127,8 +127,10 @@ __device__ __forceinline__ float decay_pow(double g, int n) { return n == 0 ? 1.
 cudaError_t launch_mix_simt(const MixParams& p, int dtype, bool state_only, cudaStream_t s);
 bool mix_tc_usable(const MixParams& p, int dtype);
 cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStream_t s);
-// 0, or kErrChainTimeout when a bounded wait of a tensor-core sweep has run out on this device
+// 0, or kErrChainTimeout when a bounded wait of a tensor-core sweep has run out on this device: of all sweeps
+// so far (waits for the device), of those that have reported by now
 int linattn_status(int clear);
+int linattn_poll(int clear);
 // states [item][head] from per-segment contributions (in place); s_out = state behind the last segment
 cudaError_t launch_fold_states(const MixParams& p, float* seg_states, const float* s_in, float* s_out,
                                bool reverse, cudaStream_t s);

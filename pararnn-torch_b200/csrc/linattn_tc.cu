@@ -47,9 +47,11 @@
 // resp. 40 % of the cycles.  128 tokens per chunk because tcgen05 works on 128 rows;
 // one CTA per SM because the TMEM regions and two to four stages of tiles fill one.
 //
-// Every wait has a limit; a CTA whose wait runs out raises g_status, lets its copies and matrix
+// Every wait has a limit; a CTA whose wait runs out sets the device's status word, lets its copies and matrix
 // products in flight end, frees its TMEM and leaves.
 #include <cuda_bf16.h>
+
+#include <atomic>
 
 #include "linattn.cuh"
 #include "tma.cuh"
@@ -62,8 +64,6 @@ constexpr int kC = 128;        // tokens per chunk
 constexpr int kThreads = 512;  // 4 state warps, 8 output warps, TMA, MMA, store and scan warp
 constexpr uint32_t kPanel = kC * 128;  // bytes of a 128-token x 64-channel bf16 panel
 constexpr uint32_t kWaitLimit = 1u << 22;
-
-__device__ int g_status;
 
 // ------------------------------------------------------------------------------- tcgen05 wrappers
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -197,6 +197,7 @@ struct TcParams {
     CUtensorMap map[3][4];  // [job][a, b, c, out]
     int units;              // heads of all jobs per state head
     uint32_t wait_limit;    // polls after which a wait gives up
+    int* status;            // word of the device in host memory
 };
 
 constexpr uint32_t kCtlBytes = 2048, kMaxSmem = 227 * 1024;
@@ -955,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1) mix_tc_kernel(const __grid_consta
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (tid == 0 && ct.dead) g_status = kErrChainTimeout;
+    if (tid == 0 && ct.dead) *(volatile int*)tp.status = kErrChainTimeout;
     if (warp == 13) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -1209,7 +1210,7 @@ __global__ void __launch_bounds__(kThreads, 1) state_tc_kernel(const __grid_cons
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (tid == 0 && ct.dead) g_status = kErrChainTimeout;
+    if (tid == 0 && ct.dead) *(volatile int*)tp.status = kErrChainTimeout;
     if (warp == 13) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -1229,6 +1230,31 @@ bool head_map(CUtensorMap* out, const HeadView& v, int d, int heads, int time, i
     return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(v.p), dims, strides, box, one,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Status words of the devices, in page-locked host memory that kernels on any of them can write: every call can
+// look at its device's word without a copy or a wait.
+constexpr int kDevices = 64;
+std::atomic<int*> g_status{nullptr};
+
+int* status_word(int dev) {
+    int* words = g_status.load(std::memory_order_acquire);
+    if (!words) {
+        // the first sweep may be one that is being captured
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* p = nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, kDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        for (int i = 0; i < kDevices; ++i) static_cast<int*>(p)[i] = 0;
+        // of two threads that get here at once one leaves its 256 bytes unused
+        if (g_status.compare_exchange_strong(words, static_cast<int*>(p))) words = static_cast<int*>(p);
+    }
+    return words + (dev & (kDevices - 1));
 }
 
 enum Sweep { kMix, kMixExact, kState };
@@ -1283,6 +1309,8 @@ cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStr
     cudaError_t bound = cudaGetDevice(&dev);
     if (bound == cudaSuccess) bound = cudaSetDevice(dev);
     if (bound != cudaSuccess) return bound;
+    int* const status = status_word(dev);
+    if (!status) return cudaErrorMemoryAllocation;
     // jobs of one tile shape share a launch (dq, dk and dv all do when dk and dv round up alike)
     bool left[3] = {false, false, false};
     for (int j = 0; j < p.n_jobs; ++j) left[j] = true;
@@ -1291,6 +1319,7 @@ cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStr
         TcParams tp;
         tp.p = p;
         tp.wait_limit = options().spin_limit < kWaitLimit ? options().spin_limit : kWaitLimit;
+        tp.status = status;
         tp.p.n_jobs = 0;
         tp.units = 0;
         for (int j = j0; j < p.n_jobs; ++j) {
@@ -1319,16 +1348,21 @@ cudaError_t launch_mix_tc(const MixParams& p, int rows, bool state_only, cudaStr
     return cudaSuccess;
 }
 
-int linattn_status(int clear) {
-    int v = 0;
-    // the copy alone would not wait for sweeps on non-blocking streams
-    if (cudaDeviceSynchronize() != cudaSuccess) return kErrLaunch;
-    if (cudaMemcpyFromSymbol(&v, g_status, sizeof(int)) != cudaSuccess) return kErrLaunch;
-    if (v && clear) {
-        const int zero = 0;
-        if (cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) != cudaSuccess) return kErrLaunch;
-    }
+int linattn_poll(int clear) {
+    int* const words = g_status.load(std::memory_order_acquire);
+    if (!words) return 0;  // no sweep has run
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return kErrLaunch;
+    volatile int* word = words + (dev & (kDevices - 1));
+    const int v = *word;
+    if (v && clear) *word = 0;
     return v;
+}
+
+int linattn_status(int clear) {
+    if (!g_status.load(std::memory_order_acquire)) return 0;
+    if (cudaDeviceSynchronize() != cudaSuccess) return kErrLaunch;
+    return linattn_poll(clear);
 }
 
 }  // namespace prb

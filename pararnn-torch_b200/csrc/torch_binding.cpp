@@ -71,6 +71,14 @@ Tensor heads(const Tensor& t, prb_heads& h) {
     return c;
 }
 
+// A bounded wait of an earlier sweep on the current device ran out: told by whatever call of the family comes next,
+// so that a model without any other check of the device hears of it.
+void reported(const Tensor& t) {
+    const int rc = prb_linear_attention_poll(1);
+    TORCH_CHECK(rc == PRB_OK, "pararnn_b200: a bounded device-side wait ran out in an earlier linear attention call on ",
+                t.device(), " (status ", rc, "); the results of that call are not valid");
+}
+
 struct AttnCall {
     int rows, time, n_seq, longest, hq, hkv, dk, dv, dtype;
     bool packed;
@@ -90,6 +98,7 @@ std::tuple<Tensor, Tensor> attention_fwd(const Tensor& q, const Tensor& k, const
                                          int64_t longest, double scale, bool want_state, bool sparse) {
     const AttnCall c = attn_call(q, k, v, cu_.has_value(), n_seq, longest);
     const c10::cuda::CUDAGuard guard(q.device());
+    reported(q);
     const Tensor state = plain(get(state_)), cu = get(cu_);
     prb_heads hq, hk, hv;
     const Tensor qc = heads(q, hq), kc = heads(k, hk), vc = heads(v, hv);
@@ -112,6 +121,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_bwd(const Tensor& q, const 
                                                          double scale, bool want_state, bool sparse) {
     const AttnCall c = attn_call(q, k, v, cu_.has_value(), n_seq, longest);
     const c10::cuda::CUDAGuard guard(q.device());
+    reported(q);
     const Tensor state = plain(get(state_)), gs = plain(get(grad_state_)), cu = get(cu_);
     prb_heads hq, hk, hv, hg;
     const Tensor qc = heads(q, hq), kc = heads(k, hk), vc = heads(v, hv), gc = heads(grad_.to(q.scalar_type()), hg);
@@ -198,6 +208,7 @@ void attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
     apart(state, "state", decay, "log_decay");
     apart(state, "state", get(table_), "block_table");
     const c10::cuda::CUDAGuard guard(q.device());
+    reported(q);
     const Tensor qc = q.contiguous(), kc = k.contiguous(), vc = v.contiguous(), table = plain(get(table_));
     check(prb_linear_attention_step(ptr(qc), ptr(kc), ptr(vc), (const float*)ptr(decay), (float*)ptr(state), ptr(table),
                                     table.defined() && table.scalar_type() == at::kLong, ptr(out), (int)q.size(0),

@@ -81,6 +81,7 @@ _SIGNATURES = {
     "prb_linear_attention": (_INT, [_VOIDP] * 8 + [_INT] * 9 + [_FLOAT, _VOIDP, _SIZE, _VOIDP]),
     "prb_bwd_linear_attention": (_INT, [_VOIDP] * 12 + [_INT] * 9 + [_FLOAT, _VOIDP, _SIZE, _VOIDP]),
     "prb_linear_attention_status": (_INT, [_INT]),
+    "prb_linear_attention_poll": (_INT, [_INT]),
     "prb_linear_attention_step": (_INT, [_VOIDP] * 6 + [_INT, _VOIDP] + [_INT] * 7 + [_FLOAT, _VOIDP]),
     "prb_group_norm_workspace_bytes": (_SIZE, [_LONG] + [_INT] * 5),
     "prb_group_norm": (_INT, [_VOIDP] * 5 + [_LONG] + [_INT] * 3 + [_FLOAT] + [_INT] * 3 + [_VOIDP, _SIZE, _VOIDP]),

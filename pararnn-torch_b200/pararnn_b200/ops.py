@@ -125,13 +125,15 @@ def _track_backward(sb: DeviceStats) -> None:
         del _pending_backward[0]
 
 
-# Devices on which linear attention ran since its status word was last read.
+# Devices on which linear attention has run.  Its backward pass starts in C++, and a captured one starts at
+# every replay, so a device stays on the list once it is there.
 _attention_devices: set = set()
 
 
 def _check_attention() -> None:
+    if not _attention_devices or torch.cuda.is_current_stream_capturing():
+        return  # the device cannot be waited for inside a capture
     for dev in list(_attention_devices):
-        _attention_devices.discard(dev)
         with torch.cuda.device(dev):
             status = L.lib().prb_linear_attention_status(1)
         if status < 0:
@@ -144,7 +146,9 @@ def _check_attention() -> None:
 def check_pending_backward() -> None:
     """Raise if a reverse scan (or a linear attention sweep) issued since the last check ran into a
     bounded device-side wait that gave up (its results are not valid).  One small device-to-host
-    copy per device."""
+    copy per device; where linear attention has run, a wait for the device.  Linear attention calls
+    report what earlier ones on their device left, without waiting; a program that only replays
+    graphs of them asks here."""
     _check_attention()
     if not _pending_backward:
         return

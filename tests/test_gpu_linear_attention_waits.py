@@ -39,12 +39,15 @@ def test_a_wait_that_runs_out_ends_the_launch_and_is_reported(shape, dk, dv, wan
     want = run(p, want_state)
     torch.cuda.synchronize()
     assert lib.prb_linear_attention_status(1) == 0
-    prb_options("spin_limit", 1)
-    run(p, want_state)
-    torch.cuda.synchronize()
-    prb_options("spin_limit", 0)
-    assert lib.prb_linear_attention_status(0) == 1 and lib.prb_linear_attention_status(1) == 1
-    assert lib.prb_linear_attention_status(1) == 0
+    args, do, s0, ds, cu = p
+    for call in (lambda: la.linear_attention_fused(*args, s0, cu, want_state=want_state),
+                 lambda: la.linear_attention_reverse_vjp(*args, do, s0, ds, cu, want_state=want_state)):
+        prb_options("spin_limit", 1)
+        call()
+        torch.cuda.synchronize()
+        prb_options("spin_limit", 0)
+        assert lib.prb_linear_attention_status(0) == 1 and lib.prb_linear_attention_poll(1) == 1
+        assert lib.prb_linear_attention_status(1) == 0
     for a, b in zip(run(p, want_state), want):
         assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
     torch.cuda.synchronize()
@@ -62,7 +65,52 @@ def test_the_status_waits_for_sweeps_on_other_streams(prb_options):
     prb_options("spin_limit", 1)
     with torch.cuda.stream(side):
         torch.cuda._sleep(20_000_000)  # about 10 ms
-        run(p, False)
+        la.linear_attention_fused(*p[0], p[2], want_state=False)
     prb_options("spin_limit", 0)
     assert lib.prb_linear_attention_status(1) == 1
     assert side.query()
+
+
+def fail_once(prb_options, p):
+    prb_options("spin_limit", 1)
+    la.linear_attention_fused(*p[0], p[2], want_state=False)
+    torch.cuda.synchronize()
+    prb_options("spin_limit", 0)
+
+
+def test_the_next_call_of_any_kind_reports_it(prb_options):
+    """A model of linear attention layers alone calls no other check: the next prompt, gradient or token raises, once."""
+    import pararnn_b200 as prb
+
+    p = problem(2, 700, 1, 64, 64)
+    (q, k, v, g), do, s0, ds, _ = p
+    pool = torch.zeros(2, 2, 64, 64, device="cuda")
+    leaf = q.clone().requires_grad_(True)
+    out = prb.linear_attention(leaf, k, v, g)
+    for call in (lambda: prb.linear_attention(q, k, v, g), lambda: la.linear_attention_reverse_vjp(q, k, v, g, do),
+                 lambda: prb.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, pool),
+                 lambda: torch.autograd.grad(out, [leaf], do, retain_graph=True)):
+        fail_once(prb_options, p)
+        with pytest.raises(RuntimeError, match="bounded device-side wait ran out in an earlier linear attention"):
+            call()
+        call()
+
+
+def test_replays_are_reported_by_the_check(prb_options):
+    """A graph keeps the limit that it was captured with."""
+    from pararnn_b200 import ops
+
+    p = problem(2, 700, 1, 64, 64)
+    run(p, False)
+    ops.check_pending_backward()
+    graph = torch.cuda.CUDAGraph()
+    prb_options("spin_limit", 1)
+    with torch.cuda.graph(graph):
+        la.linear_attention_fused(*p[0], p[2], want_state=False)
+        ops.check_pending_backward()  # nothing to wait for inside a capture
+    prb_options("spin_limit", 0)
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(RuntimeError, match="linear attention"):
+            ops.check_pending_backward()
+    ops.check_pending_backward()
