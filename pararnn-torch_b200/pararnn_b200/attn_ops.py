@@ -70,6 +70,8 @@ def _offsets(cu_seqlens: Tensor | None, batch: int, time: int, dev):
             raise RuntimeError("a CUDA graph needs cu_seqlens as a contiguous int32 CUDA tensor")
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
             raise ValueError(f"cu_seqlens must be (S+1,), got {tuple(cu_seqlens.shape)}")
+        if cu_seqlens.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} and {cu_seqlens.device}")
         return cu_seqlens, cu_seqlens.numel() - 1, time
     cs = validate_cu_seqlens(cu_seqlens, time)
     longest = max(b - a for a, b in zip(cs[:-1], cs[1:]))

@@ -111,3 +111,28 @@ def test_sequences_refuse_sizes_that_32_bits_would_cut(shape):
         _lib.native().attention_fwd(x, x, x, g, None, None, shape[0], shape[1], 1.0, False, False)
     with pytest.raises(ValueError, match="32 bits"):
         _lib.native().attention_bwd(x, x, x, g, x, None, None, None, shape[0], shape[1], 1.0, False, False)
+
+
+class Captured:
+    """A tensor as _offsets sees it, on a second GPU."""
+
+    is_cuda, dtype, device = True, torch.int32, torch.device("cuda", 1)
+
+    def is_contiguous(self):
+        return True
+
+    def dim(self):
+        return 1
+
+    def numel(self):
+        return 3
+
+
+def test_captured_offsets_have_to_lie_on_the_device_of_the_inputs(monkeypatch):
+    from pararnn_b200 import attn_ops
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    cu = Captured()
+    assert attn_ops._offsets(cu, 1, 5, torch.device("cuda", 1)) == (cu, 2, 5)
+    with pytest.raises(RuntimeError, match="different devices"):
+        attn_ops._offsets(cu, 1, 5, torch.device("cuda", 0))
