@@ -422,8 +422,8 @@ typedef struct prb_heads {
  *   log_decay fp32 (kv_heads); state_in / state_out fp32 (n_seq,kv_heads,dk,dv) or NULL;
  *   out (rows,time,q_heads,dv) contiguous in `dtype`.
  * cu_seqlens NULL: n_seq = rows sequences of `time` tokens.  Otherwise a packed batch: rows = 1 and
- * n_seq + 1 device int32 offsets; offsets outside [0, time] or out of order are clamped, and a
- * sequence without tokens passes its state through.  max_len bounds the sequences' lengths.
+ * n_seq + 1 device int32 offsets; an offset outside [0, time] or below an earlier one is clamped (no
+ * token is in two sequences), and a sequence without tokens passes its state through.  max_len bounds the sequences' lengths.
  * Tokens behind the last sequence are neither read nor written.  Values at later positions never
  * reach earlier outputs, not even when they are inf or NaN. */
 size_t prb_linear_attention_workspace_bytes(int rows, int time, int n_seq, int max_len, int q_heads, int kv_heads,

@@ -71,10 +71,22 @@ struct Seg {
     int row, seq, t0, len, first, last;
 };
 
-__device__ __forceinline__ void seq_span(const SegMap& m, int s, int& lo, int& hi) {
-    // offsets are clamped to the row, so that no table can send an access out of range
-    lo = min(max(m.cu[s], 0), m.time);
-    hi = min(max(m.cu[s + 1], lo), m.time);
+// Sequences s0 .. s0 + 31 of a packed batch, one for each lane of a warp (empty behind the last one).  `end` is where
+// the sequence before s0 ends; it is moved on.  An offset counts as the largest one up to it, within the row: no
+// table can send an access out of range or give a token to two sequences.
+__device__ __forceinline__ int first_token(const SegMap& m) { return min(max(m.cu[0], 0), m.time); }
+__device__ __forceinline__ void seq_spans(const SegMap& m, int s0, int& end, int& lo, int& hi) {
+    const int lane = threadIdx.x & 31;
+    hi = end;
+    if (s0 + lane < m.n_seq) hi = max(hi, min(m.cu[s0 + lane + 1], m.time));
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, hi, o);
+        if (lane >= o) hi = max(hi, v);
+    }
+    lo = __shfl_up_sync(0xffffffffu, hi, 1);
+    if (lane == 0) lo = end;
+    end = __shfl_sync(0xffffffffu, hi, 31);
 }
 
 // Item x of the grid (whole warp calls it); false when the packed batch has fewer items.
@@ -89,13 +101,11 @@ __device__ inline bool locate(const SegMap& m, int x, Seg& s) {
         return true;
     }
     const int lane = threadIdx.x & 31;
-    int base = 0;
+    int base = 0, end = first_token(m);
     for (int s0 = 0; s0 < m.n_seq; s0 += 32) {
-        int lo = 0, hi = 0, cnt = 0;
-        if (s0 + lane < m.n_seq) {
-            seq_span(m, s0 + lane, lo, hi);
-            cnt = max(1, (hi - lo + m.seg_len - 1) / m.seg_len);
-        }
+        int lo, hi, cnt = 0;
+        seq_spans(m, s0, end, lo, hi);
+        if (s0 + lane < m.n_seq) cnt = max(1, (hi - lo + m.seg_len - 1) / m.seg_len);
         int inc = cnt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

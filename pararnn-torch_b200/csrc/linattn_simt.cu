@@ -236,14 +236,18 @@ __global__ void fold_states_kernel(const __grid_constant__ MixParams p, float* s
     if (m.cu) {
         base = 0;
         const int lane = threadIdx.x & 31;
-        for (int s = lane; s < seq; s += 32) {
+        int end = first_token(m);
+        for (int s0 = 0; s0 <= seq; s0 += 32) {
             int l, h;
-            seq_span(m, s, l, h);
-            base += max(1, (h - l + m.seg_len - 1) / m.seg_len);
+            seq_spans(m, s0, end, l, h);
+            if (s0 + lane < seq) base += max(1, (h - l + m.seg_len - 1) / m.seg_len);
+            if (s0 + 32 > seq) {
+                lo = __shfl_sync(0xffffffffu, l, seq - s0);
+                hi = __shfl_sync(0xffffffffu, h, seq - s0);
+            }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
-        seq_span(m, seq, lo, hi);
         n = max(1, (hi - lo + m.seg_len - 1) / m.seg_len);
         n = max(0, min(n, m.n_items - base));
     }
