@@ -421,6 +421,7 @@ typedef struct prb_heads {
  *   q_heads a multiple of kv_heads, query head h reads state head h / (q_heads / kv_heads);
  *   log_decay fp32 (kv_heads); state_in / state_out fp32 (n_seq,kv_heads,dk,dv) or NULL;
  *   out (rows,time,q_heads,dv) contiguous in `dtype`.
+ * Outputs share no memory with inputs; state_out may be state_in where q_heads = kv_heads.
  * cu_seqlens NULL: n_seq = rows sequences of `time` tokens.  Otherwise a packed batch: rows = 1 and
  * n_seq + 1 device int32 offsets; an offset outside [0, time] or below an earlier one is clamped (no
  * token is in two sequences), and a sequence without tokens passes its state through.  max_len bounds the sequences' lengths.
@@ -435,7 +436,7 @@ int prb_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads
 
 /* Gradients from grad_out (same layout rules as q) and grad_state_out (fp32, NULL = zeros): g_q, g_k,
  * g_v contiguous in `dtype` (g_k, g_v summed over the query heads that share them), g_state fp32 or
- * NULL.  log_decay is a constant of the head. */
+ * NULL, neither state_in nor grad_state_out.  log_decay is a constant of the head. */
 int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads* v, const prb_heads* grad_out,
                              const float* log_decay, const float* state_in, const float* grad_state_out,
                              const int* cu_seqlens, void* g_q, void* g_k, void* g_v, float* g_state, int rows,

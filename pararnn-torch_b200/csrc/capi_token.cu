@@ -131,6 +131,8 @@ int prb_linear_attention(const prb_heads* q, const prb_heads* k, const prb_heads
     if (!q || !k || !v || !q->data || !k->data || !v->data || !log_decay || !out) return PRB_ERR_BAD_ARG;
     if (const int rc = check_attn(a)) return rc;
     if (cu_seqlens ? rows != 1 : rows != n_seq) return PRB_ERR_BAD_ARG;
+    // one of the query heads of a state writes it while the others may not have read it yet
+    if (state_out && state_out == state_in && q_heads != kv_heads) return PRB_ERR_BAD_ARG;
     const SegMap m = plan_segments(a, cu_seqlens, false);
     const bool seg = segmented(m);
     if (seg && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
@@ -175,6 +177,8 @@ int prb_bwd_linear_attention(const prb_heads* q, const prb_heads* k, const prb_h
         return PRB_ERR_BAD_ARG;
     if (const int rc = check_attn(a)) return rc;
     if (cu_seqlens ? rows != 1 : rows != n_seq) return PRB_ERR_BAD_ARG;
+    // the jobs of dq and dk read these while the job of dv writes
+    if (g_state && (g_state == state_in || g_state == grad_state_out)) return PRB_ERR_BAD_ARG;
     const SegMap m = plan_segments(a, cu_seqlens, true);
     const bool seg = segmented(m);
     if (seg && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||

@@ -136,3 +136,25 @@ def test_captured_offsets_have_to_lie_on_the_device_of_the_inputs(monkeypatch):
     assert attn_ops._offsets(cu, 1, 5, torch.device("cuda", 1)) == (cu, 2, 5)
     with pytest.raises(RuntimeError, match="different devices"):
         attn_ops._offsets(cu, 1, 5, torch.device("cuda", 0))
+
+
+def test_c_entry_points_refuse_states_in_place_that_others_still_read():
+    """PRB_ERR_BAD_ARG before any launch.  The sizes need a workspace that is not given, so that the calls that stay
+    allowed end in PRB_ERR_WORKSPACE instead of on a device."""
+    import ctypes
+
+    lib = _lib.lib()
+    buf = ctypes.create_string_buffer(1024)
+    p = (ctypes.addressof(buf) + 255) & ~255
+    a, b, h, T = p, p + 256, ctypes.byref(_lib.Heads(p, 1, 1, 1)), 1 << 20
+
+    def fwd(s_in, s_out, hq):
+        return lib.prb_linear_attention(h, h, h, p, s_in, None, p, s_out, 1, T, 1, T, hq, 2, 8, 8, 1, 1.0, None, 0, None)
+
+    def bwd(s_in, gs, g_state):
+        return lib.prb_bwd_linear_attention(h, h, h, h, p, s_in, gs, None, p, p, p, g_state, 1, T, 1, T, 2, 2, 8, 8, 1,
+                                            1.0, None, 0, None)
+
+    bad, ws = -1, -2
+    assert fwd(a, a, 4) == bad and fwd(a, a, 2) == ws and fwd(a, b, 4) == ws and fwd(None, None, 4) == ws
+    assert bwd(a, None, a) == bad and bwd(None, a, a) == bad and bwd(b, b, a) == ws and bwd(None, None, None) == ws
