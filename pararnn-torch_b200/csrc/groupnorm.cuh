@@ -11,14 +11,17 @@ struct GroupNormArgs {
     void *y, *dx, *dw, *db;
     float2* stats;      // (samples, groups): mean, rstd
     float* partial;     // rows of [2][channels]: sum du xhat, sum du
-    float* group_part;  // per (sample, slab, channel block, group) float4
-    long long samples, sample0;
-    int positions, channels, groups, act, w_f32, slabs;
+    float* group_part;  // float4 per (sample of the piece, slab, group, channel block of the group)
+    long long samples, sample0, sample1;  // all samples; first and end of the piece
+    int positions, channels, groups, act, w_f32, slabs, span;
     float eps;
 };
 
 struct GroupNormPlan {
     int rows, vec, nv, lanes, blocks, slabs;
+    int span;           // channel blocks that a group can touch
+    int walkers;        // CTAs per slab that share the samples of a piece (backward sums)
+    long long piece;    // samples per pair of launches
     long long part_rows;
     size_t group_floats;
 };

@@ -1,0 +1,31 @@
+"""Scratch of the group norm, on the CPU: it follows the size of the GPU and of its cache, not the number of samples."""
+
+import pytest
+
+from pararnn_b200 import _lib
+
+F32, BF16 = _lib.PRB_F32, _lib.PRB_BF16
+PIECE = 72 << 20  # bytes of samples that one pair of launches covers
+
+# samples, positions, channels, groups: rows wider than the one-pass kernels take, and many samples of few positions
+SHAPES = [(32768, 1, 2048, 1), (8192, 1, 4096, 1), (32768, 1, 1056, 32), (65536, 4, 64, 8), (4_000_000, 2, 2, 1),
+          (1_000_000, 2, 1024, 8), (500_000, 2, 512, 512), (200, 2, 65536, 32768), (100_000, 3, 999, 27),
+          (3, 50, 4400, 2), (16, 4096, 256, 32)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scratch_does_not_grow_with_the_samples(shape, dtype):
+    n, pos, c, g = shape
+    size = lambda k, back: _lib.lib().prb_group_norm_workspace_bytes(k, pos, c, g, dtype, back)  # noqa: E731
+    # rows of partial sums, two floats a channel: a wave of CTAs and a rounding, or a sixteenth of a piece
+    wide = max(2 * 296 * 2 * 4 * c, PIECE // 16)
+    for back in (0, 1):
+        assert size(n, back) <= PIECE + back * wide
+        # ten times the samples need no more than the samples that fill a piece do
+        full = max(1, PIECE // (pos * c * 2)) + 1
+        assert size(10 * max(n, full), back) <= size(max(n, full), back)
+    # and no more than the data itself once that is worth mentioning
+    data = n * pos * c * (4 if dtype == F32 else 2)
+    if data >= 16 << 20:
+        assert size(n, 1) <= 2 * data
