@@ -760,15 +760,15 @@ GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int ch
     // vectors of 16 bytes where a group holds whole ones, else of 2, else single channels
     pl.vec = cg % most == 0 ? most : cg % 2 == 0 ? 2 : 1;
     const int sm = sm_count();
-    if (positions == 1 && cg <= pl.vec * 32 * (pl.vec > 1 ? 4 : 1)) {
+    const int need = (cg + pl.vec - 1) / pl.vec;
+    pl.lanes = 1;
+    while (pl.lanes < need && pl.lanes < 32) pl.lanes *= 2;
+    const long long row_slots = (long long)groups * pl.lanes, wide = (row_slots + kT - 1) / kT;
+    // a row is at most as wide as the grid's second axis
+    if (positions == 1 && cg <= pl.vec * 32 * (pl.vec > 1 ? 4 : 1) && wide <= 65535) {
         pl.rows = 1;
-        const int need = (cg + pl.vec - 1) / pl.vec;
-        pl.lanes = 1;
-        while (pl.lanes < need && pl.lanes < 32) pl.lanes *= 2;
         pl.nv = need <= 32 ? 1 : need <= 64 ? 2 : 4;
-        const long long slots = (long long)groups * pl.lanes;
-        const long long at_once = slots >= kT ? 1 : kT / slots;
-        const long long wide = (slots + kT - 1) / kT;
+        const long long at_once = row_slots >= kT ? 1 : kT / row_slots;
         // one wave of persistent CTAs, each with one row of partial sums
         const int per_sm = pl.nv > 1 ? (backward ? 1 : 2) : backward ? kRowCtasBwd : kRowCtasFwd;
         long long ctas = (long long)sm * per_sm / wide;
@@ -791,8 +791,8 @@ GroupNormPlan groupnorm_plan(int dtype, long long samples, int positions, int ch
     want = want < 1 ? 1 : want > room ? room : want;
     pl.slabs = (int)want;
     // channel blocks of kT vectors that a group touches at most
-    const int wide = kT * pl.vec;
-    pl.span = wide % cg == 0 ? 1 : (cg + wide - 2) / wide + 1;
+    const int block = kT * pl.vec;
+    pl.span = block % cg == 0 ? 1 : (cg + block - 2) / block + 1;
     if (pl.span > pl.blocks) pl.span = pl.blocks;
     // the workspace holds one piece: neither its group sums nor the rows of partial sums grow with the samples
     const long long entries = want * groups * pl.span;

@@ -72,3 +72,20 @@ def test_samples_keep_their_bits_whatever_stands_beside_them():
     for lo, hi in ((0, 1), (65530, 65540), (65999, 66000), (100, 900)):
         for a, b in zip(run(lo, hi), whole):
             assert torch.equal(a, b[lo:hi])
+
+
+def test_a_row_of_twelve_million_channels():
+    x = torch.randn(1, 12_000_000, device="cuda", requires_grad=True)
+    y = prb.group_norm(x, 2_400_000)
+    dy = torch.randn_like(y)
+    (gx,) = torch.autograd.grad(y, [x], dy)
+    wide = x.detach().double().requires_grad_(True)
+    want = norm_oracle(wide, 2_400_000, None, None, 1e-5, None)
+    (wx,) = torch.autograd.grad(want, [wide], dy.double())
+    z = wide.detach().view(-1, 5)
+    rstd = (z.var(1, correction=0) + 1e-5).rsqrt()
+    # five terms a group, all in fp32: 2^-19 of 1 + |xhat| + |mean| rstd <= 4 + |mean| rstd; dx the same times rstd |dy|
+    lift = ((4 + z.mean(1).abs() * rstd) * 2 ** -19)[:, None]
+    assert bool(((y.detach().double() - want.detach()).view(-1, 5).abs() <= lift).all())
+    size = lift * (rstd * dy.double().view(-1, 5).abs().amax(1))[:, None] * 8
+    assert bool(((gx.double() - wx).view(-1, 5).abs() <= size).all())

@@ -29,3 +29,11 @@ def test_scratch_does_not_grow_with_the_samples(shape, dtype):
     data = n * pos * c * (4 if dtype == F32 else 2)
     if data >= 16 << 20:
         assert size(n, 1) <= 2 * data
+
+
+def test_rows_too_wide_for_the_grid_take_the_other_kernels():
+    """Five channels a group in slots of eight lanes: 75000 CTAs side by side, where a grid's second axis ends at
+    65535.  The one-pass kernels need no scratch forwards, the others do."""
+    size = lambda c, g: _lib.lib().prb_group_norm_workspace_bytes(1, 1, c, g, F32, 0)  # noqa: E731
+    assert size(12_000_000, 2_400_000) > 0
+    assert size(1_200_000, 240_000) == 0
