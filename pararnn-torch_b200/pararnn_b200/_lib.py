@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import types
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libpararnn_b200.so")
@@ -117,6 +118,10 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+NATIVE_OPS = ("attention", "attention_fwd", "attention_bwd", "attention_step", "norm", "norm_fwd", "norm_bwd", "embed",
+              "embed_fwd", "embed_bwd")
+
+
 def native():
     """The C++ operators of ``torch_binding.cpp`` (``torch.ops.pararnn_b200_native``)."""
     global _native
@@ -131,7 +136,10 @@ def native():
             torch.ops.load_library(path)
         except OSError as exc:  # pragma: no cover
             raise ExtensionMissingError(f"cannot load {path}: {exc}") from exc
-        _native = torch.ops.pararnn_b200_native
+        ops = torch.ops.pararnn_b200_native
+        # The callables behind the packets: a compiler that meets one breaks its graph and calls it, while it would
+        # trace a packet's operator with tensors that have no memory.
+        _native = types.SimpleNamespace(**{name: getattr(ops, name)._op for name in NATIVE_OPS})
     return _native
 
 
