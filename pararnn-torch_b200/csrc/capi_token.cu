@@ -276,6 +276,8 @@ static int group_norm(GroupNormArgs& a, int dtype, int weight_dtype, bool backwa
                            reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.dx);
     if (bits & 15) return PRB_ERR_BAD_ARG;
     if ((long long)a.channels > 256ll * 65535 || a.channels > (1 << 30)) return PRB_ERR_UNSUPPORTED;
+    // the kernels step over up to kT x 8 positions at once and count them in 32 bits
+    if (a.positions > 0x7fffffff - 4096) return PRB_ERR_UNSUPPORTED;
     const size_t need = prb_group_norm_workspace_bytes(a.samples, a.positions, a.channels, a.groups, dtype, backward);
     if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < need)) return PRB_ERR_WORKSPACE;
     const GroupNormPlan pl = groupnorm_plan(dtype, a.samples, a.positions, a.channels, a.groups, backward);

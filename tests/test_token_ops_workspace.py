@@ -37,3 +37,20 @@ def test_rows_too_wide_for_the_grid_take_the_other_kernels():
     size = lambda c, g: _lib.lib().prb_group_norm_workspace_bytes(1, 1, c, g, F32, 0)  # noqa: E731
     assert size(12_000_000, 2_400_000) > 0
     assert size(1_200_000, 240_000) == 0
+
+
+def c_pointer():
+    import ctypes
+
+    buf = ctypes.create_string_buffer(1024)
+    return buf, (ctypes.addressof(buf) + 255) & ~255
+
+
+def test_norm_refuses_positions_whose_steps_pass_32_bits():
+    """PRB_ERR_UNSUPPORTED before any launch; the largest size that stays allowed ends at the missing workspace."""
+    keep, p = c_pointer()
+    call = lambda n: _lib.lib().prb_group_norm(p, None, None, p, None, 1, n, 1, 1, 1e-5, 0, 1, 0, None, 0, None)  # noqa: E731
+    assert call(2 ** 31 - 1) == -3 and call(2 ** 31 - 4096) == -3 and call(2 ** 31 - 1 - 4096) == -2
+    back = lambda n: _lib.lib().prb_bwd_group_norm(p, p, None, None, p, p, None, None, 1, n, 1, 1, 0, 1, 0, None, 0,  # noqa: E731
+                                                   None)
+    assert back(2 ** 31 - 1) == -3 and back(2 ** 31 - 1 - 4096) == -2
