@@ -418,6 +418,7 @@ typedef struct prb_heads {
  * w = exp(log_decay[h]), log_decay <= 0 (-inf: no memory).  No counterpart in the reference (its
  * matrix-state cells are cells/para_m2rnn.py and cells/para_rwkv7.py).
  *   q (rows,time,q_heads,dk); k (..,kv_heads,dk); v (..,kv_heads,dv) in `dtype`; dk, dv in 1..128;
+ *   time up to 2^30;
  *   q_heads a multiple of kv_heads, query head h reads state head h / (q_heads / kv_heads);
  *   log_decay fp32 (kv_heads); state_in / state_out fp32 (n_seq,kv_heads,dk,dv) or NULL;
  *   out (rows,time,q_heads,dv) contiguous in `dtype`.

@@ -70,6 +70,7 @@ int check_attn(const AttnShape& s) {
         return PRB_ERR_BAD_ARG;
     if (s.hq % s.hkv || s.dk > kMaxHeadDim || s.dv > kMaxHeadDim) return PRB_ERR_UNSUPPORTED;
     if (s.hq > 8192 || s.hkv > 8192) return PRB_ERR_UNSUPPORTED;  // grid.y = heads x channel blocks x jobs
+    if (s.time > (1 << 30)) return PRB_ERR_UNSUPPORTED;  // a length and a segment are added in 32 bits
     return PRB_OK;
 }
 

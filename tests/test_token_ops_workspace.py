@@ -54,3 +54,17 @@ def test_norm_refuses_positions_whose_steps_pass_32_bits():
     back = lambda n: _lib.lib().prb_bwd_group_norm(p, p, None, None, p, p, None, None, 1, n, 1, 1, 0, 1, 0, None, 0,  # noqa: E731
                                                    None)
     assert back(2 ** 31 - 1) == -3 and back(2 ** 31 - 1 - 4096) == -2
+
+
+def test_attention_refuses_rows_whose_segments_pass_32_bits():
+    import ctypes
+
+    keep, p = c_pointer()
+    h = ctypes.byref(_lib.Heads(p, 1, 1, 1))
+
+    def call(n, cu):
+        return _lib.lib().prb_linear_attention(h, h, h, p, None, p if cu else None, p, None, 1, n, 1, n, 1, 1, 1, 1, 1, 1.0,
+                                               None, 0, None)
+
+    for cu in (False, True):
+        assert call(2 ** 31 - 1, cu) == -3 and call(2 ** 30 + 1, cu) == -3 and call(2 ** 30, cu) == -2
