@@ -479,7 +479,8 @@ int prb_bwd_group_norm(const void* x, const void* grad_y, const void* weight, co
 
 /* Embedding lookup out_t = scale table[id_t] and its dense gradient g_table[v] = scale sum_{id_t = v}
  * grad_out_t, added in fp32 in the order of the positions.  ids int32 or int64 (tokens); an id outside
- * [0, vocab) gives a row of zeros and takes part in no gradient.  Every row of g_table is written. */
+ * [0, vocab) gives a row of zeros and takes part in no gradient.  Every row of g_table is written.
+ * The gradient takes up to 2^31 - 2^16 tokens and ids. */
 int prb_embedding(const void* ids, int ids_is_int64, const void* table, void* out, long long tokens, int vocab,
                   int channels, int dtype, float scale, prb_stream_t stream);
 size_t prb_bwd_embedding_workspace_bytes(long long tokens, int vocab, int channels);

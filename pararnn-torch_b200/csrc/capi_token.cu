@@ -10,6 +10,9 @@ using namespace prb;
 
 namespace {
 
+// the sort adds a piece's or a block's length to counts of tokens and ids in 32 bits
+constexpr long long kMaxSorted = 0x7fff0000;
+
 bool bad_type(int dtype) { return dtype != PRB_F32 && dtype != PRB_BF16; }
 int done(cudaError_t e) { return e == cudaSuccess ? PRB_OK : PRB_ERR_LAUNCH; }
 HeadView view(const prb_heads* h) { return HeadView{h->data, h->stride_b, h->stride_t, h->stride_h}; }
@@ -338,7 +341,7 @@ int prb_embedding(const void* ids, int ids_is_int64, const void* table, void* ou
 }
 
 size_t prb_bwd_embedding_workspace_bytes(long long tokens, int vocab, int channels) {
-    if (tokens < 1 || tokens > 0x7fffffffLL || vocab < 1 || channels < 1) return 0;
+    if (tokens < 1 || tokens > kMaxSorted || vocab < 1 || vocab > kMaxSorted || channels < 1) return 0;
     return embedding_plan(tokens, vocab, channels).total;
 }
 
@@ -347,7 +350,7 @@ int prb_bwd_embedding(const void* ids, int ids_is_int64, const void* grad_out, v
                       prb_stream_t stream) {
     if (!ids || !grad_out || !g_table || tokens < 1 || vocab < 1 || channels < 1 || bad_type(dtype))
         return PRB_ERR_BAD_ARG;
-    if (tokens > 0x7fffffffLL) return PRB_ERR_UNSUPPORTED;
+    if (tokens > kMaxSorted || vocab > kMaxSorted) return PRB_ERR_UNSUPPORTED;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
         workspace_bytes < embedding_plan(tokens, vocab, channels).total)
         return PRB_ERR_WORKSPACE;

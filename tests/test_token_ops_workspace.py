@@ -68,3 +68,12 @@ def test_attention_refuses_rows_whose_segments_pass_32_bits():
 
     for cu in (False, True):
         assert call(2 ** 31 - 1, cu) == -3 and call(2 ** 30 + 1, cu) == -3 and call(2 ** 30, cu) == -2
+
+
+def test_embedding_gradient_refuses_counts_whose_sums_pass_32_bits():
+    keep, p = c_pointer()
+    most = 2 ** 31 - 2 ** 16
+    size = _lib.lib().prb_bwd_embedding_workspace_bytes
+    call = lambda n, v: _lib.lib().prb_bwd_embedding(p, 0, p, p, n, v, 1, 1, 1.0, None, 0, None)  # noqa: E731
+    assert call(most + 1, 5) == -3 and call(5, most + 1) == -3 and call(most, most) == -2
+    assert size(most + 1, 5, 1) == 0 and size(5, most + 1, 1) == 0 and size(most, most, 1) > 0
