@@ -456,7 +456,8 @@ int prb_linear_attention_poll(int clear);
 /* One token per row on a pool of fp32 states (slots,kv_heads,dk,dv), updated in place.  q (rows,q_heads,dk),
  * k (rows,kv_heads,dk), v (rows,kv_heads,dv), out (rows,q_heads,dv) contiguous.  block_table (int32 or
  * int64, NULL = row r uses slot r): a slot outside [0, slots) marks a padding row, which touches no
- * state and gives zeros; a slot named by several rows takes them in row order. */
+ * state and gives zeros; a slot named by several rows takes them in row order.  Up to 2^20 rows with a
+ * block_table, 2^30 without. */
 int prb_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, float* state,
                               const void* block_table, int table_is_int64, void* out, int rows, int slots, int q_heads,
                               int kv_heads, int dk, int dv, int dtype, float scale, prb_stream_t stream);

@@ -258,6 +258,8 @@ int prb_linear_attention_step(const void* q, const void* k, const void* v, const
         return PRB_ERR_BAD_ARG;
     if (!block_table && rows != slots) return PRB_ERR_BAD_ARG;
     if (q_heads % kv_heads || dk > kMaxHeadDim || dv > kMaxHeadDim || kv_heads > 65535) return PRB_ERR_UNSUPPORTED;
+    // every CTA looks for other rows of its slot: the time of a table grows with the square of its rows
+    if (rows > (block_table ? 1 << 20 : 1 << 30)) return PRB_ERR_UNSUPPORTED;
     StepArgs a{q, k, v, log_decay, state, block_table, out, rows, slots, q_heads, kv_heads, dk, dv, table_is_int64,
                scale};
     return done(launch_linattn_step(a, dtype, (cudaStream_t)stream));

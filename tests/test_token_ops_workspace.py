@@ -77,3 +77,14 @@ def test_embedding_gradient_refuses_counts_whose_sums_pass_32_bits():
     call = lambda n, v: _lib.lib().prb_bwd_embedding(p, 0, p, p, n, v, 1, 1, 1.0, None, 0, None)  # noqa: E731
     assert call(most + 1, 5) == -3 and call(5, most + 1) == -3 and call(most, most) == -2
     assert size(most + 1, 5, 1) == 0 and size(5, most + 1, 1) == 0 and size(most, most, 1) > 0
+
+
+def test_step_refuses_tables_that_it_would_search_for_minutes():
+    """Refusals only: a call that is allowed would go to the device."""
+    keep, p = c_pointer()
+
+    def call(rows, table):
+        return _lib.lib().prb_linear_attention_step(p, p, p, p, p, p if table else None, 0, p, rows, rows, 1, 1, 1, 1, 0,
+                                                    1.0, None)
+
+    assert call(2 ** 20 + 1, True) == -3 and call(2 ** 31 - 1, True) == -3 and call(2 ** 30 + 1, False) == -3
