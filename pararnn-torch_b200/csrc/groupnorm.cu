@@ -12,9 +12,11 @@
 //          lanes, mean and variance are two register passes, the data moves exactly once.
 //   slabs  everything else: a first launch leaves each slab's (mean, M2) or (sum du, sum du xhat) per
 //          group, a second one merges them and writes the result; it finds the data still in L2
-//          because the host walks the samples in pieces of at most kPieceBytes.
-// Variances are merged as (count, mean, M2), never as sums of squares, and all partial sums are
-// added in a fixed order, so results repeat bit for bit.
+//          because the host walks the samples in pieces of at most kPieceBytes.  Backwards a CTA of the
+//          first launch walks several samples, so that dw and db need as many partial rows as CTAs.
+// Squares are only ever summed about the mean of their own batch of positions, never about zero or about a chosen
+// value; batches, threads, slabs and channel blocks are joined as (count, mean, M2).  All partial sums are added
+// in a fixed order, so results repeat bit for bit.
 #include <type_traits>
 
 #include "groupnorm.cuh"
@@ -417,12 +419,10 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_stats(const __grid_cons
     const SlabSlot s = slab_slot<V>(p);
     const size_t n = p.sample0 + blockIdx.y;
     const T* x = reinterpret_cast<const T*>(p.x) + n * p.positions * p.channels + s.c;
-    // sums about the thread's first value, so that a large mean cancels nothing
+    // each batch's mean first, then its squares about that mean; batches are joined as (count, mean, M2)
     using E = Elem<V>;
-    E t1 = all<E>(0.f), t2 = all<E>(0.f);
-    float pivot = 0.f, cnt = 0.f;
-    if (s.live && s.p0 + s.sub < s.p1) {
-        pivot = static_cast<float>(x[(size_t)(s.p0 + s.sub) * p.channels]);
+    float cnt = 0.f, mean = 0.f, m2 = 0.f;
+    if (s.live) {
         for (int q0 = s.p0 + s.sub; q0 < s.p1; q0 += kBatch * s.rows) {
             Pack<T, V> raw[kBatch];
 #pragma unroll
@@ -430,25 +430,37 @@ __global__ void __launch_bounds__(kT, kSlabCtas) gn_slab_stats(const __grid_cons
                 const int q = min(q0 + e * s.rows, s.p1 - 1);
                 raw[e] = load_raw<T, V>(x + (size_t)q * p.channels);
             }
+            const int here = min(kBatch, (s.p1 - q0 + s.rows - 1) / s.rows);
+            E t1 = all<E>(0.f), t2 = all<E>(0.f);
 #pragma unroll
             for (int e = 0; e < kBatch; ++e) {
-                if (q0 + e * s.rows >= s.p1) break;
+                if (e >= here) break;
+                Vals<V> v;
+                unpack<T, V>(v, raw[e]);
+#pragma unroll
+                for (int i = 0; i < kN<V>; ++i) t1 = op_add(t1, v.a[i]);
+            }
+            const float n = (float)(here * V), m = total(t1) / n;
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                if (e >= here) break;
                 Vals<V> v;
                 unpack<T, V>(v, raw[e]);
 #pragma unroll
                 for (int i = 0; i < kN<V>; ++i) {
-                    const E d = op_add(v.a[i], all<E>(-pivot));
-                    t1 = op_add(t1, d);
+                    const E d = op_add(v.a[i], all<E>(-m));
                     t2 = op_fma(d, d, t2);
                 }
-                cnt += V;
             }
+            const float d = m - mean, part = n / (cnt + n);
+            m2 += fmaf(d * (cnt * part), d, total(t2));
+            mean = fmaf(d, part, mean);
+            cnt += n;
         }
     }
-    const float s1 = total(t1), s2 = total(t2), m = cnt > 0.f ? s1 / cnt : 0.f;
     sn[threadIdx.x] = cnt;
-    sm[threadIdx.x] = pivot + m;
-    sv[threadIdx.x] = cnt > 0.f ? fmaxf(s2 - s1 * m, 0.f) + 0.f * s2 : 0.f;
+    sm[threadIdx.x] = mean;
+    sv[threadIdx.x] = m2;
     __syncthreads();
     int g0, ng;
     local_groups<V>(p, g0, ng);
