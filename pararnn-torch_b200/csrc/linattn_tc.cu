@@ -16,6 +16,7 @@
 // stores the output tile with TMA out of the stage whose a and b it has replaced; warp 15 looks for
 // inf and NaN in c.  The state rows take up to 128 registers a thread, so the warpgroups trade
 // registers (setmaxnreg).
+// The compiler still plans with the 128 registers of the launch: 8 of the 12 instances spill 40 - 112 bytes.
 //
 // Roundings: the scores and the state are rounded to bf16 once as operands, 2^-9 each, which is
 // what the bf16 output loses anyway.  The decayed b^T is split into two bf16 parts (2^-17), since the state
@@ -40,8 +41,8 @@
 // on the tensor cores; its rows are summed over the positions that they may see (row_mix),
 // so that nothing behind the mask can reach them.
 //
-// Measured: forward 16 x 4096, 8 heads of 64: 77 us, 16 x 2048, 8 heads of 128: 59 us, against 41 us of memory traffic
-// at the copy rate for both; with backward 294 and 224 against 82 (its three jobs read 9 inputs where one
+// Measured: forward 16 x 4096, 8 heads of 64: 77 us, 16 x 2048, 8 heads of 128: 60 us, against 41 us of memory traffic
+// at the copy rate for both; with backward 294 and 226 against 82 (its three jobs read 9 inputs where one
 // pass would read 4).  A chunk takes 2.4 resp. 3.7 us (time over chunks, start-up included) where the copy rate
 // would allow 1.3 resp. 2.6: the MMA warp's walk over the barriers, with the tensor pipe active for 22
 // resp. 40 % of the cycles.  128 tokens per chunk because tcgen05 works on 128 rows;
